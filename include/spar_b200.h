@@ -348,6 +348,136 @@ struct SparCudaStatus spar_b200_attention_backward_gqa(
     uint64_t kv_heads, uint64_t head_dim, const float* rope_table, int device, void* stream);
 /* As spar_b200_gemm_error, for the attention kernels' bounded waits. */
 int spar_b200_attention_error(int device, int clear);
+
+/* ------------------------------------------------------------------------------------------ */
+/* Rotary positions on queries and keys addressed as [batch, seq, heads, head_dim] views, and   */
+/* the per-head RMSNorm of queries and keys with the rotation in the same pass.                 */
+/*                                                                                              */
+/* Element types of the operators below; weights, tables and statistics are always fp32.        */
+enum SparB200Element {
+  SPAR_B200_FLOAT32 = 0,
+  SPAR_B200_BFLOAT16 = 1,
+};
+/* How a table of angles is scaled for contexts longer than the model was trained on.           */
+/* With f_i = theta^(-2i/D), i < D/2, the angle of pair i per position:                         */
+/*   NONE    f_i                                                                                */
+/*   LINEAR  f_i / factor (position interpolation)                                              */
+/*   BASE    (theta * factor^(D / (D - 2)))^(-2i/D) (a larger base: the slowest pair is          */
+/*           stretched by factor, the fastest kept; D > 2)                                       */
+/*   PARTS   g f_i + (1 - g) f_i / factor, g = clamp((r_i - slow_turns) / (fast_turns -          */
+/*           slow_turns), 0, 1), r_i = original_length f_i / (2 pi) the turns pair i makes over  */
+/*           the trained context; cos and sin times `magnitude` (interpolation by parts, Peng    */
+/*           et al. 2023)                                                                        */
+enum SparB200RotaryScalingKind {
+  SPAR_B200_ROTARY_NONE = 0,
+  SPAR_B200_ROTARY_LINEAR = 1,
+  SPAR_B200_ROTARY_BASE = 2,
+  SPAR_B200_ROTARY_PARTS = 3,
+};
+struct SparB200RotaryScaling {
+  int kind;               /* SparB200RotaryScalingKind */
+  double factor;          /* > 0 (kinds other than NONE) */
+  double original_length; /* PARTS: trained context, > 0 */
+  double fast_turns;      /* PARTS: pairs above this many turns are kept (32 in the paper) */
+  double slow_turns;      /* PARTS: pairs below this many are interpolated (1); < fast_turns */
+  double magnitude;       /* factor on cos and sin; 0: 0.1 ln(factor) + 1 for PARTS with        */
+                          /* factor > 1, 1 otherwise                                            */
+};
+/* table[r, i] = magnitude * (cos, sin)((start + r) * angle_i) for r < rows, i < rotary_dim / 2;  */
+/* angles in double, results rounded to fp32. `scaling` NULL means NONE.                        */
+struct SparCudaStatus spar_b200_rotary_table(float* table, uint64_t rows, uint64_t rotary_dim,
+                                             double theta, uint64_t start,
+                                             const struct SparB200RotaryScaling* scaling,
+                                             int device, void* stream);
+
+enum SparB200RotaryLayout {
+  SPAR_B200_ROTARY_INTERLEAVED = 0, /* pair i is elements 2i and 2i + 1 (spar_b200_rope_apply) */
+  SPAR_B200_ROTARY_HALF = 1,        /* pair i is elements i and i + rotary_dim / 2 */
+};
+/* A strided view of heads: element (b, t, h, e) at data + b*batch + t*token + h*head + e.       */
+struct SparB200Heads {
+  void* data;
+  uint64_t batch, token, head; /* strides in elements */
+};
+struct SparB200Rotary {
+  int dtype;  /* SparB200Element of q, k and their outputs */
+  int layout; /* SparB200RotaryLayout */
+  int inverse; /* rotate: 1 turns back (the backward pass of the rotation) */
+  uint64_t batch, seq, heads, kv_heads; /* k has kv_heads heads; 0: there is no k */
+  uint64_t head_dim;   /* 1 .. 256 */
+  uint64_t rotary_dim; /* even, 2 .. head_dim: the first rotary_dim elements of a head turn, the */
+                       /* others pass                                                           */
+  const float* table;  /* [table_rows, rotary_dim / 2] (cos, sin) */
+  uint64_t table_rows;
+  const int32_t* positions; /* [batch, seq] table rows of the tokens; NULL: token t of every     */
+  uint64_t start;           /* sequence has row start + t                                        */
+  int32_t* invalid; /* optional: set to 1 when a position lies outside the table; that token's   */
+                    /* outputs are zeros and it adds nothing to a weight gradient                */
+  struct SparB200Heads q, k;         /* inputs */
+  struct SparB200Heads q_out, k_out; /* outputs; may be the inputs themselves (same strides) */
+  /* norms of queries and keys */
+  const float* q_weight; /* [head_dim] */
+  const float* k_weight; /* [head_dim] */
+  double epsilon;
+  /* their backward: gradients of the forward's outputs, weight gradients, scratch */
+  struct SparB200Heads dq, dk;
+  float* dq_weight; /* [head_dim] */
+  float* dk_weight;
+  int accumulate; /* 1: add to dq_weight and dk_weight instead of overwriting them */
+  void* scratch;  /* spar_b200_qk_norm_rotary_scratch_bytes(head_dim, device) bytes, 16-byte     */
+                  /* aligned                                                                     */
+};
+/* q_out, k_out = q, k rotated (inverse: rotated back). batch * seq * (heads + kv_heads) must be */
+/* below 2^31. Any strides and alignment of whole elements are taken; 16-byte aligned rows with  */
+/* rotary_dim a multiple of 8 (fp32) or 16 (bf16) and head_dim of 4 / 8 run vectorised.          */
+struct SparCudaStatus spar_b200_rotary(const struct SparB200Rotary* r, int device, void* stream);
+/* q_out = rotate(q / sqrt(mean(q^2) + epsilon) * q_weight) per head, and k likewise: qk-norm    */
+/* (reference src/nn/attention.cpp:183-186, 208-215; src/nn/rmsnorm.cpp:50-52) and the rotation  */
+/* in one pass, one rounding at the end. `inverse` is not read.                                 */
+struct SparCudaStatus spar_b200_qk_norm_rotary_forward(const struct SparB200Rotary* r, int device,
+                                                       void* stream);
+/* Its backward: from dq, dk (gradients of the forward's outputs) and the forward's inputs q, k   */
+/* the gradients q_out, k_out of q, k (may be dq, dk themselves) and the weight gradients, which  */
+/* are summed in a fixed order (deterministic). With zero tokens the weight gradients are zeros   */
+/* (or left alone, accumulate = 1).                                                             */
+uint64_t spar_b200_qk_norm_rotary_scratch_bytes(uint64_t head_dim, int device);
+struct SparCudaStatus spar_b200_qk_norm_rotary_backward(const struct SparB200Rotary* r, int device,
+                                                        void* stream);
+
+/* ------------------------------------------------------------------------------------------ */
+/* Causal attention with a sliding window and a few first tokens that stay visible ("sinks").   */
+/* Query head h reads key / value head h / (heads / kv_heads). Row i of sequence b stands at     */
+/* position p = first[b] + i and sees key j of its sequence iff                                  */
+/*   j <= p  and  (j > p - window  or  j < sinks)  and  j < lengths[b]  and  p < lengths[b].     */
+/*   out = softmax(scale q k^T over the visible keys) v,  lse = ln sum exp(scale q k^T).         */
+/* A row that sees nothing (padding behind lengths[b], a position below 0) gives zeros, lse =    */
+/* -infinity, and no gradient. Keys and values at or behind lengths[b] reach no result, whatever */
+/* they hold (a cache's unused slots may hold NaN). A NaN or infinity in a key or value below    */
+/* lengths[b] may also reach rows near those that see it.                                        */
+struct SparB200WindowAttention {
+  int dtype; /* SparB200Element of q, k, v, out and the gradients */
+  uint64_t batch, q_len, kv_len, heads, kv_heads;
+  uint64_t head_dim; /* 1 .. 256 */
+  uint64_t window;   /* >= 1; at least kv_len: plain causal attention */
+  uint64_t sinks;
+  double scale; /* > 0, or 0 for 1 / sqrt(head_dim) */
+  const int32_t* lengths; /* [batch] keys of each sequence, clamped to 0 .. kv_len; NULL: kv_len */
+  const int32_t* first;   /* [batch] position of each sequence's row 0; NULL: kv_len - q_len    */
+  struct SparB200Heads q, k, v, out;
+  float* lse; /* [batch, heads, q_len]; the forward may be given NULL */
+  /* backward */
+  struct SparB200Heads dout, dq, dk, dv;
+  void* scratch; /* spar_b200_window_attention_scratch_bytes bytes, 256-byte aligned */
+};
+/* Scratch bytes of the forward (backward = 0) or backward (1) of this call on `device`.         */
+uint64_t spar_b200_window_attention_scratch_bytes(const struct SparB200WindowAttention* w,
+                                                  int backward, int device);
+struct SparCudaStatus spar_b200_window_attention_forward(const struct SparB200WindowAttention* w,
+                                                         int device, void* stream);
+/* dq, dk, dv (every element written) from dout and the forward's q, k, v, out and lse;          */
+/* deterministic: dk, dv are sums over the head group in a fixed order.                         */
+struct SparCudaStatus spar_b200_window_attention_backward(const struct SparB200WindowAttention* w,
+                                                          int device, void* stream);
 /* Host-side fault injection for tests of the error path (no counterpart in the reference): sets  */
 /* (value != 0) or clears the bounded-wait flag of the GEMM (kernel 0) or attention (kernel 1)    */
 /* kernels on `device` without running a kernel. A training step that finds either flag set      */

@@ -57,6 +57,46 @@ class SparB200LMConfig(ctypes.Structure):
     ]
 
 
+def _heads(*names):
+    """Fields of consecutive SparB200Heads members (data, batch, token and head strides)."""
+    return [(name + part, kind) for name in names
+            for part, kind in (("", c_void_p), ("_batch", c_uint64), ("_token", c_uint64),
+                               ("_head", c_uint64))]
+
+
+class SparB200RotaryScaling(ctypes.Structure):
+    _fields_ = [("kind", c_int), ("factor", c_double), ("original_length", c_double),
+                ("fast_turns", c_double), ("slow_turns", c_double), ("magnitude", c_double)]
+
+
+class SparB200Rotary(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int), ("layout", c_int), ("inverse", c_int),
+        ("batch", c_uint64), ("seq", c_uint64), ("heads", c_uint64), ("kv_heads", c_uint64),
+        ("head_dim", c_uint64), ("rotary_dim", c_uint64),
+        ("table", c_void_p), ("table_rows", c_uint64), ("positions", c_void_p),
+        ("start", c_uint64), ("invalid", c_void_p),
+        *_heads("q", "k", "q_out", "k_out"),
+        ("q_weight", c_void_p), ("k_weight", c_void_p), ("epsilon", c_double),
+        *_heads("dq", "dk"),
+        ("dq_weight", c_void_p), ("dk_weight", c_void_p), ("accumulate", c_int),
+        ("scratch", c_void_p),
+    ]
+
+
+class SparB200WindowAttention(ctypes.Structure):
+    _fields_ = [
+        ("dtype", c_int),
+        ("batch", c_uint64), ("q_len", c_uint64), ("kv_len", c_uint64), ("heads", c_uint64),
+        ("kv_heads", c_uint64), ("head_dim", c_uint64), ("window", c_uint64), ("sinks", c_uint64),
+        ("scale", c_double), ("lengths", c_void_p), ("first", c_void_p),
+        *_heads("q", "k", "v", "out"),
+        ("lse", c_void_p),
+        *_heads("dout", "dq", "dk", "dv"),
+        ("scratch", c_void_p),
+    ]
+
+
 S = SparCudaStatus
 p, u64, i, d, f = c_void_p, c_uint64, c_int, c_double, c_float
 
@@ -86,6 +126,14 @@ SIGNATURES = {
     "spar_b200_column_sum": (S, [p, p, u64, u64, u64, i, i, p]),
     "spar_b200_rope_table": (S, [p, u64, u64, d, u64, i, p]),
     "spar_b200_rope_apply": (S, [p, p, u64, u64, u64, u64, u64, i, i, p]),
+    "spar_b200_rotary_table": (S, [p, u64, u64, d, u64, POINTER(SparB200RotaryScaling), i, p]),
+    "spar_b200_rotary": (S, [POINTER(SparB200Rotary), i, p]),
+    "spar_b200_qk_norm_rotary_forward": (S, [POINTER(SparB200Rotary), i, p]),
+    "spar_b200_qk_norm_rotary_scratch_bytes": (u64, [u64, i]),
+    "spar_b200_qk_norm_rotary_backward": (S, [POINTER(SparB200Rotary), i, p]),
+    "spar_b200_window_attention_scratch_bytes": (u64, [POINTER(SparB200WindowAttention), i, i]),
+    "spar_b200_window_attention_forward": (S, [POINTER(SparB200WindowAttention), i, p]),
+    "spar_b200_window_attention_backward": (S, [POINTER(SparB200WindowAttention), i, p]),
     "spar_b200_gemm": (S, [POINTER(SparB200Gemm), i, p]),
     "spar_b200_gemm_error": (c_int, [i, i]),
     "spar_b200_matmul": (S, [p, p, p, u64, u64, u64, u64, i, i, i, p]),

@@ -34,6 +34,8 @@ SOURCES = [
     "checkpoint.cpp",
     "batches.cu",
     "qknorm.cu",
+    "rotary.cu",
+    "window_attention.cu",
 ]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

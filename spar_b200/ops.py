@@ -8,11 +8,13 @@ libspar_b200.so on torch's current stream.
 from __future__ import annotations
 
 import ctypes
+from dataclasses import dataclass
 
 import torch
 
 from . import _lib
-from ._lib import SparB200Gemm, SparB200TensorSlice, call
+from ._lib import (SparB200Gemm, SparB200Rotary, SparB200RotaryScaling, SparB200TensorSlice,
+                   SparB200WindowAttention, call)
 
 TF32, TF32X3 = 0, 1
 EPI_NONE, EPI_BIAS, EPI_BIAS_GELU, EPI_GELU_BWD, EPI_BIAS_ADD = 0, 1, 2, 3, 4
@@ -321,6 +323,220 @@ def rope_apply_(x, table, batch: int, t: int, heads: int, d: int, ld: int, inver
     call("spar_b200_rope_apply", x.data_ptr(), table.data_ptr(), batch, t, heads, d, ld,
          int(inverse), _dev(x), _stream(x))
     return x
+
+
+# ------------------------------------------------------------------------------- rotary positions
+_ELEMENT = {torch.float32: 0, torch.bfloat16: 1}
+_ROTARY_LAYOUT = {"interleaved": 0, "half": 1}
+_ROTARY_SCALING = {"none": 0, "linear": 1, "base": 2, "parts": 3}
+_NO_HEADS = (None, 0, 0, 0)
+
+
+def _heads_view(t, name, like=None, shape=None):
+    """(pointer, batch, token, head strides) of a [batch, tokens, heads, head_dim] view whose head
+    elements are contiguous; `like` gives the type and device it must have."""
+    if t.dim() != 4 or t.dtype not in _ELEMENT:
+        raise ValueError(f"{name} must be a 4-D float32 or bfloat16 tensor [batch, tokens, heads, "
+                         "head_dim]")
+    if not t.is_cuda:
+        raise ValueError("spar_b200 ops take CUDA tensors")
+    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+        raise ValueError(f"{name} must have the type and device of the other tensors")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}")
+    batch, token, head, element = t.stride()
+    if element != 1 and t.shape[3] != 1:
+        raise ValueError(f"the elements of a head of {name} must be contiguous")
+    return t.data_ptr(), batch, token, head
+
+
+def _small(t, name, dtype, shape, like):
+    """Pointer of an optional contiguous tensor of the given type and shape on like's device."""
+    if t is None:
+        return None
+    if t.dtype != dtype or tuple(t.shape) != shape or t.device != like.device or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on the "
+                         "device of the other tensors")
+    return t.data_ptr()
+
+
+@dataclass(frozen=True)
+class RotaryScaling:
+    """How rotary_table scales angles for contexts longer than `original_length`: "linear"
+    (position interpolation), "base" (a larger theta) or "parts" (interpolation by parts: pairs of
+    more than fast_turns turns over the original length kept, of less than slow_turns divided by
+    `factor`). `magnitude` multiplies cos and sin; None: 0.1 ln(factor) + 1 for "parts", else 1."""
+    kind: str
+    factor: float
+    original_length: float = 0.0
+    fast_turns: float = 32.0
+    slow_turns: float = 1.0
+    magnitude: float | None = None
+
+
+def rotary_table(rows: int, rotary_dim: int, theta: float = 10000.0, start: int = 0,
+                 scaling: RotaryScaling | None = None, device=None):
+    """[rows, rotary_dim / 2, 2] cos and sin of positions start .. start + rows - 1."""
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise ValueError("spar_b200 ops take CUDA tensors")
+    if rows < 0 or start < 0 or rotary_dim < 2:
+        raise ValueError("rows and start must not be negative, rotary_dim at least 2")
+    c = None
+    if scaling is not None:
+        if scaling.kind not in _ROTARY_SCALING:
+            raise ValueError(f"scaling kind must be one of {list(_ROTARY_SCALING)}")
+        c = SparB200RotaryScaling(_ROTARY_SCALING[scaling.kind], scaling.factor,
+                                  scaling.original_length, scaling.fast_turns, scaling.slow_turns,
+                                  scaling.magnitude or 0.0)
+    table = torch.empty(rows, rotary_dim // 2, 2, device=device, dtype=torch.float32)
+    call("spar_b200_rotary_table", table.data_ptr(), rows, rotary_dim, theta, start,
+         None if c is None else ctypes.byref(c), _dev(table), _stream(table))
+    return table
+
+
+def _rotary_desc(q, k, table, layout, inverse, positions, start, invalid, q_out, k_out, q_weight=None,
+                 k_weight=None, eps=0.0, dq=None, dk=None, dq_weight=None, dk_weight=None,
+                 accumulate=False, scratch=None):
+    qv = _heads_view(q, "q")
+    batch, seq, heads, dim = q.shape
+    kv_heads, kv = 0, _NO_HEADS
+    if k is not None:
+        kv = _heads_view(k, "k", q)
+        kv_heads = k.shape[2]
+        if k.shape[0] != batch or k.shape[1] != seq or k.shape[3] != dim:
+            raise ValueError("k must have the batch, tokens and head_dim of q")
+    if layout not in _ROTARY_LAYOUT:
+        raise ValueError(f"layout must be one of {list(_ROTARY_LAYOUT)}")
+    if table.dim() != 3 or start < 0:
+        raise ValueError("table must be [rows, rotary_dim / 2, 2] and start not negative")
+    rows, pairs, _ = table.shape
+    k_views = [_NO_HEADS if k is None else _heads_view(t, name, q, k.shape) if t is not None else _NO_HEADS
+               for t, name in ((k_out, "k_out"), (dk, "dk"))]
+    return SparB200Rotary(
+        _ELEMENT[q.dtype], _ROTARY_LAYOUT[layout], int(inverse), batch, seq, heads, kv_heads, dim,
+        2 * pairs, _small(table, "table", torch.float32, (rows, pairs, 2), q), rows,
+        _small(positions, "positions", torch.int32, (batch, seq), q), start,
+        _small(invalid, "invalid", torch.int32, (1,), q), *qv, *kv,
+        *_heads_view(q_out, "q_out", q, q.shape), *k_views[0],
+        _small(q_weight, "q_weight", torch.float32, (dim,), q),
+        _small(k_weight, "k_weight", torch.float32, (dim,), q), eps,
+        *(_NO_HEADS if dq is None else _heads_view(dq, "dq", q, q.shape)), *k_views[1],
+        _small(dq_weight, "dq_weight", torch.float32, (dim,), q),
+        _small(dk_weight, "dk_weight", torch.float32, (dim,), q), int(accumulate), _ptr(scratch))
+
+
+def _like(t, out):
+    if out is not None or t is None:
+        return out
+    return torch.empty(t.shape, device=t.device, dtype=t.dtype)
+
+
+def rotary(q, k, table, *, layout: str = "interleaved", positions=None, start: int = 0,
+           inverse: bool = False, q_out=None, k_out=None, invalid=None):
+    """q and k (or q alone, k None), [batch, tokens, heads, head_dim] views, with the first
+    rotary_dim elements of every head rotated by the table row of their token: positions
+    [batch, tokens] int32, or start + t. inverse turns back (the backward pass). q_out=q rotates in
+    place. `invalid` (int32 [1]) is set to 1 by a position outside the table (outputs zeros)."""
+    q_out, k_out = _like(q, q_out), _like(k, k_out)
+    desc = _rotary_desc(q, k, table, layout, inverse, positions, start, invalid, q_out, k_out)
+    call("spar_b200_rotary", ctypes.byref(desc), _dev(q), _stream(q))
+    return q_out, k_out
+
+
+def qk_norm_rotary_forward(q, k, q_weight, k_weight, table, eps: float = 1e-6, *,
+                           layout: str = "interleaved", positions=None, start: int = 0, q_out=None,
+                           k_out=None, invalid=None):
+    """RMSNorm of every query and key head (weights [head_dim], float32) and the rotation of
+    `rotary`, in one pass."""
+    q_out, k_out = _like(q, q_out), _like(k, k_out)
+    desc = _rotary_desc(q, k, table, layout, False, positions, start, invalid, q_out, k_out, q_weight,
+                        k_weight, eps)
+    call("spar_b200_qk_norm_rotary_forward", ctypes.byref(desc), _dev(q), _stream(q))
+    return q_out, k_out
+
+
+def qk_norm_rotary_backward(dq_out, dk_out, q, k, q_weight, k_weight, table, eps: float = 1e-6, *,
+                            layout: str = "interleaved", positions=None, start: int = 0, dq=None,
+                            dk=None, dq_weight=None, dk_weight=None, accumulate_params: bool = False,
+                            invalid=None):
+    """(dq, dk, dq_weight, dk_weight) of qk_norm_rotary_forward from the gradients of its outputs and
+    its inputs; dq=dq_out writes in place. accumulate_params adds to the weight gradients given."""
+    dq, dk = _like(q, dq), _like(k, dk)
+    if accumulate_params and (dq_weight is None or (k is not None and dk_weight is None)):
+        raise ValueError("accumulate_params adds to weight gradients that must be given")
+    dim = q.shape[-1]
+    if dq_weight is None:
+        dq_weight = torch.empty(dim, device=q.device, dtype=torch.float32)
+    if dk_weight is None and k is not None:
+        dk_weight = torch.empty(dim, device=q.device, dtype=torch.float32)
+    nbytes = _lib.load().spar_b200_qk_norm_rotary_scratch_bytes(dim, _dev(q))
+    scratch = torch.empty(max(nbytes, 16), device=q.device, dtype=torch.uint8)
+    desc = _rotary_desc(q, k, table, layout, False, positions, start, invalid, dq, dk, q_weight,
+                        k_weight, eps, dq_out, dk_out, dq_weight, dk_weight, accumulate_params, scratch)
+    call("spar_b200_qk_norm_rotary_backward", ctypes.byref(desc), _dev(q), _stream(q))
+    return dq, dk, dq_weight, dk_weight
+
+
+# ------------------------------------------------------------------------------- window attention
+def _window_desc(q, k, v, out, lse, window, sinks, scale, lengths, first, dout=None, dq=None, dk=None,
+                 dv=None):
+    qv = _heads_view(q, "q")
+    batch, q_len, heads, dim = q.shape
+    if k.dim() != 4:
+        raise ValueError("k must be a 4-D float32 or bfloat16 tensor [batch, tokens, heads, head_dim]")
+    kv_len, kv_heads = k.shape[1], k.shape[2]
+    if k.shape[0] != batch or k.shape[3] != dim or kv_heads < 1 or heads % kv_heads:
+        raise ValueError("k must have the batch and head_dim of q and a number of heads that divides q's")
+    if window < 1 or sinks < 0:
+        raise ValueError("window must be at least 1 and sinks not negative")
+    if scale is not None and not scale > 0.0:
+        raise ValueError("scale must be positive")
+    back = _NO_HEADS * 4
+    if dout is not None:
+        back = (*_heads_view(dout, "dout", q, q.shape), *_heads_view(dq, "dq", q, q.shape),
+                *_heads_view(dk, "dk", q, k.shape), *_heads_view(dv, "dv", q, k.shape))
+    return SparB200WindowAttention(
+        _ELEMENT[q.dtype], batch, q_len, kv_len, heads, kv_heads, dim, window, sinks, scale or 0.0,
+        _small(lengths, "lengths", torch.int32, (batch,), q),
+        _small(first, "first", torch.int32, (batch,), q), *qv, *_heads_view(k, "k", q),
+        *_heads_view(v, "v", q, k.shape), *_heads_view(out, "out", q, q.shape),
+        _small(lse, "lse", torch.float32, (batch, heads, q_len), q), *back, None)
+
+
+def _window_call(name, desc, backward, q):
+    nbytes = _lib.load().spar_b200_window_attention_scratch_bytes(ctypes.byref(desc), backward, _dev(q))
+    scratch = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes else None
+    desc.scratch = _ptr(scratch)
+    call(name, ctypes.byref(desc), _dev(q), _stream(q))
+
+
+def window_attention_forward(q, k, v, window: int, sinks: int = 0, *, scale: float | None = None,
+                             lengths=None, first=None, out=None):
+    """Causal attention over a sliding window and the first `sinks` tokens.
+
+    q [batch, q_len, heads, head_dim], k and v [batch, kv_len, kv_heads, head_dim] views (a packed
+    projection's parts, or a cache); query head h reads key head h / (heads / kv_heads). Row i of
+    sequence b stands at position p = first[b] + i (first None: kv_len - q_len) and sees key j iff
+    j <= p, j < lengths[b] (None: kv_len), and j > p - window or j < sinks; a row with p < 0 or
+    p >= lengths[b] sees nothing (out 0, lse -inf). scale None: 1 / sqrt(head_dim).
+    Returns (out like q, lse [batch, heads, q_len])."""
+    out = _like(q, out)
+    lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], device=q.device, dtype=torch.float32)
+    desc = _window_desc(q, k, v, out, lse, window, sinks, scale, lengths, first)
+    _window_call("spar_b200_window_attention_forward", desc, 0, q)
+    return out, lse
+
+
+def window_attention_backward(dout, q, k, v, out, lse, window: int, sinks: int = 0, *,
+                              scale: float | None = None, lengths=None, first=None, dq=None, dk=None,
+                              dv=None):
+    """(dq, dk, dv) of window_attention_forward; dk and dv are summed over each key head's group.
+    dq, dk, dv may be given as views of a packed gradient buffer."""
+    dq, dk, dv = _like(q, dq), _like(k, dk), _like(v, dv)
+    desc = _window_desc(q, k, v, out, lse, window, sinks, scale, lengths, first, dout, dq, dk, dv)
+    _window_call("spar_b200_window_attention_backward", desc, 1, q)
+    return dq, dk, dv
 
 
 # ------------------------------------------------------------------------------- GEMM

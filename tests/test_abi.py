@@ -114,3 +114,65 @@ def test_warmup_cosine_entry_point_matches_reference_fixture():
     f = np.load(ROOT / "tests" / "golden" / "schedule.npz")
     for s, lr in zip(f["steps"], f["lr"]):
         assert warmup_cosine(3e-4, 3e-5, 100, 900, int(s)) == lr
+
+
+def test_rotary_and_window_attention_refuse_bad_calls_without_gpu():
+    """Sizes, strides, tags and pointers are checked before any CUDA call (code 1); zero-count calls
+    succeed."""
+    from spar_b200 import _lib
+
+    lib = _lib.load()
+    at = 1 << 20  # never dereferenced: validation fails first
+
+    def rotary(**k):
+        base = dict(dtype=0, layout=1, batch=2, seq=3, heads=4, kv_heads=2, head_dim=64, rotary_dim=32,
+                    table=at, table_rows=3, q=at, k=at, q_out=at, k_out=at, q_weight=at, k_weight=at,
+                    epsilon=1e-6, dq=at, dk=at, dq_weight=at, dk_weight=at, scratch=at)
+        return ctypes.byref(_lib.SparB200Rotary(**{**base, **k}))
+
+    for bad in (dict(dtype=2), dict(layout=2), dict(head_dim=0), dict(head_dim=257), dict(rotary_dim=31),
+                dict(rotary_dim=66), dict(rotary_dim=0), dict(heads=0), dict(table=None), dict(q=None),
+                dict(k_out=None), dict(table_rows=2), dict(start=1), dict(start=2 ** 64 - 1), dict(q=at + 2),
+                dict(batch=1 << 20, seq=1 << 20), dict(batch=1 << 40, seq=1 << 40)):
+        assert lib.spar_b200_rotary(rotary(**bad), 0, None).code == 1, bad
+        assert lib.spar_b200_qk_norm_rotary_forward(rotary(**bad), 0, None).code == 1, bad
+        assert lib.spar_b200_qk_norm_rotary_backward(rotary(**bad), 0, None).code == 1, bad
+    for bad in (dict(q_weight=None), dict(k_weight=at + 2), dict(epsilon=-1.0), dict(epsilon=float("nan"))):
+        assert lib.spar_b200_qk_norm_rotary_forward(rotary(**bad), 0, None).code == 1, bad
+    for bad in (dict(dq_weight=None), dict(dk_weight=None), dict(scratch=None), dict(scratch=at + 4),
+                dict(dk=None)):
+        assert lib.spar_b200_qk_norm_rotary_backward(rotary(**bad), 0, None).code == 1, bad
+    assert lib.spar_b200_rotary(None, 0, None).code == 1
+    assert lib.spar_b200_rotary(rotary(seq=0, table=None, q=None, q_out=None), 0, None).code == 0
+    for args in ((at, 4, 31, 1e4, 0), (at, 4, 0, 1e4, 0), (at, 4, 32, 0.0, 0), (None, 4, 32, 1e4, 0),
+                 (at + 4, 4, 32, 1e4, 0), (at, 4, 258, 1e4, 0), (at, 4, 32, float("inf"), 0)):
+        assert lib.spar_b200_rotary_table(*args, None, 0, None).code == 1, args
+    assert lib.spar_b200_rotary_table(None, 0, 32, 1e4, 0, None, 0, None).code == 0
+
+    def window(**k):
+        base = dict(dtype=1, batch=2, q_len=3, kv_len=5, heads=4, kv_heads=2, head_dim=64, window=4,
+                    sinks=1, q=at, k=at, v=at, out=at, lse=at, dout=at, dq=at, dk=at, dv=at, scratch=at)
+        return ctypes.byref(_lib.SparB200WindowAttention(**{**base, **k}))
+
+    for bad in (dict(dtype=7), dict(heads=0), dict(kv_heads=0), dict(kv_heads=3), dict(kv_heads=8),
+                dict(head_dim=0), dict(head_dim=257), dict(window=0), dict(scale=-1.0),
+                dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None), dict(k=at + 1),
+                dict(q_len=1 << 30), dict(kv_len=1 << 40), dict(batch=1 << 29, heads=64, kv_heads=64),
+                dict(batch=1 << 12, kv_len=1 << 20)):
+        assert lib.spar_b200_window_attention_forward(window(**bad), 0, None).code == 1, bad
+        assert lib.spar_b200_window_attention_backward(window(**bad), 0, None).code == 1, bad
+    for bad in (dict(dout=None), dict(lse=None), dict(dv=None), dict(scratch=None), dict(scratch=at + 16)):
+        assert lib.spar_b200_window_attention_backward(window(**bad), 0, None).code == 1, bad
+    assert lib.spar_b200_window_attention_forward(window(batch=0, q=None, k=None), 0, None).code == 0
+    assert lib.spar_b200_window_attention_forward(window(q_len=0, q=None, out=None), 0, None).code == 0
+    assert lib.spar_b200_window_attention_backward(window(batch=0), 0, None).code == 0
+    assert lib.spar_b200_window_attention_scratch_bytes(window(), 1, 0) >= 2 * 4 * 3 * 4
+
+
+def test_new_structures_mirror_the_header():
+    """Sizes that a C compiler gives the header's structs (all members 8-byte aligned after the tags)."""
+    from spar_b200 import _lib
+
+    assert ctypes.sizeof(_lib.SparB200Rotary) == 352
+    assert ctypes.sizeof(_lib.SparB200WindowAttention) == 368
+    assert ctypes.sizeof(_lib.SparB200RotaryScaling) == 48

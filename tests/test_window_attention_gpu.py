@@ -1,0 +1,343 @@
+"""Attention with a sliding window and first tokens that stay visible, forward and backward, against
+the 64-bit form, with element-wise bounds that follow from the roundings (see _attention_ref)."""
+import math
+
+import pytest
+import torch
+
+from _attention_ref import assert_within, half_step, window_attention
+
+pytestmark = pytest.mark.gpu
+
+
+def _packed(cuda, g, dtype, b, t, h, kv, d, offset=0):
+    width = (h + 2 * kv) * d
+    x = torch.randn(b * t * width + offset, generator=g, device=cuda).to(dtype)[offset:].view(b, t, width)
+    return (x[..., :h * d].unflatten(-1, (h, d)), x[..., h * d:(h + kv) * d].unflatten(-1, (kv, d)),
+            x[..., (h + kv) * d:].unflatten(-1, (kv, d)))
+
+
+def _check(q, k, v, window, sinks, dout=None, **where):
+    from spar_b200 import ops
+
+    out, lse = ops.window_attention_forward(q, k, v, window, sinks, **where)
+    got = {"out": out, "lse": lse}
+    if dout is not None:
+        got["dq"], got["dk"], got["dv"] = ops.window_attention_backward(dout, q, k, v, out, lse, window,
+                                                                        sinks, **where)
+    torch.cuda.synchronize()
+    assert ops.attention_error() == 0
+    want, bound = window_attention(
+        *(x.double().cpu() for x in (q, k, v)), window, sinks, where.get("scale"), where.get("lengths"),
+        where.get("first"), None if dout is None else dout.double().cpu(), half_step(q.dtype))
+    for name in want:
+        assert_within(got[name], want[name], bound[name], name)
+    return got
+
+
+SELF = [
+    # b, t, heads, kv, dim, window, sinks
+    (1, 1, 1, 1, 64, 1, 0),
+    (2, 2, 2, 1, 64, 1, 1),
+    (1, 5, 4, 2, 32, 3, 2),
+    (2, 63, 2, 2, 64, 16, 4),
+    (1, 128, 4, 1, 64, 128, 0),     # one tile
+    (1, 129, 2, 1, 64, 64, 4),      # one row behind it
+    (2, 200, 3, 1, 128, 50, 3),     # a group of three
+    (1, 257, 2, 2, 128, 1000, 0),   # plain causal
+    (1, 300, 2, 1, 64, 1, 0),       # each row sees itself
+    (1, 300, 2, 1, 64, 1, 300),     # everything is a first token
+    (1, 520, 4, 4, 32, 100, 130),   # first tokens over more than a tile
+    (2, 513, 2, 1, 128, 127, 1),
+    (1, 700, 2, 1, 64, 300, 64),
+    (1, 150, 2, 1, 96, 40, 5),
+    (1, 150, 2, 1, 80, 40, 5),
+    (1, 140, 2, 2, 33, 20, 2),      # odd head: element by element
+    (1, 70, 1, 1, 200, 30, 2),
+    (1, 1400, 2, 1, 64, 200, 4),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", SELF)
+def test_self_attention(cuda, shape, dtype):
+    b, t, h, kv, d, window, sinks = shape
+    g = torch.Generator(device=cuda)
+    g.manual_seed(t * 3 + d)
+    q, k, v = _packed(cuda, g, dtype, b, t, h, kv, d)
+    dout = torch.randn(b, t, h, d, generator=g, device=cuda).to(dtype)
+    _check(q, k, v, window, sinks, dout)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("offset", [1, 4])
+def test_rows_that_are_not_aligned(cuda, dtype, offset):
+    g = torch.Generator(device=cuda)
+    g.manual_seed(5)
+    q, k, v = _packed(cuda, g, dtype, 2, 140, 4, 2, 64, offset)
+    dout = torch.randn(2, 140, 4, 64, generator=g, device=cuda).to(dtype)
+    _check(q, k, v, 33, 3, dout)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_padded_batch_ignores_what_lies_behind_the_lengths(cuda, dtype, dim):
+    """Lengths 0, 1, inside a tile and whole; NaN and infinities behind them, in the gradients too."""
+    g = torch.Generator(device=cuda)
+    g.manual_seed(6)
+    lengths = [300, 0, 1, 131, 128, 299, 500, -4]
+    q, k, v = _packed(cuda, g, dtype, len(lengths), 300, 4, 2, dim)
+    dout = torch.randn(q.shape, generator=g, device=cuda).to(dtype)
+    n = torch.tensor(lengths, dtype=torch.int32, device=cuda)
+    clean = _check(q, k, v, 70, 4, dout, lengths=n)
+    for b, m in enumerate(lengths):
+        for x, bad in ((q, math.nan), (k, math.nan), (v, math.inf), (dout, math.nan)):
+            x[b, max(m, 0):] = bad
+    from spar_b200 import ops
+
+    out, lse = ops.window_attention_forward(q, k, v, 70, 4, lengths=n)
+    grads = ops.window_attention_backward(dout, q, k, v, out, lse, 70, 4, lengths=n)
+    for x, name in zip((out, lse, *grads), ("out", "lse", "dq", "dk", "dv")):
+        assert torch.equal(x, clean[name]), name
+
+
+CACHE = [
+    # b, q_len, kv_len, heads, kv, dim, window, sinks
+    (1, 1, 1, 1, 1, 64, 5, 0),
+    (3, 1, 40, 4, 4, 64, 16, 4),
+    (2, 1, 1000, 8, 2, 128, 256, 4),
+    (4, 1, 2100, 16, 1, 64, 5000, 0),   # sixteen heads of one cache
+    (2, 3, 777, 8, 2, 64, 100, 1),      # a few tokens at once
+    (1, 5, 640, 32, 4, 128, 600, 64),
+    (2, 1, 300, 6, 3, 96, 100, 3),
+    (1, 2, 500, 3, 1, 50, 100, 3),
+    (2, 1, 700, 2, 1, 256, 300, 4),
+    (1, 40, 900, 4, 2, 64, 300, 4),     # a chunk of a prompt
+    (1, 200, 700, 4, 2, 128, 130, 4),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", CACHE)
+def test_tokens_against_a_cache(cuda, shape, dtype):
+    b, t, n, h, kv, d, window, sinks = shape
+    g = torch.Generator(device=cuda)
+    g.manual_seed(n + d)
+    q = torch.randn(b, t, h, d, generator=g, device=cuda).to(dtype)
+    k = torch.randn(b, n, kv, d, generator=g, device=cuda).to(dtype)
+    v = torch.randn(b, n, kv, d, generator=g, device=cuda).to(dtype)
+    dout = torch.randn(q.shape, generator=g, device=cuda).to(dtype)
+    _check(q, k, v, window, sinks, dout)
+    lengths = torch.tensor([n - (x * 37) % max(n - t, 1) for x in range(b)], dtype=torch.int32, device=cuda)
+    for x in range(b):
+        k[x, int(lengths[x]):] = math.nan
+        v[x, int(lengths[x]):] = math.nan
+    _check(q, k, v, window, sinks, dout, lengths=lengths, first=lengths - t)
+
+
+def test_positions_of_the_first_row(cuda):
+    """Rows before position 0, rows behind the length, and positions far outside."""
+    g = torch.Generator(device=cuda)
+    g.manual_seed(11)
+    for dtype in (torch.float32, torch.bfloat16):
+        for t, n in ((4, 200), (160, 200), (200, 90)):
+            first = [0, -3, n - 2, n + 5, 2 ** 31 - 1, -2 ** 31, n - t]
+            q = torch.randn(len(first), t, 2, 64, generator=g, device=cuda).to(dtype)
+            k = torch.randn(len(first), n, 1, 64, generator=g, device=cuda).to(dtype)
+            v = torch.randn(len(first), n, 1, 64, generator=g, device=cuda).to(dtype)
+            dout = torch.randn(q.shape, generator=g, device=cuda).to(dtype)
+            _check(q, k, v, 50, 3, dout, first=torch.tensor(first, dtype=torch.int32, device=cuda))
+            if t > n:
+                _check(q, k, v, 50, 3, dout)  # default: the first rows stand before position 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_large_logits_and_a_given_scale(cuda, dtype):
+    g = torch.Generator(device=cuda)
+    g.manual_seed(12)
+    q, k, v = _packed(cuda, g, dtype, 1, 260, 2, 1, 64)
+    dout = torch.randn(q.shape, generator=g, device=cuda).to(dtype)
+    _check(q * 6, k * 6, v, 90, 4, dout)
+    _check(q, k, v, 90, 4, dout, scale=0.9)
+    rising = (k * torch.linspace(0, 8, 260, device=cuda)[None, :, None, None]).to(dtype)
+    _check(q, rising, v, 260, 0, dout)  # the maximum keeps moving
+
+
+def test_outputs_into_a_packed_buffer_leave_the_rest(cuda):
+    from spar_b200 import ops
+
+    g = torch.Generator(device=cuda)
+    g.manual_seed(13)
+    for dtype in (torch.float32, torch.bfloat16):
+        for d in (64, 33):
+            q, k, v = _packed(cuda, g, dtype, 2, 135, 4, 2, d)
+            dout = torch.randn(q.shape, generator=g, device=cuda).to(dtype)
+            out, lse = ops.window_attention_forward(q, k, v, 40, 2)
+            want = ops.window_attention_backward(dout, q, k, v, out, lse, 40, 2)
+            wide = torch.full((2, 137, 11, d + 8), 7.0, device=cuda, dtype=dtype)
+            o = wide[:, 1:136, 0:4, :d]
+            ops.window_attention_forward(q, k, v, 40, 2, out=o)
+            assert torch.equal(o, out)
+            o.fill_(7.0)
+            assert bool((wide == 7.0).all())
+            dq, dk, dv = (wide[:, 1:136, s, :d] for s in (slice(0, 4), slice(4, 6), slice(7, 9)))
+            got = ops.window_attention_backward(dout, q, k, v, out, lse, 40, 2, dq=dq, dk=dk, dv=dv)
+            for x, y in zip(got, want):
+                assert torch.equal(x, y)
+                x.fill_(7.0)
+            assert bool((wide == 7.0).all())
+
+
+def test_repeats_streams_and_captured_graphs(cuda):
+    """The same bits on every run; two captured graphs and an eager call share nothing."""
+    from spar_b200 import ops
+
+    g = torch.Generator(device=cuda)
+    g.manual_seed(14)
+    sets = []
+    for b, t, n in ((2, 260, 260), (1, 1, 900)):
+        for dtype in (torch.float32, torch.bfloat16):
+            q = torch.randn(b, t, 8, 64, generator=g, device=cuda).to(dtype)
+            k = torch.randn(b, n, 2, 64, generator=g, device=cuda).to(dtype)
+            v = torch.randn(b, n, 2, 64, generator=g, device=cuda).to(dtype)
+            sets.append((q, k, v, torch.randn(q.shape, generator=g, device=cuda).to(dtype)))
+
+    def block(s):
+        q, k, v, dout = s
+        out, lse = ops.window_attention_forward(q, k, v, 100, 4)
+        return (out, lse, *ops.window_attention_backward(dout, q, k, v, out, lse, 100, 4))
+
+    want = [block(s) for s in sets]
+    for s, w in zip(sets, want):
+        assert all(torch.equal(a, b) for a, b in zip(block(s), w))
+    graphs = []
+    for s in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            graphs.append((graph, block(s)))
+        graphs[-1] = (graph, graphs[-1][1])
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for (graph, _), stream in zip(graphs, streams):
+        with torch.cuda.stream(stream):
+            graph.replay()
+    eager = [block(s) for s in sets]
+    torch.cuda.synchronize()
+    for (_, held), e, w in zip(graphs, eager, want):
+        assert all(torch.equal(a, b) for a, b in zip(held, w))
+        assert all(torch.equal(a, b) for a, b in zip(e, w))
+
+
+def test_nothing_to_do(cuda):
+    from spar_b200 import ops
+
+    empty = torch.empty(2, 0, 4, 64, device=cuda)
+    some = torch.ones(2, 5, 2, 64, device=cuda)
+    out, lse = ops.window_attention_forward(empty, some, some, 4)
+    assert out.shape == empty.shape and lse.shape == (2, 4, 0)
+    dq, dk, dv = ops.window_attention_backward(empty, empty, some, some, out, lse, 4)
+    assert not dk.any() and not dv.any()
+    q = torch.ones(2, 3, 4, 64, device=cuda)
+    none = torch.empty(2, 0, 2, 64, device=cuda)
+    out, lse = ops.window_attention_forward(q, none, none, 4)
+    assert not out.any() and bool((lse == -math.inf).all())
+    dq, dk, dv = ops.window_attention_backward(q, q, none, none, out, lse, 4)
+    assert not dq.any() and dk.shape == none.shape
+
+
+def test_wide_window_is_the_framework_causal_attention(cuda):
+    """With a window over everything this is attention_forward / attention_backward, within the
+    2e-3 of their TF32 products."""
+    from _util import rel_l2
+    from spar_b200 import ops
+
+    g = torch.Generator(device=cuda)
+    g.manual_seed(15)
+    b, t, h, kv, d = 2, 200, 4, 2, 64
+    x = torch.randn(b, t, (h + 2 * kv) * d, generator=g, device=cuda)
+    dout = torch.randn(b, t, h * d, generator=g, device=cuda)
+    ctx, top, inv = ops.attention_forward(x, h, kv)
+    dx = ops.attention_backward(dout, x, ctx, top, inv, h, kv_heads=kv)
+    parts = lambda y: (y[..., :h * d].unflatten(-1, (h, d)), y[..., h * d:(h + kv) * d].unflatten(-1, (kv, d)),  # noqa: E731
+                       y[..., (h + kv) * d:].unflatten(-1, (kv, d)))
+    q, k, v = parts(x)
+    out, lse = ops.window_attention_forward(q, k, v, t)
+    mine = torch.empty_like(x)
+    dq, dk, dv = parts(mine)
+    ops.window_attention_backward(dout.unflatten(-1, (h, d)), q, k, v, out, lse, t, dq=dq, dk=dk, dv=dv)
+    assert rel_l2(out.flatten(2).cpu(), ctx.cpu()) <= 2e-3
+    for a, b_ in zip(parts(mine), parts(dx)):
+        assert rel_l2(a.cpu(), b_.cpu()) <= 3e-3
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_attention_block_forward_and_backward(cuda, dtype):
+    """Norm and rotation of the packed projection's queries and keys, window attention, and back to
+    the gradient of the projection, as a layer runs them; then one token against the cache that the
+    layer's keys and values make, at its position in the table."""
+    from _attention_ref import norm_rotate
+    from _util import rel_l2
+    from spar_b200 import ops
+
+    g = torch.Generator(device=cuda)
+    g.manual_seed(16)
+    b, t, h, kv, d, window, sinks = 2, 190, 8, 2, 64, 60, 4
+    width = (h + 2 * kv) * d
+    x = (2 * torch.randn(b, t, width, generator=g, device=cuda)).to(dtype)
+    dout = torch.randn(b, t, h, d, generator=g, device=cuda).to(dtype)
+    w = [1 + 0.2 * torch.randn(d, generator=g, device=cuda) for _ in range(2)]
+    scaling = ops.RotaryScaling("parts", 4.0, 64)
+    table = ops.rotary_table(t, d // 2, scaling=scaling, device=cuda)
+    parts = lambda y: (y[..., :h * d].unflatten(-1, (h, d)), y[..., h * d:(h + kv) * d].unflatten(-1, (kv, d)),  # noqa: E731
+                       y[..., (h + kv) * d:].unflatten(-1, (kv, d)))
+    q, k, v = parts(x)
+    rq, rk = ops.qk_norm_rotary_forward(q, k, *w, table, layout="half")
+    out, lse = ops.window_attention_forward(rq, rk, v, window, sinks)
+    dx = torch.empty_like(x)
+    dq, dk, dv = parts(dx)
+    ops.window_attention_backward(dout, rq, rk, v, out, lse, window, sinks, dq=dq, dk=dk, dv=dv)
+    _, _, dwq, dwk = ops.qk_norm_rotary_backward(dq, dk, q, k, *w, table, layout="half", dq=dq, dk=dk)
+
+    x64 = x.double().cpu().requires_grad_()
+    w64 = [y.double().cpu().requires_grad_() for y in w]
+    angles = table.double().cpu()[None]
+    q64, k64, v64 = parts(x64)
+    q64 = norm_rotate(q64, w64[0], angles, d // 2, "half", 1e-6)
+    k64 = norm_rotate(k64, w64[1], angles, d // 2, "half", 1e-6)
+    p = torch.arange(t)
+    see = (p[None] <= p[:, None]) & ((p[None] > p[:, None] - window) | (p[None] < sinks))
+    s = torch.einsum("bihd,bjhd->bhij", q64, k64.repeat_interleave(h // kv, 2)) * d ** -0.5
+    o64 = torch.einsum("bhij,bjhd->bihd", torch.softmax(s.masked_fill(~see, -math.inf), -1),
+                       v64.repeat_interleave(h // kv, 2))
+    o64.backward(dout.double().cpu())
+    # A chain of a handful of roundings to the stored type (rotated q, k, P, dS, out, the gradients
+    # twice): at most eight half steps in the 2-norm, and 2^-20 for the sums in 32 bits.
+    tol = 8 * half_step(dtype) + 2.0 ** -20
+    for got, want in ((out, o64), (dx, x64.grad), (dwq, w64[0].grad), (dwk, w64[1].grad)):
+        assert rel_l2(got.detach().double().cpu(), want.detach()) <= tol
+
+    token = torch.full((b, 1), t - 1, dtype=torch.int32, device=cuda)
+    q1, _ = ops.qk_norm_rotary_forward(q[:, t - 1:], None, w[0], None, table, layout="half",
+                                       positions=token)
+    assert torch.equal(q1, rq[:, t - 1:])
+    o1, lse1 = ops.window_attention_forward(q1, rk, v, window, sinks)
+    assert rel_l2(o1.double().cpu(), o64[:, t - 1:].detach()) <= tol
+    assert float((lse1[..., 0] - lse[..., t - 1]).abs().max()) <= 2.0 ** -18
+
+
+def test_wrong_calls_are_refused(cuda):
+    from spar_b200 import ops
+
+    q, k = torch.zeros(2, 4, 4, 64, device=cuda), torch.zeros(2, 9, 2, 64, device=cuda)
+    n = torch.zeros(2, dtype=torch.int32, device=cuda)
+    f = ops.window_attention_forward
+    bad = [lambda: f(q, k, k, 0), lambda: f(q, k, k, 4, -1), lambda: f(q, k, k[:, :8], 4),
+           lambda: f(q, k.bfloat16(), k.bfloat16(), 4), lambda: f(q.double(), k.double(), k.double(), 4),
+           lambda: f(q[:, :, :3], k, k, 4), lambda: f(q, k[..., :32], k[..., :32], 4),
+           lambda: f(q, k, k, 4, scale=0.0), lambda: f(q, k, k, 4, lengths=n[:1]),
+           lambda: f(q, k, k, 4, first=n.long()), lambda: f(q.cpu(), k.cpu(), k.cpu(), 4),
+           lambda: f(q, k, k, 4, out=torch.zeros(2, 4, 4, 64, device=cuda, dtype=torch.bfloat16)),
+           lambda: f(q[:1], k, k, 4)]
+    for call in bad:
+        with pytest.raises(ValueError):
+            call()
