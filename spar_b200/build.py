@@ -36,6 +36,7 @@ SOURCES = [
     "qknorm.cu",
     "rotary.cu",
     "window_attention.cu",
+    "window_tc.cu",
 ]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

@@ -1,0 +1,66 @@
+// What the window-attention kernels share: one call's tensors and sizes, and what of them one
+// sequence of the batch uses.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace spar_b200 {
+namespace window {
+
+constexpr int64_t kMaxLength = 1ll << 29;  // so that sums of two positions stay in 32 bits
+constexpr uint64_t kMaxHeadDim = 256;
+
+// A strided view of heads: element (b, t, h, e) at data + b*batch + t*token + h*head + e.
+struct View {
+  char* data;
+  uint64_t batch, token, head;  // strides in elements
+};
+
+struct WindowParams {
+  View q, k, v, out, dout, dq, dk, dv;
+  float* lse;
+  float* delta;  // [batch, heads, q_len] D
+  const int32_t* lengths;
+  const int32_t* first;
+  int q_len, kv_len, heads, kv_heads, group, head_dim;
+  int window, sinks;
+  int batch;
+  int dtype;
+  float scale;
+};
+
+// What one sequence of the batch holds: n keys, and the position of its first row.
+struct Sequence {
+  int n, p0;
+};
+__device__ __forceinline__ Sequence sequence_of(const WindowParams& w, int b) {
+  Sequence s;
+  s.n = w.lengths ? min(max(__ldg(w.lengths + b), 0), w.kv_len) : w.kv_len;
+  // Positions beyond +-2^29 see nothing, as every position at or behind the length does.
+  const int far = 1 << 29;
+  s.p0 = w.first ? min(max(__ldg(w.first + b), -far), far) : w.kv_len - w.q_len;
+  return s;
+}
+
+template <typename T>
+__device__ __forceinline__ const T* row_ptr(const View& v, int b, int t, int h) {
+  return reinterpret_cast<const T*>(v.data) + b * v.batch + t * v.token + h * v.head;
+}
+template <typename T>
+__device__ __forceinline__ T* row_out(const View& v, int b, int t, int h) {
+  return reinterpret_cast<T*>(v.data) + b * v.batch + t * v.token + h * v.head;
+}
+__device__ __forceinline__ float as_float(float v) { return v; }
+__device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void put(float* p, float v) { *p = v; }
+__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// Tensor-core path (window_tc.cu): whether it takes this call, its scratch, and the launches.
+bool tc_supported(const WindowParams& w, bool backward);
+uint64_t tc_scratch_bytes(const WindowParams& w, bool backward, int device);
+cudaError_t tc_forward(const WindowParams& w, void* scratch, int device, cudaStream_t stream);
+
+}  // namespace window
+}  // namespace spar_b200

@@ -12,55 +12,11 @@
 
 #include "common.cuh"
 #include "kernels.cuh"
+#include "window.cuh"
 
 namespace spar_b200 {
+namespace window {
 namespace {
-
-constexpr int64_t kMaxLength = 1ll << 30;
-constexpr uint64_t kMaxHeadDim = 256;
-
-struct View {
-  char* data;
-  uint64_t batch, token, head;  // strides in elements
-};
-
-struct WindowParams {
-  View q, k, v, out, dout, dq, dk, dv;
-  float* lse;
-  float* delta;  // [batch, heads, q_len] D
-  const int32_t* lengths;
-  const int32_t* first;
-  int q_len, kv_len, heads, kv_heads, group, head_dim;
-  int window, sinks;
-  int batch;
-  float scale;
-};
-
-// What one sequence of the batch holds: n keys, and the position of its first row.
-struct Sequence {
-  int n, p0;
-};
-__device__ __forceinline__ Sequence sequence_of(const WindowParams& w, int b) {
-  Sequence s;
-  s.n = w.lengths ? min(max(__ldg(w.lengths + b), 0), w.kv_len) : w.kv_len;
-  // Positions beyond +-2^30 see nothing, as every position at or behind the length does.
-  const int far = 1 << 30;
-  s.p0 = w.first ? min(max(__ldg(w.first + b), -far), far) : w.kv_len - w.q_len;
-  return s;
-}
-
-template <typename T>
-__device__ __forceinline__ const T* row_ptr(const View& v, int b, int t, int h) {
-  return reinterpret_cast<const T*>(v.data) + b * v.batch + t * v.token + h * v.head;
-}
-template <typename T>
-__device__ __forceinline__ T* row_out(const View& v, int b, int t, int h) {
-  return reinterpret_cast<T*>(v.data) + b * v.batch + t * v.token + h * v.head;
-}
-__device__ __forceinline__ float as_float(float v) { return v; }
-__device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
 // ------------------------------------------------------------------------- any shape and stride
 // One warp per row, lanes over the head's elements (E of them each), one pass over the visible
@@ -280,6 +236,7 @@ bool make_params(const SparB200WindowAttention* a, bool backward, WindowParams& 
   w.head_dim = static_cast<int>(a->head_dim);
   w.window = static_cast<int>(a->window < static_cast<uint64_t>(kMaxLength) ? a->window : kMaxLength);
   w.sinks = static_cast<int>(a->sinks < a->kv_len ? a->sinks : a->kv_len);
+  w.dtype = a->dtype;
   w.scale = static_cast<float>(
       a->scale > 0.0 ? a->scale : 1.0 / std::sqrt(static_cast<double>(a->head_dim)));
   return true;
@@ -320,15 +277,36 @@ cudaError_t row_path(const WindowParams& w, bool backward, cudaStream_t stream) 
 }
 
 }  // namespace
+}  // namespace window
 }  // namespace spar_b200
 
 using namespace spar_b200;
+using namespace spar_b200::window;
+
+namespace {
+
+// What a call will run, decided from its sizes, types and strides alone, so that the scratch it is
+// asked for and the launch agree.
+struct Plan {
+  bool tiled;
+  uint64_t delta_bytes, bytes;
+};
+Plan plan_of(const WindowParams& w, bool backward, int device) {
+  Plan p;
+  p.tiled = tc_supported(w, backward);
+  p.delta_bytes =
+      backward ? round256(static_cast<uint64_t>(w.batch) * w.heads * w.q_len * sizeof(float)) : 0;
+  p.bytes = p.delta_bytes + (p.tiled ? tc_scratch_bytes(w, backward, device) : 0);
+  return p;
+}
+
+}  // namespace
 
 extern "C" uint64_t spar_b200_window_attention_scratch_bytes(const SparB200WindowAttention* a,
                                                              int backward, int device) {
-  (void)device;
-  if (!valid_sizes(a) || !backward) return 0;
-  return round256(a->batch * a->heads * a->q_len * sizeof(float));
+  WindowParams w;
+  if (!make_params(a, backward != 0, w) || !w.batch) return 0;
+  return plan_of(w, backward != 0, device).bytes;
 }
 
 extern "C" SparCudaStatus spar_b200_window_attention_forward(const SparB200WindowAttention* a,
@@ -336,11 +314,17 @@ extern "C" SparCudaStatus spar_b200_window_attention_forward(const SparB200Windo
   WindowParams w;
   if (!make_params(a, false, w)) return invalid();
   if (!w.batch || !w.q_len) return ok();
+  const Plan plan = plan_of(w, false, device);
+  if (plan.bytes && (!a->scratch || (reinterpret_cast<uintptr_t>(a->scratch) & 255))) return invalid();
   DeviceScope scope(device);
   if (scope.error() != cudaSuccess) return runtime(scope.error());
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = a->dtype == SPAR_B200_FLOAT32 ? row_path<float>(w, false, s)
-                                                      : row_path<__nv_bfloat16>(w, false, s);
+  cudaError_t e;
+  if (plan.tiled)
+    e = tc_forward(w, a->scratch, device, s);
+  else
+    e = w.dtype == SPAR_B200_FLOAT32 ? row_path<float>(w, false, s)
+                                     : row_path<__nv_bfloat16>(w, false, s);
   return e == cudaSuccess ? launch_status() : runtime(e);
 }
 
@@ -349,13 +333,13 @@ extern "C" SparCudaStatus spar_b200_window_attention_backward(const SparB200Wind
   WindowParams w;
   if (!make_params(a, true, w)) return invalid();
   if (!w.batch || (!w.q_len && !w.kv_len)) return ok();
-  const uint64_t need = round256(a->batch * a->heads * a->q_len * sizeof(float));
-  if (need && (!a->scratch || (reinterpret_cast<uintptr_t>(a->scratch) & 255))) return invalid();
+  const Plan plan = plan_of(w, true, device);
+  if (plan.bytes && (!a->scratch || (reinterpret_cast<uintptr_t>(a->scratch) & 255))) return invalid();
   w.delta = static_cast<float*>(a->scratch);
   DeviceScope scope(device);
   if (scope.error() != cudaSuccess) return runtime(scope.error());
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = a->dtype == SPAR_B200_FLOAT32 ? row_path<float>(w, true, s)
-                                                      : row_path<__nv_bfloat16>(w, true, s);
+  const cudaError_t e = w.dtype == SPAR_B200_FLOAT32 ? row_path<float>(w, true, s)
+                                                     : row_path<__nv_bfloat16>(w, true, s);
   return e == cudaSuccess ? launch_status() : runtime(e);
 }

@@ -1,0 +1,737 @@
+// Window attention on the sm_100a tensor cores: tcgen05.mma kind::f16 over bf16 operands staged by
+// TMA, accumulators in TMEM, the softmax in the warps that read the scores out of TMEM. The
+// mathematics stands at the top of window_attention.cu; scores never reach memory.
+//
+// fp32 inputs run on the same kernels as three bf16 planes: x = x0 + x1 + x2 with x0, x1 the upper
+// 16 bits of x and of x - x0, and x2 the rest (8 significant bits each, so the sum is exact for
+// normal values). A product keeps the six pairs of planes above 2^-24 of it (x0y0; x0y1, x1y0;
+// x1y1, x0y2, x2y0), issued smallest first so that the tensor cores' truncating accumulation
+// cuts the small terms at their own size; the product over keys starts afresh for every key tile
+// and tiles are added in fp32 registers, so no truncating accumulator spans more than one tile.
+//
+// One CTA per SM works through its items (two query tiles of 128 rows that share their key tiles:
+// two heads of one key head where the group is even, else neighbouring tiles of one head).
+// Warp 0 feeds key and value tiles by TMA, one thread of warp 1 issues every product, warps 2-5
+// and 6-9 are the softmax of the two tiles (thread = row): while one tile's scores are
+// exponentiated the other tile's products run. The keys of an item are its first tokens' tiles,
+// then tiles that start exactly at the first key of the window, so a window of W keys under a tile
+// of 128 rows costs ceil((W + 127) / BN) tiles. Every wait is bounded and leaves an error flag.
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <cstring>
+
+#include "common.cuh"
+#include "kernels.cuh"
+#include "tc.cuh"
+#include "window.cuh"
+
+namespace spar_b200 {
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn();
+
+namespace window {
+namespace {
+
+constexpr uint32_t kMaxSmem = 232448;
+constexpr uint32_t kTmemCols = 512;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr float kRescaleLog2 = 8.f;  // the running maximum moves only past this margin (P <= 2^8)
+
+// Why a CTA gives up: the CTA's flag, and the one that spar_b200_attention_error reads.
+struct Abort {
+  volatile int* cta;
+  int* device;
+};
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, const Abort& abort) {
+  if (tc::mbar_wait(bar, parity & 1)) return true;
+  atomicExch(abort.device, 1);
+  *abort.cta = 1;
+  return false;
+}
+
+__device__ __forceinline__ uint8_t* align1024(uint8_t* p) {
+  return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(p) + 1023) & ~uintptr_t(1023));
+}
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Operand tiles in shared memory: per plane, DH / 64 boxes of `rows` rows x 64 elements (128 bytes,
+// 128-byte swizzle). The same image is a K-major operand (rows = M or N, elements = K) and an
+// MN-major one (elements = N, rows = K).
+__device__ __forceinline__ uint64_t kmajor(uint32_t base, uint32_t rows, int ks) {
+  return tc::smem_desc(base + (ks >> 2) * rows * 128 + (ks & 3) * 32, 16, 1024, tc::kLayoutSw128);
+}
+__device__ __forceinline__ uint64_t mnmajor(uint32_t base, uint32_t rows, int ks) {
+  return tc::smem_desc(base + ks * 2048, rows * 128, 1024, tc::kLayoutSw128);
+}
+
+// Pairs of planes of a product, smallest first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0).
+template <int NP>
+constexpr int kProducts = NP == 1 ? 1 : 6;
+template <int NP>
+__host__ __device__ constexpr int plane_a(int i) { return NP == 1 ? 0 : (0x001102 >> (4 * i)) & 15; }
+template <int NP>
+__host__ __device__ constexpr int plane_b(int i) { return NP == 1 ? 0 : (0x010120 >> (4 * i)) & 15; }
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// The upper halves of two floats (their bf16 truncations), and what they leave.
+__device__ __forceinline__ uint32_t take_upper(float& lo, float& hi) {
+  const uint32_t a = __float_as_uint(lo), b = __float_as_uint(hi);
+  lo -= __uint_as_float(a & 0xffff0000u);
+  hi -= __uint_as_float(b & 0xffff0000u);
+  return __byte_perm(a, b, 0x7632);
+}
+
+// 64 consecutive values of a row as bf16 operand columns: one plane rounded to nearest (NP = 1:
+// half a step of bf16, as the stored results have), or three planes that hold all 24 bits.
+template <int NP, int N>
+__device__ __forceinline__ void store_planes(uint32_t taddr, uint32_t plane_cols, float (&v)[N]) {
+  static_assert(N == 64, "one pair of 32-column stores");
+#pragma unroll
+  for (int pl = 0; pl < NP; ++pl) {
+    uint32_t r[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e)
+      r[e] = NP == 1 ? pack_bf16(v[2 * e], v[2 * e + 1]) : take_upper(v[2 * e], v[2 * e + 1]);
+    tc::tmem_store_32x32(taddr + pl * plane_cols, r);
+  }
+}
+
+struct TcParams {
+  WindowParams w;
+  CUtensorMap q, k, v;
+  int* wait_flag;
+  int tiles;        // query tiles of 128 rows
+  int pair_heads;   // 1: items are (query tile, two heads); 0: (two query tiles, head)
+  int items;
+  int ksteps;       // K steps of 16 that cover head_dim
+  float scale_log2;
+};
+
+// Which keys one item visits: `n` tiles of BN keys, the first `ns` over the first tokens (keys
+// below `sinks`), the others from `start` on; query tile x uses the first-token tiles and tiles
+// ns + a[x] .. ns + b[x] - 1 of the rest (none of any when `any[x]` is false).
+struct Item {
+  int b, kh, h[2], row[2];
+  Sequence s;
+  int ns, n, start;
+  int a[2], b_end[2];
+  bool any[2];
+};
+
+template <int QT, int BN>
+__device__ __forceinline__ Item item_of(const TcParams& p, int idx) {
+  const WindowParams& w = p.w;
+  Item it;
+  int bh;
+  if (QT == 2 && p.pair_heads) {
+    const int pairs = w.heads / 2, per = w.batch * pairs, t = idx / per;
+    bh = idx - t * per;
+    it.b = bh / pairs;
+    it.h[0] = (bh - it.b * pairs) * 2;
+    it.h[1] = it.h[0] + 1;
+    it.row[0] = it.row[1] = t * 128;
+  } else {
+    const int per = w.batch * w.heads, t = idx / per;
+    bh = idx - t * per;
+    it.b = bh / w.heads;
+    it.h[0] = it.h[1] = bh - it.b * w.heads;
+    it.row[0] = t * 128 * QT;
+    it.row[1] = it.row[0] + 128;
+  }
+  it.kh = it.h[0] / w.group;
+  it.s = sequence_of(w, it.b);
+  int lo[2], hi[2], ulo = INT_MAX, uhi = -1;
+#pragma unroll
+  for (int x = 0; x < QT; ++x) {
+    const int rows = min(128, w.q_len - it.row[x]);
+    const int pa = max(it.s.p0 + it.row[x], 0), pb = min(it.s.p0 + it.row[x] + rows - 1, it.s.n - 1);
+    it.any[x] = rows > 0 && pb >= pa;
+    lo[x] = max(0, pa - w.window + 1);
+    hi[x] = pb;
+    if (it.any[x]) {
+      ulo = min(ulo, lo[x]);
+      uhi = max(uhi, hi[x]);
+    }
+  }
+  it.ns = it.n = it.start = 0;
+  if (uhi < 0) return it;
+  const bool apart = w.sinks > 0 && ulo > w.sinks;
+  it.start = w.sinks > 0 && !apart ? 0 : ulo;
+  it.ns = apart ? (w.sinks + BN - 1) / BN : 0;
+  it.n = it.ns + (uhi - it.start) / BN + 1;
+#pragma unroll
+  for (int x = 0; x < QT; ++x) {
+    it.a[x] = w.sinks > 0 && !apart ? 0 : (lo[x] - it.start) / BN;
+    it.b_end[x] = (hi[x] - it.start) / BN + 1;
+  }
+  return it;
+}
+// The next tile of query tile x from j on, or n.
+__device__ __forceinline__ int next_tile(const Item& it, int x, int j) {
+  if (j < it.ns) return j;
+  j = max(j, it.ns + it.a[x]);
+  return j < it.ns + it.b_end[x] ? j : it.n;
+}
+template <int BN>
+__device__ __forceinline__ int key_of(const Item& it, int j) {
+  return j < it.ns ? j * BN : it.start + (j - it.ns) * BN;
+}
+
+template <int DH, int NP, int QT, int BN, int KS, int VS>
+struct Fwd {
+  static constexpr uint32_t kQTile = NP * DH * 256;      // 128 rows
+  static constexpr uint32_t kKTile = NP * DH * BN * 2;   // BN rows
+  static constexpr uint32_t kQ = 0;
+  static constexpr uint32_t kK = kQ + QT * kQTile;
+  static constexpr uint32_t kV = kK + KS * kKTile;
+  static constexpr uint32_t kBar = kV + VS * kKTile;
+  static constexpr uint32_t kSmem = kBar + 256 + 1024;
+  static_assert(kSmem <= kMaxSmem, "forward shared memory");
+  // TMEM columns of one query tile: scores, which P overwrites, then O of the current key tile
+  // (NP = 1: of the item), then (NP = 3) the sum of the earlier tiles' O.
+  static constexpr uint32_t kS = NP == 1 ? BN : (NP * BN / 2 > BN ? NP * BN / 2 : BN);
+  static constexpr uint32_t kCols = kS + DH * (NP == 1 ? 1 : 2);
+  static_assert(QT * kCols <= kTmemCols, "forward TMEM");
+};
+
+template <int DH, int NP, int QT, int BN, int KS, int VS>
+__global__ void __launch_bounds__(64 + 128 * QT, 1) window_forward_kernel(
+    const __grid_constant__ TcParams p) {
+  using L = Fwd<DH, NP, QT, BN, KS, VS>;
+  constexpr int kBoxes = DH / 64;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
+  uint64_t* q_full = bars;         // [2]
+  uint64_t* q_empty = bars + 2;    // [2]
+  uint64_t* s_full = bars + 4;     // [2]
+  uint64_t* p_full = bars + 6;     // [2]
+  uint64_t* o_full = bars + 8;     // [2]
+  uint64_t* o_empty = bars + 10;   // [2]
+  uint64_t* k_full = bars + 12;    // [KS]
+  uint64_t* k_empty = k_full + KS;
+  uint64_t* v_full = k_empty + KS;  // [VS]
+  uint64_t* v_empty = v_full + VS;
+  uint64_t* drain = v_empty + VS;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  const Abort abort_flag = {reinterpret_cast<volatile int*>(tmem_slot + 1), p.wait_flag};
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const WindowParams& w = p.w;
+
+  if (threadIdx.x == 0) {
+    for (int x = 0; x < 2; ++x) {
+      tc::mbar_init(q_full + x, 1);
+      tc::mbar_init(q_empty + x, 1);
+      tc::mbar_init(s_full + x, 1);
+      tc::mbar_init(p_full + x, 4);
+      tc::mbar_init(o_full + x, 1);
+      tc::mbar_init(o_empty + x, 4);
+    }
+    for (int i = 0; i < KS; ++i) {
+      tc::mbar_init(k_full + i, 1);
+      tc::mbar_init(k_empty + i, 1);
+    }
+    for (int i = 0; i < VS; ++i) {
+      tc::mbar_init(v_full + i, 1);
+      tc::mbar_init(v_empty + i, 1);
+    }
+    tc::mbar_init(drain, 1);
+    *abort_flag.cta = 0;
+    tc::fence_barrier_init();
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(tmem_slot, kTmemCols);
+    tc::tmem_relinquish();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_begin();
+
+  if (warp == 0) {
+    // -------------------------------------------------------------- TMA producer
+    if (tc::elect_one()) {
+      tc::tma_prefetch(&p.q);
+      tc::tma_prefetch(&p.k);
+      tc::tma_prefetch(&p.v);
+      uint32_t kn = 0, vn = 0, qn[2] = {0, 0};
+      bool ok = true;
+      for (int idx = blockIdx.x; idx < p.items && ok && !*abort_flag.cta; idx += gridDim.x) {
+        const Item it = item_of<QT, BN>(p, idx);
+#pragma unroll
+        for (int x = 0; x < QT; ++x) {
+          if (!it.any[x] || !ok) continue;
+          if (!(ok = wait_or_abort(q_empty + x, qn[x] + 1, abort_flag))) break;
+          tc::mbar_arrive_expect_tx(q_full + x, L::kQTile);
+          ++qn[x];
+          for (int pl = 0; pl < NP; ++pl)
+            for (int c = 0; c < kBoxes; ++c)
+              tc::tma_load_5d(smem + L::kQ + x * L::kQTile + (pl * kBoxes + c) * 16384, &p.q,
+                              q_full + x, 64 * c, it.row[x], it.h[x], it.b, pl);
+        }
+        for (int j = 0; j < it.n && ok; ++j) {
+          const int key = key_of<BN>(it, j);
+          const uint32_t ks = kn % KS, vs = vn % VS;
+          if (!(ok = wait_or_abort(k_empty + ks, kn / KS + 1, abort_flag))) break;
+          tc::mbar_arrive_expect_tx(k_full + ks, L::kKTile);
+          for (int pl = 0; pl < NP; ++pl)
+            for (int c = 0; c < kBoxes; ++c)
+              tc::tma_load_5d(smem + L::kK + ks * L::kKTile + (pl * kBoxes + c) * BN * 128, &p.k,
+                              k_full + ks, 64 * c, key, it.kh, it.b, pl);
+          ++kn;
+          if (!(ok = wait_or_abort(v_empty + vs, vn / VS + 1, abort_flag))) break;
+          tc::mbar_arrive_expect_tx(v_full + vs, L::kKTile);
+          for (int pl = 0; pl < NP; ++pl)
+            for (int c = 0; c < kBoxes; ++c)
+              tc::tma_load_5d(smem + L::kV + vs * L::kKTile + (pl * kBoxes + c) * BN * 128, &p.v,
+                              v_full + vs, 64 * c, key, it.kh, it.b, pl);
+          ++vn;
+        }
+      }
+      // Every load issued must have landed before the CTA exits: the last one of each barrier.
+      for (int x = 0; x < QT; ++x)
+        if (qn[x]) wait_or_abort(q_full + x, qn[x] - 1, abort_flag);
+      for (uint32_t i = kn > KS ? kn - KS : 0; i < kn; ++i)
+        wait_or_abort(k_full + i % KS, i / KS, abort_flag);
+      for (uint32_t i = vn > VS ? vn - VS : 0; i < vn; ++i)
+        wait_or_abort(v_full + i % VS, i / VS, abort_flag);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    // -------------------------------------------------------------- product issuer
+    if (tc::elect_one()) {
+      const uint32_t idesc_s = tc::idesc_bf16(128, BN, 0, 0);
+      const uint32_t idesc_o = tc::idesc_bf16(128, 16 * p.ksteps, 0, 1);
+      const uint32_t q_addr = tc::smem_u32(smem + L::kQ), k_addr = tc::smem_u32(smem + L::kK),
+                     v_addr = tc::smem_u32(smem + L::kV);
+      uint32_t base = 0, qn[2] = {0, 0}, pn[2] = {0, 0}, on[2] = {0, 0};
+      bool ok = true;
+      for (int idx = blockIdx.x; idx < p.items && ok && !*abort_flag.cta; idx += gridDim.x) {
+        const Item it = item_of<QT, BN>(p, idx);
+        int issued[2] = {it.n, it.n};  // the last tile whose scores were issued; n: none ever
+#pragma unroll
+        for (int x = 0; x < QT; ++x)
+          if (it.any[x]) issued[x] = -1;
+        // Scores of tile j; K_j is free once every query tile that uses it has issued its own.
+        auto scores = [&](int x, int j) -> bool {
+          const uint32_t st = (base + j) % KS;
+          if (!wait_or_abort(k_full + st, (base + j) / KS, abort_flag)) return false;
+          tc::tc_fence_after();
+          const uint32_t qa = q_addr + x * L::kQTile, ka = k_addr + st * L::kKTile;
+          uint32_t acc = 0;
+#pragma unroll
+          for (int pr = 0; pr < kProducts<NP>; ++pr)
+#pragma unroll
+            for (int ks = 0; ks < DH / 16; ++ks)
+              if (ks < p.ksteps) {
+                tc::mma_f16(tmem + x * L::kCols,
+                            kmajor(qa + plane_a<NP>(pr) * kBoxes * 16384, 128, ks),
+                            kmajor(ka + plane_b<NP>(pr) * kBoxes * BN * 128, BN, ks), idesc_s, acc);
+                acc = 1;
+              }
+          tc::mma_commit(s_full + x);
+          issued[x] = j;
+          const int y = x ^ 1;
+          if (QT == 1 || !it.any[y] || next_tile(it, y, j) != j || issued[y] >= j)
+            tc::mma_commit(k_empty + st);
+          if (next_tile(it, x, j + 1) == it.n) tc::mma_commit(q_empty + x);
+          return true;
+        };
+#pragma unroll
+        for (int x = 0; x < QT; ++x) {
+          if (!ok || !it.any[x]) continue;
+          if (!(ok = wait_or_abort(q_full + x, qn[x], abort_flag))) break;
+          ++qn[x];
+          if (next_tile(it, x, 0) == 0) ok = scores(x, 0);
+        }
+        for (int j = 0; j < it.n && ok; ++j) {
+          const uint32_t st = (base + j) % VS;
+#pragma unroll
+          for (int x = 0; x < QT; ++x) {
+            if (!ok || !it.any[x]) continue;
+            if (next_tile(it, x, j) == j) {
+              if (!(ok = wait_or_abort(p_full + x, pn[x], abort_flag))) break;
+              ++pn[x];
+              const bool first = next_tile(it, x, 0) == j;
+              if (first && !(ok = wait_or_abort(o_empty + x, on[x] + 1, abort_flag))) break;
+              if (!(ok = wait_or_abort(v_full + st, (base + j) / VS, abort_flag))) break;
+              tc::tc_fence_after();
+              uint32_t acc = NP == 1 && !first;
+              const uint32_t va = v_addr + st * L::kKTile;
+#pragma unroll
+              for (int pr = 0; pr < kProducts<NP>; ++pr)
+#pragma unroll
+                for (int ks = 0; ks < BN / 16; ++ks) {
+                  tc::mma_f16_ts(tmem + x * L::kCols + L::kS,
+                                 tmem + x * L::kCols + plane_a<NP>(pr) * (BN / 2) + ks * 8,
+                                 mnmajor(va + plane_b<NP>(pr) * kBoxes * BN * 128, BN, ks), idesc_o,
+                                 acc);
+                  acc = 1;
+                }
+              if (next_tile(it, x, j + 1) == it.n) {
+                tc::mma_commit(o_full + x);
+                ++on[x];
+              }
+            }
+            // The next scores overwrite P, which the product above reads: one thread's products run
+            // in the order of their issue. Never more than one tile ahead of the products over
+            // keys, so that a query tile that skips tiles cannot wait for a stage still in use.
+            if (j + 1 < it.n && next_tile(it, x, j + 1) == j + 1) ok = scores(x, j + 1);
+          }
+          if (ok) tc::mma_commit(v_empty + st);
+        }
+        base += it.n;
+      }
+      tc::mma_commit(drain);
+      wait_or_abort(drain, 0, abort_flag);
+    }
+    __syncwarp();
+  } else {
+    // -------------------------------------------------------------- softmax
+    const int x = (warp - 2) >> 2;
+    const uint32_t quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const uint32_t lanes = tmem + ((quarter * 32) << 16) + x * L::kCols;
+    uint32_t base = 0, sn = 0, on = 0;
+    bool ok = true;
+    for (int idx = blockIdx.x; idx < p.items && ok; idx += gridDim.x) {
+      const Item it = item_of<QT, BN>(p, idx);
+      const int row = it.row[x], pos = it.s.p0 + row + r;
+      const bool valid = row + r < w.q_len && pos >= 0 && pos < it.s.n;
+      const int first_pos = it.s.p0 + row + static_cast<int>(quarter) * 32;  // of this warp
+      float m = -INFINITY, sum = 0.f, pending = 0.f;
+      int done = 0;
+      if (it.any[x]) {
+        for (int j = next_tile(it, x, 0); j < it.n && ok; j = next_tile(it, x, j + 1), ++done) {
+          const int key = key_of<BN>(it, j);
+          if (!(ok = wait_or_abort(s_full + x, sn, abort_flag))) break;
+          ++sn;
+          tc::tc_fence_after();
+          if constexpr (NP > 1) {
+            // s_full also tells that the product over the previous tile is complete.
+            if (done) {
+#pragma unroll 1
+              for (int c = 0; c < DH / 32; ++c) {
+                uint32_t o[32], a[32];
+                tc::tmem_load_2x32(lanes + L::kS + c * 32, lanes + L::kS + DH + c * 32, o, a);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                  const float u = __uint_as_float(o[e]);
+                  o[e] = __float_as_uint(done > 1 ? fmaf(__uint_as_float(a[e]), pending, u) : u);
+                }
+                tc::tmem_store_32x32(lanes + L::kS + DH + c * 32, o);
+              }
+            }
+          }
+          uint32_t v[BN / 32][32];
+#pragma unroll
+          for (int c = 0; c < BN / 64; ++c)
+            tc::tmem_load_2x32(lanes + c * 64, lanes + c * 64 + 32, v[2 * c], v[2 * c + 1]);
+          // Keys of this tile that this row sees: c <= last and (c >= near or c < kept).
+          const bool all_seen = key + BN - 1 <= first_pos && first_pos + 31 < it.s.n && first_pos >= 0 &&
+                                (j < it.ns ? key + BN <= w.sinks
+                                           : key > first_pos + 31 - w.window || key + BN <= w.sinks);
+          if (!all_seen) {
+            int last = min(pos, it.s.n - 1) - key;
+            if (j < it.ns) last = min(last, w.sinks - 1 - key);
+            if (!valid) last = -1;
+            const int near = pos - w.window + 1 - key, kept = w.sinks - key;
+#pragma unroll
+            for (int c = 0; c < BN; ++c)
+              if (c > last || (c < near && c >= kept)) v[c / 32][c % 32] = 0xff800000u;
+          }
+          float mxs[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) mxs[i] = -INFINITY;
+#pragma unroll
+          for (int c = 0; c < BN; ++c) mxs[c & 7] = fmaxf(mxs[c & 7], __uint_as_float(v[c / 32][c % 32]));
+          const float mx = fmaxf(fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])),
+                                 fmaxf(fmaxf(mxs[4], mxs[5]), fmaxf(mxs[6], mxs[7]))) * p.scale_log2;
+          const bool move = m == -INFINITY ? mx > m : mx > m + kRescaleLog2;
+          float f = 1.f;
+          if (move) {
+            f = ex2(m - mx);
+            m = mx;
+            sum *= f;
+          }
+          if constexpr (NP == 1) {
+            // O follows the new maximum (s_full: the last O += P V is complete).
+            if (done && __any_sync(0xffffffffu, move)) {
+#pragma unroll 1
+              for (int c = 0; c < DH / 32; ++c) {
+                uint32_t o[32];
+                tc::tmem_load_32x32(lanes + L::kS + c * 32, o);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                tc::tmem_store_32x32(lanes + L::kS + c * 32, o);
+              }
+            }
+          } else {
+            pending = f;
+          }
+          const float base_m = m == -INFINITY ? 0.f : m;
+          float sums[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int half = 0; half < BN / 64; ++half) {
+            float pr[64];
+#pragma unroll
+            for (int c = 0; c < 64; ++c) {
+              const int at = half * 64 + c;
+              pr[c] = ex2(fmaf(__uint_as_float(v[at / 32][at % 32]), p.scale_log2, -base_m));
+              sums[c & 3] += pr[c];
+            }
+            store_planes<NP, 64>(lanes + half * 32, BN / 2, pr);
+          }
+          sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+          // Value rows behind the sequence may hold anything, and 0 times NaN is NaN: clear them.
+          if (key + BN > it.s.n && it.s.n < w.kv_len) {
+            const uint32_t st = (base + j) % VS;
+            if (!(ok = wait_or_abort(v_full + st, (base + j) / VS, abort_flag))) break;
+            uint8_t* vt = smem + L::kV + st * L::kKTile;
+            for (int i = (max(0, it.s.n - key)) * 8 + r; i < BN * 8; i += 128)
+              for (int box = 0; box < NP * kBoxes; ++box)
+                *reinterpret_cast<uint4*>(vt + box * BN * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+            tc::fence_proxy_async_smem();
+          }
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(p_full + x);
+        }
+        if (!ok) break;
+        if (!(ok = wait_or_abort(o_full + x, on, abort_flag))) break;
+        ++on;
+        tc::tc_fence_after();
+      }
+      base += it.n;
+      const bool stored = row + r < w.q_len;
+      const float inv = valid ? 1.f / sum : 0.f;
+#pragma unroll 1
+      for (int c = 0; c < DH / 32; ++c) {
+        float o[32];
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = 0.f;
+        if (it.any[x]) {
+          uint32_t u[32];
+          if constexpr (NP == 1) {
+            tc::tmem_load_32x32(lanes + L::kS + c * 32, u);
+          } else {
+            uint32_t a[32];
+            tc::tmem_load_2x32(lanes + L::kS + c * 32, lanes + L::kS + DH + c * 32, u, a);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (done > 1) u[e] = __float_as_uint(fmaf(__uint_as_float(a[e]), pending, __uint_as_float(u[e])));
+          }
+          if (valid) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(u[e]) * inv;
+          }
+        }
+        if (stored) {
+          if constexpr (NP == 1) {
+            __nv_bfloat16* dst = row_out<__nv_bfloat16>(w.out, it.b, row + r, it.h[x]) + c * 32;
+#pragma unroll
+            for (int e = 0; e < 32; e += 8)
+              if (c * 32 + e < w.head_dim)
+                *reinterpret_cast<uint4*>(dst + e) =
+                    make_uint4(pack_bf16(o[e], o[e + 1]), pack_bf16(o[e + 2], o[e + 3]),
+                               pack_bf16(o[e + 4], o[e + 5]), pack_bf16(o[e + 6], o[e + 7]));
+          } else {
+            float* dst = row_out<float>(w.out, it.b, row + r, it.h[x]) + c * 32;
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              if (c * 32 + e < w.head_dim)
+                *reinterpret_cast<float4*>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+      }
+      if (it.any[x]) {
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(o_empty + x);
+      }
+      if (stored && w.lse)
+        w.lse[(static_cast<uint64_t>(it.b) * w.heads + it.h[x]) * w.q_len + row + r] =
+            valid ? m * kLn2 + logf(sum) : -INFINITY;
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  if (warp == 1) tc::tmem_dealloc(tmem, kTmemCols);
+}
+
+// The three bf16 planes of an fp32 view, [plane][batch][head][token][dim], in units of four elements.
+struct SplitParams {
+  View src[4];
+  uint16_t* dst[4];
+  uint64_t plane[4];  // elements of one plane
+  uint64_t units[4];  // running totals of groups of four elements
+  int tokens[4], heads[4];
+  int dim4;
+};
+__global__ void __launch_bounds__(256) split_planes_kernel(const __grid_constant__ SplitParams p) {
+  pdl_begin();
+  const uint64_t u = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  int s = 0;
+  while (s < 4 && u >= p.units[s]) ++s;
+  if (s == 4) return;
+  const uint64_t i = u - (s ? p.units[s - 1] : 0);
+  const int e = static_cast<int>(i % p.dim4);
+  uint64_t row = i / p.dim4;
+  const int t = static_cast<int>(row % p.tokens[s]);
+  row /= p.tokens[s];
+  const int h = static_cast<int>(row % p.heads[s]), b = static_cast<int>(row / p.heads[s]);
+  float4 v = *reinterpret_cast<const float4*>(row_ptr<float>(p.src[s], b, t, h) + 4 * e);
+#pragma unroll
+  for (int pl = 0; pl < 3; ++pl) {
+    const uint32_t lo = take_upper(v.x, v.y), hi = take_upper(v.z, v.w);
+    *reinterpret_cast<uint2*>(p.dst[s] + pl * p.plane[s] + 4 * i) = make_uint2(lo, hi);
+  }
+}
+
+// ------------------------------------------------------------------------------- host side
+// bf16 view as a 5-D map (element, token, head, batch, plane), boxes of 64 elements x `rows`.
+bool make_view_map(CUtensorMap* map, const void* base, const uint64_t (&dims)[5],
+                   const uint64_t (&strides)[4], uint32_t rows) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t d[5], s[4];
+  for (int i = 0; i < 5; ++i) d[i] = dims[i];
+  for (int i = 0; i < 4; ++i) s[i] = dims[i + 1] > 1 ? strides[i] * 2 : 16;
+  cuuint32_t box[5] = {64, rows, 1, 1, 1}, unit[5] = {1, 1, 1, 1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), d, s, box, unit,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+uint64_t round256(uint64_t v) { return (v + 255) & ~255ull; }
+
+// A bf16 view in place, or the planes of an fp32 one.
+struct Operand {
+  const View* view;
+  uint64_t tokens, heads;
+  uint16_t* planes;
+};
+bool operand_map(CUtensorMap* map, const WindowParams& w, const Operand& o, uint32_t rows) {
+  const uint64_t d = w.head_dim, b = w.batch;
+  if (w.dtype == SPAR_B200_BFLOAT16)
+    return make_view_map(map, o.view->data, {d, o.tokens, o.heads, b, 1},
+                         {o.view->token, o.view->head, o.view->batch, 8}, rows);
+  return make_view_map(map, o.planes, {d, o.tokens, o.heads, b, 3},
+                       {d, d * o.tokens, d * o.tokens * o.heads, d * o.tokens * o.heads * b}, rows);
+}
+uint64_t planes_bytes(const WindowParams& w, uint64_t tokens, uint64_t heads) {
+  return w.dtype == SPAR_B200_BFLOAT16
+             ? 0
+             : round256(6ull * w.batch * tokens * heads * static_cast<uint64_t>(w.head_dim));
+}
+
+cudaError_t split(const WindowParams& w, const Operand* o, int n, cudaStream_t stream) {
+  SplitParams p = {};
+  p.dim4 = w.head_dim / 4;
+  uint64_t total = 0;
+  for (int i = 0; i < 4; ++i) {
+    if (i < n) {
+      p.src[i] = *o[i].view;
+      p.dst[i] = o[i].planes;
+      p.tokens[i] = static_cast<int>(o[i].tokens);
+      p.heads[i] = static_cast<int>(o[i].heads);
+      const uint64_t elements = w.batch * o[i].tokens * o[i].heads * static_cast<uint64_t>(w.head_dim);
+      p.plane[i] = elements;
+      total += elements / 4;
+    }
+    p.units[i] = total;
+  }
+  return launch(split_planes_kernel, dim3(static_cast<unsigned>((total + 255) / 256)), dim3(256), 0,
+                stream, p);
+}
+
+// A view that TMA and 16-byte accesses can address: 16-byte rows, no broadcast dimension.
+bool tiled_view(const View& v, int size, uint64_t batch, uint64_t tokens, uint64_t heads) {
+  const uint64_t n = 16 / size;
+  const uint64_t extent[3] = {batch, tokens, heads}, stride[3] = {v.batch, v.token, v.head};
+  if (reinterpret_cast<uintptr_t>(v.data) & 15) return false;
+  for (int i = 0; i < 3; ++i)
+    if (extent[i] > 1 && (stride[i] % n || stride[i] == 0 || stride[i] * size >= (1ull << 40)))
+      return false;
+  return true;
+}
+
+template <int DH, int NP, int QT, int BN, int KS, int VS>
+cudaError_t launch_forward(TcParams& p, int device, cudaStream_t stream) {
+  using L = Fwd<DH, NP, QT, BN, KS, VS>;
+  auto kernel = window_forward_kernel<DH, NP, QT, BN, KS, VS>;
+  const cudaError_t e = raise_dynamic_smem(reinterpret_cast<const void*>(kernel), device, L::kSmem);
+  if (e != cudaSuccess) return e;
+  const WindowParams& w = p.w;
+  p.tiles = (w.q_len + 127) / 128;
+  p.pair_heads = QT == 2 && w.group % 2 == 0;
+  const int64_t per = p.pair_heads ? w.heads / 2 : w.heads;
+  p.items = static_cast<int>(w.batch * per * (p.pair_heads ? p.tiles : (p.tiles + QT - 1) / QT));
+  const unsigned grid = static_cast<unsigned>(std::min(p.items, sm_count(device)));
+  return launch(kernel, dim3(grid), dim3(64 + 128 * QT), L::kSmem, stream, p);
+}
+
+}  // namespace
+
+bool tc_supported(const WindowParams& w, bool backward) {
+  if (backward) return false;
+  if (w.head_dim % 8 || w.head_dim > 128) return false;
+  const int size = w.dtype == SPAR_B200_FLOAT32 ? 4 : 2;
+  return w.kv_len > 0 && tiled_view(w.q, size, w.batch, w.q_len, w.heads) &&
+         tiled_view(w.k, size, w.batch, w.kv_len, w.kv_heads) &&
+         tiled_view(w.v, size, w.batch, w.kv_len, w.kv_heads) &&
+         tiled_view(w.out, size, w.batch, w.q_len, w.heads);
+}
+
+uint64_t tc_scratch_bytes(const WindowParams& w, bool backward, int device) {
+  (void)device;
+  (void)backward;
+  return planes_bytes(w, w.q_len, w.heads) + 2 * planes_bytes(w, w.kv_len, w.kv_heads);
+}
+
+cudaError_t tc_forward(const WindowParams& w, void* scratch, int device, cudaStream_t stream) {
+  TcParams p;
+  memset(&p, 0, sizeof(p));
+  p.w = w;
+  p.wait_flag = attention_wait_flag(device);
+  if (!p.wait_flag) return cudaErrorInvalidDevice;
+  p.ksteps = (w.head_dim + 15) / 16;
+  p.scale_log2 = w.scale * kLog2e;
+  char* at = static_cast<char*>(scratch);
+  Operand o[3] = {{&w.q, static_cast<uint64_t>(w.q_len), static_cast<uint64_t>(w.heads), nullptr},
+                  {&w.k, static_cast<uint64_t>(w.kv_len), static_cast<uint64_t>(w.kv_heads), nullptr},
+                  {&w.v, static_cast<uint64_t>(w.kv_len), static_cast<uint64_t>(w.kv_heads), nullptr}};
+  for (Operand& x : o) {
+    x.planes = reinterpret_cast<uint16_t*>(at);
+    at += planes_bytes(w, x.tokens, x.heads);
+  }
+  const bool wide = w.head_dim > 64, f32 = w.dtype == SPAR_B200_FLOAT32;
+  const uint32_t rows = f32 ? 64 : 128;
+  if (!operand_map(&p.q, w, o[0], 128) || !operand_map(&p.k, w, o[1], rows) ||
+      !operand_map(&p.v, w, o[2], rows))
+    return cudaErrorInvalidValue;
+  if (f32) {
+    const cudaError_t e = split(w, o, 3, stream);
+    if (e != cudaSuccess) return e;
+    return wide ? launch_forward<128, 3, 1, 64, 1, 1>(p, device, stream)
+                : launch_forward<64, 3, 2, 64, 2, 2>(p, device, stream);
+  }
+  return wide ? launch_forward<128, 1, 2, 128, 2, 2>(p, device, stream)
+              : launch_forward<64, 1, 2, 128, 3, 3>(p, device, stream);
+}
+
+}  // namespace window
+}  // namespace spar_b200

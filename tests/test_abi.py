@@ -157,7 +157,7 @@ def test_rotary_and_window_attention_refuse_bad_calls_without_gpu():
     for bad in (dict(dtype=7), dict(heads=0), dict(kv_heads=0), dict(kv_heads=3), dict(kv_heads=8),
                 dict(head_dim=0), dict(head_dim=257), dict(window=0), dict(scale=-1.0),
                 dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None), dict(k=at + 1),
-                dict(q_len=1 << 30), dict(kv_len=1 << 40), dict(batch=1 << 29, heads=64, kv_heads=64),
+                dict(q_len=1 << 29), dict(kv_len=1 << 40), dict(batch=1 << 29, heads=64, kv_heads=64),
                 dict(batch=1 << 12, kv_len=1 << 20)):
         assert lib.spar_b200_window_attention_forward(window(**bad), 0, None).code == 1, bad
         assert lib.spar_b200_window_attention_backward(window(**bad), 0, None).code == 1, bad
