@@ -61,6 +61,7 @@ __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bf
 bool tc_supported(const WindowParams& w, bool backward);
 uint64_t tc_scratch_bytes(const WindowParams& w, bool backward, int device);
 cudaError_t tc_forward(const WindowParams& w, void* scratch, int device, cudaStream_t stream);
+cudaError_t tc_backward(const WindowParams& w, void* scratch, int device, cudaStream_t stream);
 
 }  // namespace window
 }  // namespace spar_b200

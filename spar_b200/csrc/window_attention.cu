@@ -339,7 +339,11 @@ extern "C" SparCudaStatus spar_b200_window_attention_backward(const SparB200Wind
   DeviceScope scope(device);
   if (scope.error() != cudaSuccess) return runtime(scope.error());
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = w.dtype == SPAR_B200_FLOAT32 ? row_path<float>(w, true, s)
-                                                     : row_path<__nv_bfloat16>(w, true, s);
+  cudaError_t e;
+  if (plan.tiled)
+    e = tc_backward(w, static_cast<char*>(a->scratch) + plan.delta_bytes, device, s);
+  else
+    e = w.dtype == SPAR_B200_FLOAT32 ? row_path<float>(w, true, s)
+                                     : row_path<__nv_bfloat16>(w, true, s);
   return e == cudaSuccess ? launch_status() : runtime(e);
 }

@@ -129,6 +129,37 @@ struct Item {
   bool any[2];
 };
 
+// Fills in the keys of an item whose heads and rows are set.
+template <int QT, int BN>
+__device__ __forceinline__ void place_keys(const WindowParams& w, Item& it) {
+  it.kh = it.h[0] / w.group;
+  it.s = sequence_of(w, it.b);
+  int lo[2], hi[2], ulo = INT_MAX, uhi = -1;
+#pragma unroll
+  for (int x = 0; x < QT; ++x) {
+    const int rows = min(128, w.q_len - it.row[x]);
+    const int pa = max(it.s.p0 + it.row[x], 0), pb = min(it.s.p0 + it.row[x] + rows - 1, it.s.n - 1);
+    it.any[x] = rows > 0 && pb >= pa;
+    lo[x] = max(0, pa - w.window + 1);
+    hi[x] = pb;
+    if (it.any[x]) {
+      ulo = min(ulo, lo[x]);
+      uhi = max(uhi, hi[x]);
+    }
+  }
+  it.ns = it.n = it.start = 0;
+  if (uhi < 0) return;
+  const bool apart = w.sinks > 0 && ulo > w.sinks;
+  it.start = w.sinks > 0 && !apart ? 0 : ulo;
+  it.ns = apart ? (w.sinks + BN - 1) / BN : 0;
+  it.n = it.ns + (uhi - it.start) / BN + 1;
+#pragma unroll
+  for (int x = 0; x < QT; ++x) {
+    it.a[x] = w.sinks > 0 && !apart ? 0 : (lo[x] - it.start) / BN;
+    it.b_end[x] = (hi[x] - it.start) / BN + 1;
+  }
+}
+
 template <int QT, int BN>
 __device__ __forceinline__ Item item_of(const TcParams& p, int idx) {
   const WindowParams& w = p.w;
@@ -149,32 +180,19 @@ __device__ __forceinline__ Item item_of(const TcParams& p, int idx) {
     it.row[0] = t * 128 * QT;
     it.row[1] = it.row[0] + 128;
   }
-  it.kh = it.h[0] / w.group;
-  it.s = sequence_of(w, it.b);
-  int lo[2], hi[2], ulo = INT_MAX, uhi = -1;
-#pragma unroll
-  for (int x = 0; x < QT; ++x) {
-    const int rows = min(128, w.q_len - it.row[x]);
-    const int pa = max(it.s.p0 + it.row[x], 0), pb = min(it.s.p0 + it.row[x] + rows - 1, it.s.n - 1);
-    it.any[x] = rows > 0 && pb >= pa;
-    lo[x] = max(0, pa - w.window + 1);
-    hi[x] = pb;
-    if (it.any[x]) {
-      ulo = min(ulo, lo[x]);
-      uhi = max(uhi, hi[x]);
-    }
-  }
-  it.ns = it.n = it.start = 0;
-  if (uhi < 0) return it;
-  const bool apart = w.sinks > 0 && ulo > w.sinks;
-  it.start = w.sinks > 0 && !apart ? 0 : ulo;
-  it.ns = apart ? (w.sinks + BN - 1) / BN : 0;
-  it.n = it.ns + (uhi - it.start) / BN + 1;
-#pragma unroll
-  for (int x = 0; x < QT; ++x) {
-    it.a[x] = w.sinks > 0 && !apart ? 0 : (lo[x] - it.start) / BN;
-    it.b_end[x] = (hi[x] - it.start) / BN + 1;
-  }
+  place_keys<QT, BN>(w, it);
+  return it;
+}
+// The item of one query tile: the last rows first (they see the most keys).
+template <int BN>
+__device__ __forceinline__ Item item_of_tile(const WindowParams& w, int idx) {
+  const int per = w.batch * w.heads, t = (w.q_len + 127) / 128 - 1 - idx / per;
+  const int bh = idx % per;
+  Item it;
+  it.b = bh / w.heads;
+  it.h[0] = bh - it.b * w.heads;
+  it.row[0] = t * 128;
+  place_keys<1, BN>(w, it);
   return it;
 }
 // The next tile of query tile x from j on, or n.
@@ -572,6 +590,579 @@ __global__ void __launch_bounds__(64 + 128 * QT, 1) window_forward_kernel(
   if (warp == 1) tc::tmem_dealloc(tmem, kTmemCols);
 }
 
+// ============================================================================ backward
+// Two launches of one kernel, after D = rowsum(dout o out):
+//   queries (KEYS = false)  stationary: 128 rows of q and dout; moving: 64 rows of k and v
+//       S = q k^T, dP = dout v^T;  dS = P o (dP - D);  dq += dS k
+//   keys (KEYS = true)      stationary: 128 rows of k and v; moving: 64 rows of q and dout, for
+//       every query head of the group: S^T = k q^T, dP^T = v dout^T;  dv += P^T dout;  dk += dS^T q
+// P = exp(S - lse) is recomputed on both sides, so every gradient element is summed in one CTA and
+// no order is left to chance. P and dS replace S and dP in TMEM and are read there as the A operand.
+// All eight softmax warps work on every tile (thread = stationary row, half of the 64 columns);
+// with two buffers the next tile's S and dP run meanwhile. `scale` is applied to dq and dk at the
+// end.
+// First tokens are seen by every later row: their key tiles' rows are cut into chunks of
+// `chunk` rows that are items of their own (and, where there are few key tiles, so are groups of
+// query heads); such items leave fp32 partial sums that a last launch adds in order.
+constexpr int kMoving = 64;
+
+struct BackwardParams {
+  WindowParams w;
+  CUtensorMap s1, s2, m1, m2;  // stationary and moving operands: q, dout / k, v or k, v / q, dout
+  int* wait_flag;
+  int items, tiles, ksteps;
+  float scale_log2;
+  // keys: the first `first_tiles` key tiles are cut into `chunks` row ranges, every tile into
+  // `head_parts` groups of query heads.
+  int first_tiles, chunks, chunk, head_parts;
+  float* partial;  // [part][2][128][head_dim]: dk, dv
+};
+
+// Which part of the key side an item is: batch, key head, tile, rows, heads; `slot`: its partial,
+// or -1 when it is the tile's only item.
+struct KeyItem {
+  int b, kh, key, row, jobs_per_head, head, heads, end;
+  Sequence s;
+  int64_t slot;
+};
+__device__ __forceinline__ KeyItem key_item(const BackwardParams& p, int idx) {
+  const WindowParams& w = p.w;
+  const int bk = w.batch * w.kv_heads, first_items = p.first_tiles * bk * p.chunks * p.head_parts;
+  KeyItem it;
+  int part, which, tile, from = 0, to = w.q_len;
+  if (idx < first_items) {
+    const int parts = p.chunks * p.head_parts;
+    part = idx % parts;
+    const int rest = idx / parts;
+    which = rest % bk;
+    tile = rest / bk;
+    from = (part / p.head_parts) * p.chunk;
+    to = min(from + p.chunk, w.q_len);
+    it.slot = parts > 1 ? idx : -1;
+    part %= p.head_parts;
+  } else {
+    const int i = idx - first_items;
+    part = i % p.head_parts;
+    const int rest = i / p.head_parts;
+    which = rest % bk;
+    tile = p.first_tiles + rest / bk;
+    it.slot = p.head_parts > 1 ? idx : -1;
+  }
+  it.b = which / w.kv_heads;
+  it.kh = which - it.b * w.kv_heads;
+  it.key = tile * 128;
+  it.s = sequence_of(w, it.b);
+  it.head = it.kh * w.group + w.group * part / p.head_parts;
+  it.heads = it.kh * w.group + w.group * (part + 1) / p.head_parts - it.head;
+  // rows that see a key of the tile: positions key .. last key + window - 1 (first tokens: n - 1)
+  const int last_key = min(it.key + 127, it.s.n - 1);
+  const int far = it.key < w.sinks ? it.s.n - 1 : min(it.s.n - 1, last_key + w.window - 1);
+  it.row = max(from, it.key - it.s.p0);
+  it.end = min(to, far - it.s.p0 + 1);
+  it.jobs_per_head =
+      last_key >= it.key && it.end > it.row ? (it.end - it.row + kMoving - 1) / kMoving : 0;
+  return it;
+}
+
+template <bool KEYS, int DH, int NP, int ST>
+struct Bwd {
+  static constexpr int kBuffers = KEYS && NP > 1 ? 1 : 2;
+  static constexpr uint32_t kStat = NP * DH * 256;            // one stationary operand
+  static constexpr uint32_t kMov = NP * DH * kMoving * 2;     // one moving operand
+  static constexpr uint32_t kA = 0;
+  static constexpr uint32_t kB = kA + 2 * kStat;
+  static constexpr uint32_t kRows = kB + ST * 2 * kMov;       // [ST][64] (lse log2 e, D)
+  static constexpr uint32_t kBar = kRows + (KEYS ? ST * kMoving * 8 : 0);
+  static constexpr uint32_t kSmem = kBar + 256 + 1024;
+  static_assert(kSmem <= kMaxSmem, "backward shared memory");
+  // TMEM: buffers of S | dP (| the third planes of P and dS), then the products' sums, then
+  // (NP = 3) the sums of earlier tiles.
+  static constexpr uint32_t kBuf = KEYS && NP > 1 ? 192 : 128;
+  static constexpr uint32_t kAcc = kBuffers * kBuf;
+  static constexpr uint32_t kOuts = KEYS ? 2 : 1;
+  static constexpr uint32_t kSum = kAcc + kOuts * DH;
+  static_assert(kAcc + kOuts * DH * (NP > 1 ? 2 : 1) <= kTmemCols, "backward TMEM");
+};
+
+// Column (in a buffer) of plane pl of K step ks of the operand that overwrites S (which = 0) or dP
+// (which = 1). Columns 32 g .. 32 g + 31 of S and dP are read by softmax group g alone, and it
+// alone overwrites them (two steps of 16 values, 8 columns each, of two planes); third planes go
+// to columns nobody reads.
+template <bool KEYS>
+__host__ __device__ constexpr uint32_t operand_col(int which, int pl, int ks) {
+  const int g = ks >> 1, sub = (ks & 1) * 8;
+  if (pl < 2) return which * 64 + g * 32 + pl * 16 + sub;
+  return KEYS ? 128 + which * 32 + g * 16 + sub : 64 + g * 32 + sub;
+}
+
+template <bool KEYS, int DH, int NP, int ST>
+__global__ void __launch_bounds__(320, 1) window_backward_kernel(
+    const __grid_constant__ BackwardParams p) {
+  using L = Bwd<KEYS, DH, NP, ST>;
+  constexpr int kBoxes = DH / 64;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = align1024(smem_raw);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
+  uint64_t* a_full = bars;
+  uint64_t* a_empty = bars + 1;
+  uint64_t* s_full = bars + 2;    // [2]
+  uint64_t* pd_full = bars + 4;   // [2]
+  uint64_t* sum_full = bars + 6;  // the products of a tile (NP = 3) or item are complete
+  uint64_t* sum_empty = bars + 7;
+  uint64_t* drain = bars + 8;
+  uint64_t* m_full = bars + 9;    // [ST]
+  uint64_t* m_empty = m_full + ST;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(m_empty + ST);
+  const Abort abort_flag = {reinterpret_cast<volatile int*>(tmem_slot + 1), p.wait_flag};
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const WindowParams& w = p.w;
+
+  if (threadIdx.x == 0) {
+    tc::mbar_init(a_full, 1);
+    tc::mbar_init(a_empty, 1);
+    for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(s_full + i, 1);
+      tc::mbar_init(pd_full + i, 8);
+    }
+    tc::mbar_init(sum_full, 1);
+    tc::mbar_init(sum_empty, 8);
+    tc::mbar_init(drain, 1);
+    for (int i = 0; i < ST; ++i) {
+      tc::mbar_init(m_full + i, KEYS ? 2 : 1);  // TMA, and the rows' statistics
+      tc::mbar_init(m_empty + i, 1);
+    }
+    *abort_flag.cta = 0;
+    tc::fence_barrier_init();
+  }
+  if (warp == 1) {
+    tc::tmem_alloc(tmem_slot, kTmemCols);
+    tc::tmem_relinquish();
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_begin();
+
+  // Moving tiles of an item; both sides number them 0 .. n - 1.
+  auto jobs_of = [&](int idx, Item& q, KeyItem& k) -> int {
+    if constexpr (KEYS) {
+      k = key_item(p, idx);
+      return k.jobs_per_head * k.heads;
+    } else {
+      q = item_of_tile<kMoving>(w, idx);
+      return q.n;
+    }
+  };
+
+  if (warp == 0) {
+    // -------------------------------------------------------------- TMA producer (whole warp)
+    if (lane == 0) {
+      tc::tma_prefetch(&p.s1);
+      tc::tma_prefetch(&p.s2);
+      tc::tma_prefetch(&p.m1);
+      tc::tma_prefetch(&p.m2);
+    }
+    uint32_t an = 0, mn = 0;
+    bool ok = true;
+    for (int idx = blockIdx.x; idx < p.items && ok && !*abort_flag.cta; idx += gridDim.x) {
+      Item q;
+      KeyItem k;
+      const int n = jobs_of(idx, q, k);
+      if (!n) continue;
+      const int b = KEYS ? k.b : q.b;
+      if (!(ok = wait_or_abort(a_empty, an + 1, abort_flag))) break;
+      ++an;
+      if (lane == 0) {
+        tc::mbar_arrive_expect_tx(a_full, 2 * L::kStat);
+        for (int pl = 0; pl < NP; ++pl)
+          for (int c = 0; c < kBoxes; ++c) {
+            uint8_t* dst = smem + L::kA + (pl * kBoxes + c) * 16384;
+            const int row = KEYS ? k.key : q.row[0], h = KEYS ? k.kh : q.h[0];
+            tc::tma_load_5d(dst, &p.s1, a_full, 64 * c, row, h, b, pl);
+            tc::tma_load_5d(dst + L::kStat, &p.s2, a_full, 64 * c, row, h, b, pl);
+          }
+      }
+      __syncwarp();
+      for (int i = 0; i < n && ok; ++i, ++mn) {
+        const uint32_t st = mn % ST;
+        if (!(ok = wait_or_abort(m_empty + st, mn / ST + 1, abort_flag))) break;
+        int row, h;
+        if constexpr (KEYS) {
+          const int head = i / k.jobs_per_head;
+          row = k.row + (i - head * k.jobs_per_head) * kMoving;
+          h = k.head + head;
+        } else {
+          row = key_of<kMoving>(q, i);
+          h = q.kh;
+        }
+        if (lane == 0) {
+          tc::mbar_arrive_expect_tx(m_full + st, 2 * L::kMov);
+          for (int pl = 0; pl < NP; ++pl)
+            for (int c = 0; c < kBoxes; ++c) {
+              uint8_t* dst = smem + L::kB + st * 2 * L::kMov + (pl * kBoxes + c) * kMoving * 128;
+              tc::tma_load_5d(dst, &p.m1, m_full + st, 64 * c, row, h, b, pl);
+              tc::tma_load_5d(dst + L::kMov, &p.m2, m_full + st, 64 * c, row, h, b, pl);
+            }
+        }
+        if constexpr (KEYS) {
+          float2* stats = reinterpret_cast<float2*>(smem + L::kRows) + st * kMoving;
+          const uint64_t at = (static_cast<uint64_t>(b) * w.heads + h) * w.q_len;
+#pragma unroll
+          for (int e = lane; e < kMoving; e += 32) {
+            const bool in = row + e < k.end;
+            stats[e] = make_float2(in ? __ldg(w.lse + at + row + e) * kLog2e : 0.f,
+                                   in ? __ldg(w.delta + at + row + e) : 0.f);
+          }
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(m_full + st);
+        }
+        __syncwarp();
+      }
+    }
+    if (an) wait_or_abort(a_full, an - 1, abort_flag);
+    for (uint32_t i = mn > ST ? mn - ST : 0; i < mn; ++i)
+      wait_or_abort(m_full + i % ST, i / ST, abort_flag);
+  } else if (warp == 1) {
+    // -------------------------------------------------------------- product issuer
+    if (tc::elect_one()) {
+      const uint32_t idesc_s = tc::idesc_bf16(128, kMoving, 0, 0);
+      const uint32_t idesc_o = tc::idesc_bf16(128, 16 * p.ksteps, 0, 1);
+      const uint32_t a_addr = tc::smem_u32(smem + L::kA), b_addr = tc::smem_u32(smem + L::kB);
+      uint32_t an = 0, mn = 0, sums = 0;
+      bool ok = true;
+      // S and dP of moving tile number m; after the item's last one the stationary operands are free.
+      auto scores = [&](uint32_t m, bool last) -> bool {
+        const uint32_t st = m % ST, buf = tmem + (m % L::kBuffers) * L::kBuf;
+        if (!wait_or_abort(m_full + st, m / ST, abort_flag)) return false;
+        tc::tc_fence_after();
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const uint32_t a = a_addr + half * L::kStat, b = b_addr + (2 * st + half) * L::kMov;
+          uint32_t acc = 0;
+#pragma unroll
+          for (int pr = 0; pr < kProducts<NP>; ++pr)
+#pragma unroll
+            for (int ks = 0; ks < DH / 16; ++ks)
+              if (ks < p.ksteps) {
+                tc::mma_f16(buf + half * 64, kmajor(a + plane_a<NP>(pr) * kBoxes * 16384, 128, ks),
+                            kmajor(b + plane_b<NP>(pr) * kBoxes * kMoving * 128, kMoving, ks), idesc_s,
+                            acc);
+                acc = 1;
+              }
+        }
+        tc::mma_commit(s_full + m % L::kBuffers);
+        if (last) tc::mma_commit(a_empty);
+        return true;
+      };
+      for (int idx = blockIdx.x; idx < p.items && ok && !*abort_flag.cta; idx += gridDim.x) {
+        Item q;
+        KeyItem k;
+        const int n = jobs_of(idx, q, k);
+        if (!n) continue;
+        if (!(ok = wait_or_abort(a_full, an, abort_flag))) break;
+        ++an;
+        ok = scores(mn, n == 1);
+        for (int i = 0; i < n && ok; ++i) {
+          const uint32_t m = mn + i, st = m % ST, buf = tmem + (m % L::kBuffers) * L::kBuf;
+          // The other buffer was last read by the products of two tiles back, issued before.
+          if (L::kBuffers == 2 && i + 1 < n && !(ok = scores(m + 1, i + 2 == n))) break;
+          if (!(ok = wait_or_abort(pd_full + m % L::kBuffers, m / L::kBuffers, abort_flag))) break;
+          // Sums start afresh with an item; the softmax warps have read the ones before.
+          if (i == 0 && !(ok = wait_or_abort(sum_empty, sums + 1, abort_flag))) break;
+          tc::tc_fence_after();
+#pragma unroll
+          for (int out = 0; out < static_cast<int>(L::kOuts); ++out) {
+            // queries: dq += dS k; keys: dk += dS^T q, dv += P^T dout
+            const int which = KEYS ? 1 - out : 0;
+            const uint32_t b = b_addr + (2 * st + out) * L::kMov;
+            uint32_t acc = NP == 1 && i > 0;
+#pragma unroll
+            for (int pr = 0; pr < kProducts<NP>; ++pr)
+#pragma unroll
+              for (int ks = 0; ks < kMoving / 16; ++ks) {
+                tc::mma_f16_ts(tmem + L::kAcc + out * DH, buf + operand_col<KEYS>(which, plane_a<NP>(pr), ks),
+                               mnmajor(b + plane_b<NP>(pr) * kBoxes * kMoving * 128, kMoving, ks), idesc_o,
+                               acc);
+                acc = 1;
+              }
+          }
+          tc::mma_commit(m_empty + st);
+          if (NP > 1 || i + 1 == n) tc::mma_commit(sum_full);
+          if (L::kBuffers == 1 && i + 1 < n) ok = scores(m + 1, i + 2 == n);
+        }
+        mn += n;
+        ++sums;
+      }
+      tc::mma_commit(drain);
+      wait_or_abort(drain, 0, abort_flag);
+    }
+    __syncwarp();
+  } else {
+    // -------------------------------------------------------------- softmax and results
+    const int g = (warp - 2) >> 2;
+    const uint32_t quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const uint32_t lanes = tmem + ((quarter * 32) << 16);
+    uint32_t mn = 0, sums = 0;
+    bool ok = true;
+    // NP = 3: adds the last tile's products to the sums of the earlier ones; the groups share the
+    // columns.
+    auto add_sums = [&](bool first) {
+      constexpr int cols = L::kOuts * DH / 2;
+#pragma unroll 1
+      for (int c = g * cols; c < (g + 1) * cols; c += 32) {
+        uint32_t o[32], a[32];
+        tc::tmem_load_2x32(lanes + L::kAcc + c, lanes + L::kSum + c, o, a);
+        if (!first) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e)
+            o[e] = __float_as_uint(__uint_as_float(a[e]) + __uint_as_float(o[e]));
+        }
+        tc::tmem_store_32x32(lanes + L::kSum + c, o);
+      }
+    };
+    for (int idx = blockIdx.x; idx < p.items && ok; idx += gridDim.x) {
+      Item q;
+      KeyItem k;
+      const int n = jobs_of(idx, q, k);
+      const int b = KEYS ? k.b : q.b;
+      const Sequence s = KEYS ? k.s : q.s;
+      // queries: this row's position and statistics; keys: this row's key
+      const int row = (KEYS ? k.key : q.row[0]) + r;
+      const int pos = KEYS ? row : s.p0 + row;
+      const bool valid = KEYS ? row < s.n : row < w.q_len && pos >= 0 && pos < s.n;
+      float lse2 = 0.f, delta = 0.f;
+      if (!KEYS && valid && n) {
+        const uint64_t at = (static_cast<uint64_t>(b) * w.heads + q.h[0]) * w.q_len + row;
+        lse2 = __ldg(w.lse + at) * kLog2e;
+        delta = __ldg(w.delta + at);
+      }
+      for (int i = 0; i < n && ok; ++i) {
+        const uint32_t m = mn + i, st = m % ST;
+        const uint32_t buf = lanes + (m % L::kBuffers) * L::kBuf;
+        if (!(ok = wait_or_abort(s_full + m % L::kBuffers, m / L::kBuffers, abort_flag))) break;
+        tc::tc_fence_after();
+        uint32_t sv[32], dv[32];
+        tc::tmem_load_2x32(buf + g * 32, buf + 64 + g * 32, sv, dv);
+        const int c0 = g * 32;
+        float pr[32], ds[32];
+        int clear;  // moving rows from here on may hold anything
+        if constexpr (KEYS) {
+          const int head = i / k.jobs_per_head;
+          const int at = k.row + (i - head * k.jobs_per_head) * kMoving;  // first moving row
+          const int base = s.p0 + at;                                     // its position
+          clear = min(s.n - base, kMoving);
+          // This key is seen from columns lo .. hi; a warp's keys all by all of this group's
+          // columns?
+          const int lo = pos - base;
+          int hi = min(k.end - 1 - at, pos < w.sinks ? kMoving : pos - base + w.window - 1);
+          if (!valid) hi = -1;
+          const int k0 = k.key + static_cast<int>(quarter) * 32;
+          const bool all_seen = k0 + 31 <= base + c0 && at + c0 + 32 <= k.end && k0 + 31 < s.n &&
+                                (base + c0 + 31 < k0 + w.window || k0 + 32 <= w.sinks);
+          if (!(ok = wait_or_abort(m_full + st, m / ST, abort_flag))) break;
+          const float2* stats = reinterpret_cast<const float2*>(smem + L::kRows) + st * kMoving + c0;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float2 t = stats[e];
+            pr[e] = ex2(fmaf(__uint_as_float(sv[e]), p.scale_log2, -t.x));
+            ds[e] = pr[e] * (__uint_as_float(dv[e]) - t.y);
+          }
+          if (!all_seen) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (c0 + e < lo || c0 + e > hi) pr[e] = ds[e] = 0.f;
+          }
+        } else {
+          const int key = key_of<kMoving>(q, i);
+          clear = min(s.n - key, kMoving);
+          const int first_pos = s.p0 + q.row[0] + static_cast<int>(quarter) * 32;
+          const bool all_seen =
+              key + c0 + 31 <= first_pos && first_pos >= 0 && first_pos + 31 < s.n &&
+              first_pos + 31 < s.p0 + w.q_len &&
+              (i < q.ns ? key + c0 + 32 <= w.sinks
+                        : key + c0 > first_pos + 31 - w.window || key + c0 + 32 <= w.sinks);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            pr[e] = ex2(fmaf(__uint_as_float(sv[e]), p.scale_log2, -lse2));
+            ds[e] = pr[e] * (__uint_as_float(dv[e]) - delta);
+          }
+          if (!all_seen) {
+            int last = min(pos, s.n - 1) - key;
+            if (i < q.ns) last = min(last, w.sinks - 1 - key);
+            if (!valid) last = -1;
+            const int near = pos - w.window + 1 - key, kept = w.sinks - key;
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              if (c0 + e > last || (c0 + e < near && c0 + e >= kept)) ds[e] = 0.f;
+          }
+        }
+        // Operands over this group's own columns: plane pl of both K steps is 16 columns.
+#pragma unroll
+        for (int pl = 0; pl < NP; ++pl) {
+          uint32_t u[16];
+          if constexpr (KEYS) {
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              u[e] = NP == 1 ? pack_bf16(pr[2 * e], pr[2 * e + 1]) : take_upper(pr[2 * e], pr[2 * e + 1]);
+            tc::tmem_store_32x16(buf + operand_col<KEYS>(0, pl, 0) + (pl < 2 ? g * 32 : g * 16), u);
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            u[e] = NP == 1 ? pack_bf16(ds[2 * e], ds[2 * e + 1]) : take_upper(ds[2 * e], ds[2 * e + 1]);
+          tc::tmem_store_32x16(
+              buf + operand_col<KEYS>(KEYS ? 1 : 0, pl, 0) + (pl < 2 || !KEYS ? g * 32 : g * 16), u);
+        }
+        // Moving rows behind the sequence may hold anything, and 0 times NaN is NaN: clear them.
+        if (clear < kMoving && s.n < (KEYS ? s.p0 + w.q_len : w.kv_len)) {
+          if (!KEYS && !(ok = wait_or_abort(m_full + st, m / ST, abort_flag))) break;
+          uint8_t* mt = smem + L::kB + st * 2 * L::kMov;
+          for (int c = max(clear, 0) * 8 + (static_cast<int>(threadIdx.x) - 64); c < kMoving * 8; c += 256)
+            for (int box = 0; box < (KEYS ? 2 : 1) * NP * kBoxes; ++box)
+              *reinterpret_cast<uint4*>(mt + box * kMoving * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+          tc::fence_proxy_async_smem();
+        }
+        if constexpr (NP > 1) {
+          if (i > 0) {
+            if (!(ok = wait_or_abort(sum_full, sums, abort_flag))) break;
+            ++sums;
+            tc::tc_fence_after();
+            add_sums(i == 1);
+          }
+        }
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(pd_full + m % L::kBuffers);
+      }
+      if (!ok) break;
+      mn += n;
+      if (n) {
+        if (!(ok = wait_or_abort(sum_full, sums, abort_flag))) break;
+        ++sums;
+        tc::tc_fence_after();
+        if constexpr (NP > 1) add_sums(n == 1);
+      }
+      // queries: both groups store half of dq; keys: group 0 stores dk, group 1 dv.
+      constexpr int cols = L::kOuts * DH / 2;
+      const uint32_t from = lanes + (NP > 1 ? L::kSum : L::kAcc) + g * cols;
+      const float factor = !KEYS || g == 0 ? w.scale : 1.f;
+#pragma unroll 1
+      for (int c = 0; c < cols; c += 32) {
+        float o[32];
+        uint32_t u[32];
+        if (n) tc::tmem_load_32x32(from + c, u);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) o[e] = n ? __uint_as_float(u[e]) * factor : 0.f;
+        const int col = KEYS ? c : g * cols + c;
+        if (KEYS && k.slot >= 0) {
+          float* dst = p.partial + ((k.slot * 2 + g) * 128 + r) * w.head_dim + col;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            if (col + e < w.head_dim)
+              *reinterpret_cast<float4*>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        } else if (row < (KEYS ? w.kv_len : w.q_len)) {
+          const View& view = KEYS ? (g ? w.dv : w.dk) : w.dq;
+          const int h = KEYS ? k.kh : q.h[0];
+          if constexpr (NP == 1) {
+            __nv_bfloat16* dst = row_out<__nv_bfloat16>(view, b, row, h) + col;
+#pragma unroll
+            for (int e = 0; e < 32; e += 8)
+              if (col + e < w.head_dim)
+                *reinterpret_cast<uint4*>(dst + e) =
+                    make_uint4(pack_bf16(o[e], o[e + 1]), pack_bf16(o[e + 2], o[e + 3]),
+                               pack_bf16(o[e + 4], o[e + 5]), pack_bf16(o[e + 6], o[e + 7]));
+          } else {
+            float* dst = row_out<float>(view, b, row, h) + col;
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              if (col + e < w.head_dim)
+                *reinterpret_cast<float4*>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          }
+        }
+      }
+      if (n) {
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(sum_empty);
+      }
+    }
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  if (warp == 1) tc::tmem_dealloc(tmem, kTmemCols);
+}
+
+// dk, dv of the key tiles that were cut: the sum of their partials in order.
+template <typename T>
+__global__ void __launch_bounds__(256) window_partials_kernel(const __grid_constant__ BackwardParams p) {
+  pdl_begin();
+  const WindowParams& w = p.w;
+  const int bk = w.batch * w.kv_heads, d4 = w.head_dim / 4;
+  const uint64_t i = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  const int e = static_cast<int>(i % d4) * 4;
+  uint64_t rest = i / d4;
+  const int r = static_cast<int>(rest % 128);
+  rest /= 128;
+  const int out = static_cast<int>(rest & 1);
+  rest >>= 1;
+  const int which = static_cast<int>(rest % bk);
+  const int tile = static_cast<int>(rest / bk), row = tile * 128 + r;
+  if (tile >= (p.head_parts > 1 ? p.tiles : p.first_tiles) || row >= w.kv_len) return;
+  const int parts_first = p.chunks * p.head_parts;
+  const bool is_first = tile < p.first_tiles;
+  const int parts = is_first ? parts_first : p.head_parts;
+  const uint64_t slot =
+      is_first ? (static_cast<uint64_t>(tile) * bk + which) * parts_first
+               : static_cast<uint64_t>(p.first_tiles) * bk * parts_first +
+                     (static_cast<uint64_t>(tile - p.first_tiles) * bk + which) * p.head_parts;
+  const float* src = p.partial + ((slot * 2 + out) * 128 + r) * w.head_dim + e;
+  const uint64_t step = 2ull * 128 * w.head_dim;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int k = 0; k < parts; ++k) {
+    const float4 v = *reinterpret_cast<const float4*>(src + k * step);
+    a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+  }
+  const int b = which / w.kv_heads, kh = which - b * w.kv_heads;
+  T* dst = row_out<T>(out ? w.dv : w.dk, b, row, kh) + e;
+  if constexpr (sizeof(T) == 2)
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16(a.x, a.y), pack_bf16(a.z, a.w));
+  else
+    *reinterpret_cast<float4*>(dst) = a;
+}
+
+// D = rowsum(dout o out), `lanes` threads per (token, head) row, eight elements each.
+template <typename T>
+__global__ void __launch_bounds__(256) window_delta_kernel(const __grid_constant__ WindowParams w,
+                                                           int lanes) {
+  pdl_begin();
+  const uint64_t unit = (static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / lanes;
+  const int l = threadIdx.x & (lanes - 1);
+  const bool live = unit < static_cast<uint64_t>(w.batch) * w.q_len * w.heads;
+  const int h = live ? static_cast<int>(unit % w.heads) : 0;
+  const uint64_t bt = live ? unit / w.heads : 0;
+  const int i = static_cast<int>(bt % w.q_len), b = static_cast<int>(bt / w.q_len);
+  float s = 0.f;
+  if (live && l * 8 < w.head_dim) {
+    const T* g = row_ptr<T>(w.dout, b, i, h) + l * 8;
+    const T* o = row_ptr<T>(w.out, b, i, h) + l * 8;
+    constexpr int n = 16 / sizeof(T);
+#pragma unroll
+    for (int v = 0; v < 8; v += n) {
+      alignas(16) T x[n];
+    alignas(16) T y[n];
+      *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(g + v);
+      *reinterpret_cast<uint4*>(y) = *reinterpret_cast<const uint4*>(o + v);
+#pragma unroll
+      for (int e = 0; e < n; ++e) s += as_float(x[e]) * as_float(y[e]);
+    }
+  }
+  for (int o = lanes >> 1; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+  if (live && l == 0) w.delta[(static_cast<uint64_t>(b) * w.heads + h) * w.q_len + i] = s;
+}
+
 // The three bf16 planes of an fp32 view, [plane][batch][head][token][dim], in units of four elements.
 struct SplitParams {
   View src[4];
@@ -684,12 +1275,57 @@ cudaError_t launch_forward(TcParams& p, int device, cudaStream_t stream) {
   return launch(kernel, dim3(grid), dim3(64 + 128 * QT), L::kSmem, stream, p);
 }
 
+struct BackwardPlan {
+  int tiles, first_tiles, chunks, chunk, head_parts;
+  uint64_t slots;  // partials
+};
+// Chunks of the first tokens' tiles cost about what another key tile does (window + 127 rows, at
+// least 512 so that a short window does not make hundreds). Query heads of a group are split
+// over items where there would be fewer than two items per SM.
+BackwardPlan backward_plan(const WindowParams& w, int device) {
+  BackwardPlan b;
+  b.tiles = (w.kv_len + 127) / 128;
+  b.first_tiles = (std::min(w.sinks, w.kv_len) + 127) / 128;
+  const int64_t rows = std::max<int64_t>(512, (static_cast<int64_t>(w.window) + 191) / 64 * 64);
+  b.chunk = static_cast<int>(std::min<int64_t>(rows, std::max(64, w.q_len)));
+  b.chunks = w.q_len > 0 ? (w.q_len + b.chunk - 1) / b.chunk : 1;
+  const int64_t bk = static_cast<int64_t>(w.batch) * w.kv_heads, items = bk * b.tiles;
+  b.head_parts = static_cast<int>(
+      std::min<int64_t>(w.group, std::max<int64_t>(1, 2 * sm_count(device) / std::max<int64_t>(1, items))));
+  b.slots = 0;
+  const uint64_t first_parts = static_cast<uint64_t>(b.chunks) * b.head_parts;
+  if (first_parts > 1) b.slots += bk * b.first_tiles * first_parts;
+  if (b.head_parts > 1) b.slots += bk * (b.tiles - b.first_tiles) * b.head_parts;
+  return b;
+}
+uint64_t partial_bytes(const WindowParams& w, const BackwardPlan& b) {
+  return round256(b.slots * 2 * 128 * w.head_dim * sizeof(float));
+}
+
+template <bool KEYS, int DH, int NP, int ST>
+cudaError_t launch_backward(const BackwardParams& p, int device, cudaStream_t stream) {
+  using L = Bwd<KEYS, DH, NP, ST>;
+  auto kernel = window_backward_kernel<KEYS, DH, NP, ST>;
+  const cudaError_t e = raise_dynamic_smem(reinterpret_cast<const void*>(kernel), device, L::kSmem);
+  if (e != cudaSuccess) return e;
+  const unsigned grid = static_cast<unsigned>(std::min(p.items, sm_count(device)));
+  return launch(kernel, dim3(grid), dim3(320), L::kSmem, stream, p);
+}
+
 }  // namespace
 
 bool tc_supported(const WindowParams& w, bool backward) {
-  if (backward) return false;
   if (w.head_dim % 8 || w.head_dim > 128) return false;
   const int size = w.dtype == SPAR_B200_FLOAT32 ? 4 : 2;
+  if (backward) {
+    // three planes of two stationary operands of 128 columns do not fit in shared memory
+    if (w.head_dim > 64 && w.dtype == SPAR_B200_FLOAT32) return false;
+    if (w.q_len == 0 || !tiled_view(w.dout, size, w.batch, w.q_len, w.heads) ||
+        !tiled_view(w.dq, size, w.batch, w.q_len, w.heads) ||
+        !tiled_view(w.dk, size, w.batch, w.kv_len, w.kv_heads) ||
+        !tiled_view(w.dv, size, w.batch, w.kv_len, w.kv_heads))
+      return false;
+  }
   return w.kv_len > 0 && tiled_view(w.q, size, w.batch, w.q_len, w.heads) &&
          tiled_view(w.k, size, w.batch, w.kv_len, w.kv_heads) &&
          tiled_view(w.v, size, w.batch, w.kv_len, w.kv_heads) &&
@@ -697,9 +1333,9 @@ bool tc_supported(const WindowParams& w, bool backward) {
 }
 
 uint64_t tc_scratch_bytes(const WindowParams& w, bool backward, int device) {
-  (void)device;
-  (void)backward;
-  return planes_bytes(w, w.q_len, w.heads) + 2 * planes_bytes(w, w.kv_len, w.kv_heads);
+  const uint64_t operands = (backward ? 2 : 1) * planes_bytes(w, w.q_len, w.heads) +
+                            2 * planes_bytes(w, w.kv_len, w.kv_heads);
+  return backward ? operands + partial_bytes(w, backward_plan(w, device)) : operands;
 }
 
 cudaError_t tc_forward(const WindowParams& w, void* scratch, int device, cudaStream_t stream) {
@@ -731,6 +1367,65 @@ cudaError_t tc_forward(const WindowParams& w, void* scratch, int device, cudaStr
   }
   return wide ? launch_forward<128, 1, 2, 128, 2, 2>(p, device, stream)
               : launch_forward<64, 1, 2, 128, 3, 3>(p, device, stream);
+}
+
+cudaError_t tc_backward(const WindowParams& w, void* scratch, int device, cudaStream_t stream) {
+  const uint64_t ql = w.q_len, kl = w.kv_len, h = w.heads, kh = w.kv_heads;
+  const BackwardPlan plan = backward_plan(w, device);
+  char* at = static_cast<char*>(scratch);
+  Operand o[4] = {{&w.q, ql, h, nullptr}, {&w.k, kl, kh, nullptr}, {&w.v, kl, kh, nullptr},
+                  {&w.dout, ql, h, nullptr}};
+  for (Operand& x : o) {
+    x.planes = reinterpret_cast<uint16_t*>(at);
+    at += planes_bytes(w, x.tokens, x.heads);
+  }
+  BackwardParams p;
+  memset(&p, 0, sizeof(p));
+  p.w = w;
+  p.partial = reinterpret_cast<float*>(at);
+  p.wait_flag = attention_wait_flag(device);
+  if (!p.wait_flag) return cudaErrorInvalidDevice;
+  p.ksteps = (w.head_dim + 15) / 16;
+  p.scale_log2 = w.scale * kLog2e;
+  p.tiles = plan.tiles;
+  p.first_tiles = plan.first_tiles;
+  p.chunks = plan.chunks;
+  p.chunk = plan.chunk;
+  p.head_parts = plan.head_parts;
+  const bool f32 = w.dtype == SPAR_B200_FLOAT32, wide = w.head_dim > 64;
+  cudaError_t e = cudaSuccess;
+  if (f32 && (e = split(w, o, 4, stream)) != cudaSuccess) return e;
+
+  int lanes = 1;
+  while (lanes * 8 < w.head_dim) lanes *= 2;
+  const uint64_t threads = static_cast<uint64_t>(w.batch) * ql * h * lanes;
+  auto delta = f32 ? window_delta_kernel<float> : window_delta_kernel<__nv_bfloat16>;
+  e = launch(delta, dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, stream, w, lanes);
+  if (e != cudaSuccess) return e;
+
+  if (!operand_map(&p.s1, w, o[0], 128) || !operand_map(&p.s2, w, o[3], 128) ||
+      !operand_map(&p.m1, w, o[1], kMoving) || !operand_map(&p.m2, w, o[2], kMoving))
+    return cudaErrorInvalidValue;
+  p.items = static_cast<int>(w.batch * h * ((ql + 127) / 128));
+  e = f32    ? launch_backward<false, 64, 3, 2>(p, device, stream)
+      : wide ? launch_backward<false, 128, 1, 4>(p, device, stream)
+             : launch_backward<false, 64, 1, 6>(p, device, stream);
+  if (e != cudaSuccess) return e;
+
+  if (!operand_map(&p.s1, w, o[1], 128) || !operand_map(&p.s2, w, o[2], 128) ||
+      !operand_map(&p.m1, w, o[0], kMoving) || !operand_map(&p.m2, w, o[3], kMoving))
+    return cudaErrorInvalidValue;
+  p.items = static_cast<int>(w.batch * kh * p.head_parts *
+                             (p.first_tiles * static_cast<uint64_t>(p.chunks) + p.tiles - p.first_tiles));
+  e = f32    ? launch_backward<true, 64, 3, 2>(p, device, stream)
+      : wide ? launch_backward<true, 128, 1, 4>(p, device, stream)
+             : launch_backward<true, 64, 1, 6>(p, device, stream);
+  if (e != cudaSuccess || !plan.slots) return e;
+
+  const uint64_t cut = p.head_parts > 1 ? p.tiles : p.first_tiles;
+  const uint64_t units = w.batch * kh * cut * 2 * 128 * (w.head_dim / 4);
+  auto sum = f32 ? window_partials_kernel<float> : window_partials_kernel<__nv_bfloat16>;
+  return launch(sum, dim3(static_cast<unsigned>((units + 255) / 256)), dim3(256), 0, stream, p);
 }
 
 }  // namespace window
