@@ -37,6 +37,7 @@ SOURCES = [
     "rotary.cu",
     "window_attention.cu",
     "window_tc.cu",
+    "window_decode.cu",
 ]
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]

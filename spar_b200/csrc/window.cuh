@@ -57,6 +57,22 @@ __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162f
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
+// A view that TMA and 16-byte accesses can address: 16-byte rows, no broadcast dimension.
+inline bool tiled_view(const View& v, int size, uint64_t batch, uint64_t tokens, uint64_t heads) {
+  const uint64_t n = 16 / size;
+  const uint64_t extent[3] = {batch, tokens, heads}, stride[3] = {v.batch, v.token, v.head};
+  if (reinterpret_cast<uintptr_t>(v.data) & 15) return false;
+  for (int i = 0; i < 3; ++i)
+    if (extent[i] > 1 && (stride[i] % n || stride[i] == 0 || stride[i] * size >= (1ull << 40)))
+      return false;
+  return true;
+}
+
+// A few rows against a cache (window_decode.cu).
+bool decode_supported(const WindowParams& w);
+uint64_t decode_scratch_bytes(const WindowParams& w, int device);
+cudaError_t decode_forward(const WindowParams& w, void* scratch, int device, cudaStream_t stream);
+
 // Tensor-core path (window_tc.cu): whether it takes this call, its scratch, and the launches.
 bool tc_supported(const WindowParams& w, bool backward);
 uint64_t tc_scratch_bytes(const WindowParams& w, bool backward, int device);

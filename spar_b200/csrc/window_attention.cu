@@ -288,15 +288,18 @@ namespace {
 // What a call will run, decided from its sizes, types and strides alone, so that the scratch it is
 // asked for and the launch agree.
 struct Plan {
-  bool tiled;
+  bool few, tiled;
   uint64_t delta_bytes, bytes;
 };
 Plan plan_of(const WindowParams& w, bool backward, int device) {
   Plan p;
-  p.tiled = tc_supported(w, backward);
+  p.few = !backward && decode_supported(w);
+  p.tiled = !p.few && tc_supported(w, backward);
   p.delta_bytes =
       backward ? round256(static_cast<uint64_t>(w.batch) * w.heads * w.q_len * sizeof(float)) : 0;
-  p.bytes = p.delta_bytes + (p.tiled ? tc_scratch_bytes(w, backward, device) : 0);
+  p.bytes = p.delta_bytes + (p.few     ? decode_scratch_bytes(w, device)
+                             : p.tiled ? tc_scratch_bytes(w, backward, device)
+                                       : 0);
   return p;
 }
 
@@ -320,7 +323,9 @@ extern "C" SparCudaStatus spar_b200_window_attention_forward(const SparB200Windo
   if (scope.error() != cudaSuccess) return runtime(scope.error());
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (plan.tiled)
+  if (plan.few)
+    e = decode_forward(w, a->scratch, device, s);
+  else if (plan.tiled)
     e = tc_forward(w, a->scratch, device, s);
   else
     e = w.dtype == SPAR_B200_FLOAT32 ? row_path<float>(w, false, s)

@@ -1249,17 +1249,6 @@ cudaError_t split(const WindowParams& w, const Operand* o, int n, cudaStream_t s
                 stream, p);
 }
 
-// A view that TMA and 16-byte accesses can address: 16-byte rows, no broadcast dimension.
-bool tiled_view(const View& v, int size, uint64_t batch, uint64_t tokens, uint64_t heads) {
-  const uint64_t n = 16 / size;
-  const uint64_t extent[3] = {batch, tokens, heads}, stride[3] = {v.batch, v.token, v.head};
-  if (reinterpret_cast<uintptr_t>(v.data) & 15) return false;
-  for (int i = 0; i < 3; ++i)
-    if (extent[i] > 1 && (stride[i] % n || stride[i] == 0 || stride[i] * size >= (1ull << 40)))
-      return false;
-  return true;
-}
-
 template <int DH, int NP, int QT, int BN, int KS, int VS>
 cudaError_t launch_forward(TcParams& p, int device, cudaStream_t stream) {
   using L = Fwd<DH, NP, QT, BN, KS, VS>;

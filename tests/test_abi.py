@@ -167,6 +167,9 @@ def test_rotary_and_window_attention_refuse_bad_calls_without_gpu():
     assert lib.spar_b200_window_attention_forward(window(q_len=0, q=None, out=None), 0, None).code == 0
     assert lib.spar_b200_window_attention_backward(window(batch=0), 0, None).code == 0
     assert lib.spar_b200_window_attention_scratch_bytes(window(), 1, 0) >= 2 * 4 * 3 * 4
+    for none in (dict(batch=0), dict(q_len=0), dict(kv_len=0), dict(q_len=0, kv_len=0)):
+        for backward in (0, 1):  # no division by a count of zero
+            assert lib.spar_b200_window_attention_scratch_bytes(window(**none), backward, 0) < 1 << 20
 
 
 def test_new_structures_mirror_the_header():
