@@ -136,8 +136,10 @@ __device__ __forceinline__ Slot slot_of(const RotaryParams& p, uint32_t s) {
     o.pair_a = HALF || VEC == 1 ? s * VEC : s * (VEC / 2);
     o.pair_b = o.pair_a + p.pairs / 2;
   } else {
-    o.a = 2 * p.pairs + 2 * (s - p.rotating) * VEC;
-    o.b = o.a + VEC;
+    // vectors v and v + (their number of slots) of the part that passes, so that neighbouring
+    // lanes' accesses are neighbours
+    o.a = 2 * p.pairs + (s - p.rotating) * VEC;
+    o.b = o.a + (p.slots - p.rotating) * VEC;
     o.has_b = o.b < p.head_dim;
     o.pair_a = o.pair_b = 0;
   }
@@ -596,7 +598,7 @@ cudaError_t launch_forward(RotaryParams& p, bool vec, int device, cudaStream_t s
   const uint64_t warps =
       (static_cast<uint64_t>(p.tokens) * (p.heads[0] + p.heads[1]) << p.lanes_log2) / 32;
   if (warps >= static_cast<uint64_t>(sm_count(device)) * 64)
-    return launch_rotary<T, VEC, 1, 4, HALF, NORM>(p, stream);
+    return launch_rotary<T, VEC, 1, VEC == 4 ? 4 : 2, HALF, NORM>(p, stream);
   return launch_rotary<T, VEC, 1, 1, HALF, NORM>(p, stream);
 }
 

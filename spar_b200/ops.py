@@ -28,7 +28,14 @@ def _dev(t: torch.Tensor) -> int:
     return t.device.index
 
 
+# The raw handle of a device's current stream; torch.cuda.current_stream builds a Stream object
+# around it (2.3 us against 0.1 us, of about 12 us for a whole call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
 def _stream(t: torch.Tensor) -> int:
+    if _raw_stream is not None:
+        return _raw_stream(t.device.index)
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
@@ -335,27 +342,43 @@ _NO_HEADS = (None, 0, 0, 0)
 def _heads_view(t, name, like=None, shape=None):
     """(pointer, batch, token, head strides) of a [batch, tokens, heads, head_dim] view whose head
     elements are contiguous; `like` gives the type and device it must have."""
-    if t.dim() != 4 or t.dtype not in _ELEMENT:
+    strides = t.stride()
+    if len(strides) != 4 or t.dtype not in _ELEMENT:
         raise ValueError(f"{name} must be a 4-D float32 or bfloat16 tensor [batch, tokens, heads, "
                          "head_dim]")
-    if not t.is_cuda:
+    device = t.get_device()
+    if device < 0:
         raise ValueError("spar_b200 ops take CUDA tensors")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device):
+    if like is not None and (t.dtype is not like.dtype or device != like.get_device()):
         raise ValueError(f"{name} must have the type and device of the other tensors")
     if shape is not None and t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}")
-    batch, token, head, element = t.stride()
+    batch, token, head, element = strides
     if element != 1 and t.shape[3] != 1:
         raise ValueError(f"the elements of a head of {name} must be contiguous")
     return t.data_ptr(), batch, token, head
+
+
+def _out_view(t, name, like):
+    """(tensor, view) of an output of like's shape and type: `t`, checked, or a new one."""
+    if t is not None:
+        return t, _heads_view(t, name, like, like.shape)
+    if like.get_device() < 0:
+        raise ValueError("spar_b200 ops take CUDA tensors")
+    if like.dim() != 4:
+        raise ValueError("queries, keys and values must be [batch, tokens, heads, head_dim]")
+    t = torch.empty_like(like, memory_format=torch.contiguous_format)
+    _, tokens, heads, dim = like.shape
+    return t, (t.data_ptr(), tokens * heads * dim, heads * dim, dim)
 
 
 def _small(t, name, dtype, shape, like):
     """Pointer of an optional contiguous tensor of the given type and shape on like's device."""
     if t is None:
         return None
-    if t.dtype != dtype or tuple(t.shape) != shape or t.device != like.device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {shape} on the "
+    if (t.dtype is not dtype or t.shape != shape or t.get_device() != like.get_device()
+            or not t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on the "
                          "device of the other tensors")
     return t.data_ptr()
 
@@ -397,39 +420,41 @@ def rotary_table(rows: int, rotary_dim: int, theta: float = 10000.0, start: int 
 
 def _rotary_desc(q, k, table, layout, inverse, positions, start, invalid, q_out, k_out, q_weight=None,
                  k_weight=None, eps=0.0, dq=None, dk=None, dq_weight=None, dk_weight=None,
-                 accumulate=False, scratch=None):
+                 accumulate=0, scratch=None):
+    """The descriptor; q_out, k_out, dq and dk are views (of _heads_view) already."""
     qv = _heads_view(q, "q")
     batch, seq, heads, dim = q.shape
     kv_heads, kv = 0, _NO_HEADS
     if k is not None:
         kv = _heads_view(k, "k", q)
-        kv_heads = k.shape[2]
-        if k.shape[0] != batch or k.shape[1] != seq or k.shape[3] != dim:
+        k_batch, k_seq, kv_heads, k_dim = k.shape
+        if k_batch != batch or k_seq != seq or k_dim != dim:
             raise ValueError("k must have the batch, tokens and head_dim of q")
-    if layout not in _ROTARY_LAYOUT:
+    tag = _ROTARY_LAYOUT.get(layout)
+    if tag is None:
         raise ValueError(f"layout must be one of {list(_ROTARY_LAYOUT)}")
-    if table.dim() != 3 or start < 0:
+    shape = table.shape
+    if len(shape) != 3 or shape[2] != 2 or start < 0:
         raise ValueError("table must be [rows, rotary_dim / 2, 2] and start not negative")
-    rows, pairs, _ = table.shape
-    k_views = [_NO_HEADS if k is None else _heads_view(t, name, q, k.shape) if t is not None else _NO_HEADS
-               for t, name in ((k_out, "k_out"), (dk, "dk"))]
+    head = (dim,)
     return SparB200Rotary(
-        _ELEMENT[q.dtype], _ROTARY_LAYOUT[layout], int(inverse), batch, seq, heads, kv_heads, dim,
-        2 * pairs, _small(table, "table", torch.float32, (rows, pairs, 2), q), rows,
+        _ELEMENT[q.dtype], tag, inverse, batch, seq, heads, kv_heads, dim, 2 * shape[1],
+        _small(table, "table", torch.float32, shape, q), shape[0],
         _small(positions, "positions", torch.int32, (batch, seq), q), start,
-        _small(invalid, "invalid", torch.int32, (1,), q), *qv, *kv,
-        *_heads_view(q_out, "q_out", q, q.shape), *k_views[0],
-        _small(q_weight, "q_weight", torch.float32, (dim,), q),
-        _small(k_weight, "k_weight", torch.float32, (dim,), q), eps,
-        *(_NO_HEADS if dq is None else _heads_view(dq, "dq", q, q.shape)), *k_views[1],
-        _small(dq_weight, "dq_weight", torch.float32, (dim,), q),
-        _small(dk_weight, "dk_weight", torch.float32, (dim,), q), int(accumulate), _ptr(scratch))
+        _small(invalid, "invalid", torch.int32, (1,), q), *qv, *kv, *q_out, *k_out,
+        _small(q_weight, "q_weight", torch.float32, head, q),
+        _small(k_weight, "k_weight", torch.float32, head, q), eps,
+        *(dq or _NO_HEADS), *(dk or _NO_HEADS),
+        _small(dq_weight, "dq_weight", torch.float32, head, q),
+        _small(dk_weight, "dk_weight", torch.float32, head, q), accumulate, scratch)
 
 
-def _like(t, out):
-    if out is not None or t is None:
-        return out
-    return torch.empty(t.shape, device=t.device, dtype=t.dtype)
+def _rotary_outputs(q, k, q_out, k_out, names=("q_out", "k_out")):
+    if k is None and k_out is not None:
+        raise ValueError(f"{names[1]} is given without k")
+    q_out, q_view = _out_view(q_out, names[0], q)
+    k_out, k_view = (None, _NO_HEADS) if k is None else _out_view(k_out, names[1], k)
+    return q_out, k_out, q_view, k_view
 
 
 def rotary(q, k, table, *, layout: str = "interleaved", positions=None, start: int = 0,
@@ -438,8 +463,8 @@ def rotary(q, k, table, *, layout: str = "interleaved", positions=None, start: i
     rotary_dim elements of every head rotated by the table row of their token: positions
     [batch, tokens] int32, or start + t. inverse turns back (the backward pass). q_out=q rotates in
     place. `invalid` (int32 [1]) is set to 1 by a position outside the table (outputs zeros)."""
-    q_out, k_out = _like(q, q_out), _like(k, k_out)
-    desc = _rotary_desc(q, k, table, layout, inverse, positions, start, invalid, q_out, k_out)
+    q_out, k_out, q_view, k_view = _rotary_outputs(q, k, q_out, k_out)
+    desc = _rotary_desc(q, k, table, layout, int(inverse), positions, start, invalid, q_view, k_view)
     call("spar_b200_rotary", ctypes.byref(desc), _dev(q), _stream(q))
     return q_out, k_out
 
@@ -449,8 +474,8 @@ def qk_norm_rotary_forward(q, k, q_weight, k_weight, table, eps: float = 1e-6, *
                            k_out=None, invalid=None):
     """RMSNorm of every query and key head (weights [head_dim], float32) and the rotation of
     `rotary`, in one pass."""
-    q_out, k_out = _like(q, q_out), _like(k, k_out)
-    desc = _rotary_desc(q, k, table, layout, False, positions, start, invalid, q_out, k_out, q_weight,
+    q_out, k_out, q_view, k_view = _rotary_outputs(q, k, q_out, k_out)
+    desc = _rotary_desc(q, k, table, layout, 0, positions, start, invalid, q_view, k_view, q_weight,
                         k_weight, eps)
     call("spar_b200_qk_norm_rotary_forward", ctypes.byref(desc), _dev(q), _stream(q))
     return q_out, k_out
@@ -462,7 +487,9 @@ def qk_norm_rotary_backward(dq_out, dk_out, q, k, q_weight, k_weight, table, eps
                             invalid=None):
     """(dq, dk, dq_weight, dk_weight) of qk_norm_rotary_forward from the gradients of its outputs and
     its inputs; dq=dq_out writes in place. accumulate_params adds to the weight gradients given."""
-    dq, dk = _like(q, dq), _like(k, dk)
+    dq, dk, q_view, k_view = _rotary_outputs(q, k, dq, dk, ("dq", "dk"))
+    if (k is None) != (dk_out is None):
+        raise ValueError("dk_out and k are given together")
     if accumulate_params and (dq_weight is None or (k is not None and dk_weight is None)):
         raise ValueError("accumulate_params adds to weight gradients that must be given")
     dim = q.shape[-1]
@@ -472,43 +499,45 @@ def qk_norm_rotary_backward(dq_out, dk_out, q, k, q_weight, k_weight, table, eps
         dk_weight = torch.empty(dim, device=q.device, dtype=torch.float32)
     nbytes = _lib.load().spar_b200_qk_norm_rotary_scratch_bytes(dim, _dev(q))
     scratch = torch.empty(max(nbytes, 16), device=q.device, dtype=torch.uint8)
-    desc = _rotary_desc(q, k, table, layout, False, positions, start, invalid, dq, dk, q_weight,
-                        k_weight, eps, dq_out, dk_out, dq_weight, dk_weight, accumulate_params, scratch)
+    desc = _rotary_desc(q, k, table, layout, 0, positions, start, invalid, q_view, k_view, q_weight,
+                        k_weight, eps, _heads_view(dq_out, "dq_out", q, q.shape),
+                        None if k is None else _heads_view(dk_out, "dk_out", q, k.shape), dq_weight,
+                        dk_weight, int(accumulate_params), scratch.data_ptr())
     call("spar_b200_qk_norm_rotary_backward", ctypes.byref(desc), _dev(q), _stream(q))
     return dq, dk, dq_weight, dk_weight
 
 
 # ------------------------------------------------------------------------------- window attention
-def _window_desc(q, k, v, out, lse, window, sinks, scale, lengths, first, dout=None, dq=None, dk=None,
-                 dv=None):
+def _window_desc(q, k, v, out, lse, window, sinks, scale, lengths, first, back=_NO_HEADS * 4):
+    """The descriptor; out and back (dout, dq, dk, dv) are views (of _heads_view) already."""
     qv = _heads_view(q, "q")
+    kv = _heads_view(k, "k", q)
     batch, q_len, heads, dim = q.shape
-    if k.dim() != 4:
-        raise ValueError("k must be a 4-D float32 or bfloat16 tensor [batch, tokens, heads, head_dim]")
-    kv_len, kv_heads = k.shape[1], k.shape[2]
-    if k.shape[0] != batch or k.shape[3] != dim or kv_heads < 1 or heads % kv_heads:
+    k_batch, kv_len, kv_heads, k_dim = k.shape
+    if k_batch != batch or k_dim != dim or kv_heads < 1 or heads % kv_heads:
         raise ValueError("k must have the batch and head_dim of q and a number of heads that divides q's")
     if window < 1 or sinks < 0:
         raise ValueError("window must be at least 1 and sinks not negative")
-    if scale is not None and not scale > 0.0:
+    if scale is None:
+        scale = 0.0
+    elif not scale > 0.0:
         raise ValueError("scale must be positive")
-    back = _NO_HEADS * 4
-    if dout is not None:
-        back = (*_heads_view(dout, "dout", q, q.shape), *_heads_view(dq, "dq", q, q.shape),
-                *_heads_view(dk, "dk", q, k.shape), *_heads_view(dv, "dv", q, k.shape))
+    each = (batch,)
     return SparB200WindowAttention(
-        _ELEMENT[q.dtype], batch, q_len, kv_len, heads, kv_heads, dim, window, sinks, scale or 0.0,
-        _small(lengths, "lengths", torch.int32, (batch,), q),
-        _small(first, "first", torch.int32, (batch,), q), *qv, *_heads_view(k, "k", q),
-        *_heads_view(v, "v", q, k.shape), *_heads_view(out, "out", q, q.shape),
+        _ELEMENT[q.dtype], batch, q_len, kv_len, heads, kv_heads, dim, window, sinks, scale,
+        _small(lengths, "lengths", torch.int32, each, q), _small(first, "first", torch.int32, each, q),
+        *qv, *kv, *_heads_view(v, "v", q, k.shape), *out,
         _small(lse, "lse", torch.float32, (batch, heads, q_len), q), *back, None)
 
 
 def _window_call(name, desc, backward, q):
-    nbytes = _lib.load().spar_b200_window_attention_scratch_bytes(ctypes.byref(desc), backward, _dev(q))
-    scratch = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes else None
-    desc.scratch = _ptr(scratch)
-    call(name, ctypes.byref(desc), _dev(q), _stream(q))
+    device = q.get_device()
+    ref = ctypes.byref(desc)
+    nbytes = _lib.load().spar_b200_window_attention_scratch_bytes(ref, backward, device)
+    if nbytes:
+        scratch = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
+        desc.scratch = scratch.data_ptr()
+    call(name, ref, device, _stream(q))
 
 
 def window_attention_forward(q, k, v, window: int, sinks: int = 0, *, scale: float | None = None,
@@ -521,9 +550,9 @@ def window_attention_forward(q, k, v, window: int, sinks: int = 0, *, scale: flo
     j <= p, j < lengths[b] (None: kv_len), and j > p - window or j < sinks; a row with p < 0 or
     p >= lengths[b] sees nothing (out 0, lse -inf). scale None: 1 / sqrt(head_dim).
     Returns (out like q, lse [batch, heads, q_len])."""
-    out = _like(q, out)
-    lse = torch.empty(q.shape[0], q.shape[2], q.shape[1], device=q.device, dtype=torch.float32)
-    desc = _window_desc(q, k, v, out, lse, window, sinks, scale, lengths, first)
+    out, view = _out_view(out, "out", q)
+    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), device=q.device, dtype=torch.float32)
+    desc = _window_desc(q, k, v, view, lse, window, sinks, scale, lengths, first)
     _window_call("spar_b200_window_attention_forward", desc, 0, q)
     return out, lse
 
@@ -533,8 +562,11 @@ def window_attention_backward(dout, q, k, v, out, lse, window: int, sinks: int =
                               dv=None):
     """(dq, dk, dv) of window_attention_forward; dk and dv are summed over each key head's group.
     dq, dk, dv may be given as views of a packed gradient buffer."""
-    dq, dk, dv = _like(q, dq), _like(k, dk), _like(v, dv)
-    desc = _window_desc(q, k, v, out, lse, window, sinks, scale, lengths, first, dout, dq, dk, dv)
+    dq, dq_view = _out_view(dq, "dq", q)
+    dk, dk_view = _out_view(dk, "dk", k)
+    dv, dv_view = _out_view(dv, "dv", v)
+    desc = _window_desc(q, k, v, _heads_view(out, "out", q, q.shape), lse, window, sinks, scale, lengths,
+                        first, (*_heads_view(dout, "dout", q, q.shape), *dq_view, *dk_view, *dv_view))
     _window_call("spar_b200_window_attention_backward", desc, 1, q)
     return dq, dk, dv
 
