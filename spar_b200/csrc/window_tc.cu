@@ -11,8 +11,8 @@
 //
 // One CTA per SM works through its items (two query tiles of 128 rows that share their key tiles:
 // two heads of one key head where the group is even, else neighbouring tiles of one head).
-// Warp 0 feeds key and value tiles by TMA, one thread of warp 1 issues every product, warps 2-5
-// and 6-9 are the softmax of the two tiles (thread = row): while one tile's scores are
+// Warp 0 feeds key and value tiles by TMA, one thread of warp 1 issues every product, warps 4-7
+// and 8-11 are the softmax of the two tiles (thread = row): while one tile's scores are
 // exponentiated the other tile's products run. The keys of an item are its first tokens' tiles,
 // then tiles that start exactly at the first key of the window, so a window of W keys under a tile
 // of 128 rows costs ceil((W + 127) / BN) tiles. Every wait is bounded and leaves an error flag.
@@ -37,6 +37,7 @@ constexpr uint32_t kMaxSmem = 232448;
 constexpr uint32_t kTmemCols = 512;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kPolyShare = 2;        // of every 8 weights of an unmasked bf16 tile (see ex2_poly)
 constexpr float kRescaleLog2 = 8.f;  // the running maximum moves only past this margin (P <= 2^8)
 
 // Why a CTA gives up: the CTA's flag, and the one that spar_b200_attention_error reads.
@@ -64,11 +65,23 @@ __device__ __forceinline__ float ex2(float x) {
 // Operand tiles in shared memory: per plane, DH / 64 boxes of `rows` rows x 64 elements (128 bytes,
 // 128-byte swizzle). The same image is a K-major operand (rows = M or N, elements = K) and an
 // MN-major one (elements = N, rows = K).
-__device__ __forceinline__ uint64_t kmajor(uint32_t base, uint32_t rows, int ks) {
-  return tc::smem_desc(base + (ks >> 2) * rows * 128 + (ks & 3) * 32, 16, 1024, tc::kLayoutSw128);
+// Descriptors differ in their low words only (address and leading offset, in 16 bytes), so that a
+// product's steps cost one addition each.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (tc::kLayoutSw128 << 29);
+__device__ __forceinline__ uint64_t desc(uint32_t low) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(low), "r"(kDescHigh));
+  return d;
 }
-__device__ __forceinline__ uint64_t mnmajor(uint32_t base, uint32_t rows, int ks) {
-  return tc::smem_desc(base + ks * 2048, rows * 128, 1024, tc::kLayoutSw128);
+__device__ __forceinline__ uint32_t kmajor_low(uint32_t addr) { return (addr >> 4) | (1u << 16); }
+__host__ __device__ constexpr uint32_t kmajor_step(uint32_t rows, int plane, int boxes, int ks) {
+  return (plane * boxes + (ks >> 2)) * rows * 8 + (ks & 3) * 2;
+}
+__device__ __forceinline__ uint32_t mnmajor_low(uint32_t addr, uint32_t rows) {
+  return (addr >> 4) | ((rows * 8) << 16);
+}
+__host__ __device__ constexpr uint32_t mnmajor_step(uint32_t rows, int plane, int boxes, int ks) {
+  return plane * boxes * rows * 8 + ks * 128;
 }
 
 // Pairs of planes of a product, smallest first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0).
@@ -90,6 +103,89 @@ __device__ __forceinline__ uint32_t take_upper(float& lo, float& hi) {
   lo -= __uint_as_float(a & 0xffff0000u);
   hi -= __uint_as_float(b & 0xffff0000u);
   return __byte_perm(a, b, 0x7632);
+}
+
+// Registers a thread of this warpgroup may use from here on (all its warps take part; the shares
+// of all groups add up to the launch's).
+template <int N>
+__device__ __forceinline__ void registers_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void registers_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+// Bits 0 .. n - 1 (none below 0, all from 32 on).
+__device__ __forceinline__ uint32_t below(int n) {
+  return n >= 32 ? 0xffffffffu : (1u << max(n, 0)) - 1u;
+}
+// Scores whose bit is not set become -infinity.
+__device__ __forceinline__ void hide32(uint32_t (&v)[32], uint32_t seen) {
+#pragma unroll
+  for (int e = 0; e < 32; ++e) v[e] = seen & (1u << e) ? v[e] : 0xff800000u;
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t both(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 halves(uint64_t v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x of two values on the FMA pipe (Cody and Waite): x = n + f with n the nearest integer, the
+// polynomial 2^f ~ c0 + .. + c4 f^4 on [-1/2, 1/2] (minimax in relative error, 2.6e-6, fitted for
+// this file), n added to the exponent. x is cut at -126. The special-function unit makes 16 values
+// per cycle and SM, less than the score tiles need; a share of them goes this way.
+__device__ __forceinline__ uint64_t ex2_poly(uint64_t x) {
+  float2 v = halves(x);
+  x = both(fmaxf(v.x, -126.f), fmaxf(v.y, -126.f));
+  constexpr float kRound = 12582912.f;  // 1.5 * 2^23: adding it leaves the integer in the low bits
+  const uint64_t n = add2(x, both(kRound, kRound));
+  const uint64_t f = add2(x, fma2(n, both(-1.f, -1.f), both(kRound, kRound)));
+  uint64_t y = fma2(f, both(0.009570102f, 0.009570102f), both(0.05591786f, 0.05591786f));
+  y = fma2(f, y, both(0.24024744f, 0.24024744f));
+  y = fma2(f, y, both(0.6931218f, 0.6931218f));
+  y = fma2(f, y, both(0.9999993f, 0.9999993f));
+  const float2 e = halves(n), r = halves(y);
+  return both(__uint_as_float(__float_as_uint(r.x) + (__float_as_uint(e.x) << 23)),
+              __uint_as_float(__float_as_uint(r.y) + (__float_as_uint(e.y) << 23)));
+}
+
+// P = 2^(s scale - m) of 32 scores as 16 columns of bf16 pairs, rounded to nearest, and the sums of
+// the unrounded values; the last kPoly of every 8 on the FMA pipe.
+template <int kPoly>
+__device__ __forceinline__ void weights32(const uint32_t (&s)[32], uint64_t scale, uint64_t minus_m,
+                                          uint64_t (&sums)[2], uint32_t (&u)[16]) {
+#pragma unroll
+  for (int e = 0; e < 32; e += 2) {
+    const uint64_t x = fma2(both(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), scale, minus_m);
+    uint64_t w;
+    if (e % 8 >= 8 - kPoly) {
+      w = ex2_poly(x);
+    } else {
+      const float2 t = halves(x);
+      w = both(ex2(t.x), ex2(t.y));
+    }
+    sums[e / 2 % 2] = add2(sums[e / 2 % 2], w);
+    const float2 t = halves(w);
+    u[e / 2] = pack_bf16(t.x, t.y);
+  }
 }
 
 // 64 consecutive values of a row as bf16 operand columns: one plane rounded to nearest (NP = 1:
@@ -224,7 +320,7 @@ struct Fwd {
 };
 
 template <int DH, int NP, int QT, int BN, int KS, int VS>
-__global__ void __launch_bounds__(64 + 128 * QT, 1) window_forward_kernel(
+__global__ void __launch_bounds__(128 + 128 * QT, 1) window_forward_kernel(
     const __grid_constant__ TcParams p) {
   using L = Fwd<DH, NP, QT, BN, KS, VS>;
   constexpr int kBoxes = DH / 64;
@@ -237,7 +333,8 @@ __global__ void __launch_bounds__(64 + 128 * QT, 1) window_forward_kernel(
   uint64_t* p_full = bars + 6;     // [2]
   uint64_t* o_full = bars + 8;     // [2]
   uint64_t* o_empty = bars + 10;   // [2]
-  uint64_t* k_full = bars + 12;    // [KS]
+  uint64_t* p_rest = bars + 12;    // [2] NP = 1: the second half of P
+  uint64_t* k_full = bars + 14;    // [KS]
   uint64_t* k_empty = k_full + KS;
   uint64_t* v_full = k_empty + KS;  // [VS]
   uint64_t* v_empty = v_full + VS;
@@ -253,6 +350,7 @@ __global__ void __launch_bounds__(64 + 128 * QT, 1) window_forward_kernel(
       tc::mbar_init(q_empty + x, 1);
       tc::mbar_init(s_full + x, 1);
       tc::mbar_init(p_full + x, 4);
+      tc::mbar_init(p_rest + x, 4);
       tc::mbar_init(o_full + x, 1);
       tc::mbar_init(o_empty + x, 4);
     }
@@ -278,147 +376,159 @@ __global__ void __launch_bounds__(64 + 128 * QT, 1) window_forward_kernel(
   const uint32_t tmem = *tmem_slot;
   pdl_begin();
 
-  if (warp == 0) {
-    // -------------------------------------------------------------- TMA producer
-    if (tc::elect_one()) {
-      tc::tma_prefetch(&p.q);
-      tc::tma_prefetch(&p.k);
-      tc::tma_prefetch(&p.v);
-      uint32_t kn = 0, vn = 0, qn[2] = {0, 0};
-      bool ok = true;
-      for (int idx = blockIdx.x; idx < p.items && ok && !*abort_flag.cta; idx += gridDim.x) {
-        const Item it = item_of<QT, BN>(p, idx);
+  // Four warps that feed and four per query tile: the launch's registers (168 a thread of three
+  // groups) are dealt out anew, 88 to the feeding group and 208 to each softmax group, whose
+  // threads hold a whole row of 128 scores.
+  if (warp < 4) {
+    if constexpr (QT == 2) registers_down<88>();
+    if (warp == 0) {
+      // -------------------------------------------------------------- TMA producer
+      if (tc::elect_one()) {
+        tc::tma_prefetch(&p.q);
+        tc::tma_prefetch(&p.k);
+        tc::tma_prefetch(&p.v);
+        uint32_t kn = 0, vn = 0, qn[2] = {0, 0};
+        bool ok = true;
+        for (int idx = blockIdx.x; idx < p.items && ok && !*abort_flag.cta; idx += gridDim.x) {
+          const Item it = item_of<QT, BN>(p, idx);
 #pragma unroll
-        for (int x = 0; x < QT; ++x) {
-          if (!it.any[x] || !ok) continue;
-          if (!(ok = wait_or_abort(q_empty + x, qn[x] + 1, abort_flag))) break;
-          tc::mbar_arrive_expect_tx(q_full + x, L::kQTile);
-          ++qn[x];
-          for (int pl = 0; pl < NP; ++pl)
-            for (int c = 0; c < kBoxes; ++c)
-              tc::tma_load_5d(smem + L::kQ + x * L::kQTile + (pl * kBoxes + c) * 16384, &p.q,
-                              q_full + x, 64 * c, it.row[x], it.h[x], it.b, pl);
+          for (int x = 0; x < QT; ++x) {
+            if (!it.any[x] || !ok) continue;
+            if (!(ok = wait_or_abort(q_empty + x, qn[x] + 1, abort_flag))) break;
+            tc::mbar_arrive_expect_tx(q_full + x, L::kQTile);
+            ++qn[x];
+            for (int pl = 0; pl < NP; ++pl)
+              for (int c = 0; c < kBoxes; ++c)
+                tc::tma_load_5d(smem + L::kQ + x * L::kQTile + (pl * kBoxes + c) * 16384, &p.q,
+                                q_full + x, 64 * c, it.row[x], it.h[x], it.b, pl);
+          }
+          for (int j = 0; j < it.n && ok; ++j) {
+            const int key = key_of<BN>(it, j);
+            const uint32_t ks = kn % KS, vs = vn % VS;
+            if (!(ok = wait_or_abort(k_empty + ks, kn / KS + 1, abort_flag))) break;
+            tc::mbar_arrive_expect_tx(k_full + ks, L::kKTile);
+            for (int pl = 0; pl < NP; ++pl)
+              for (int c = 0; c < kBoxes; ++c)
+                tc::tma_load_5d(smem + L::kK + ks * L::kKTile + (pl * kBoxes + c) * BN * 128, &p.k,
+                                k_full + ks, 64 * c, key, it.kh, it.b, pl);
+            ++kn;
+            if (!(ok = wait_or_abort(v_empty + vs, vn / VS + 1, abort_flag))) break;
+            tc::mbar_arrive_expect_tx(v_full + vs, L::kKTile);
+            for (int pl = 0; pl < NP; ++pl)
+              for (int c = 0; c < kBoxes; ++c)
+                tc::tma_load_5d(smem + L::kV + vs * L::kKTile + (pl * kBoxes + c) * BN * 128, &p.v,
+                                v_full + vs, 64 * c, key, it.kh, it.b, pl);
+            ++vn;
+          }
         }
-        for (int j = 0; j < it.n && ok; ++j) {
-          const int key = key_of<BN>(it, j);
-          const uint32_t ks = kn % KS, vs = vn % VS;
-          if (!(ok = wait_or_abort(k_empty + ks, kn / KS + 1, abort_flag))) break;
-          tc::mbar_arrive_expect_tx(k_full + ks, L::kKTile);
-          for (int pl = 0; pl < NP; ++pl)
-            for (int c = 0; c < kBoxes; ++c)
-              tc::tma_load_5d(smem + L::kK + ks * L::kKTile + (pl * kBoxes + c) * BN * 128, &p.k,
-                              k_full + ks, 64 * c, key, it.kh, it.b, pl);
-          ++kn;
-          if (!(ok = wait_or_abort(v_empty + vs, vn / VS + 1, abort_flag))) break;
-          tc::mbar_arrive_expect_tx(v_full + vs, L::kKTile);
-          for (int pl = 0; pl < NP; ++pl)
-            for (int c = 0; c < kBoxes; ++c)
-              tc::tma_load_5d(smem + L::kV + vs * L::kKTile + (pl * kBoxes + c) * BN * 128, &p.v,
-                              v_full + vs, 64 * c, key, it.kh, it.b, pl);
-          ++vn;
-        }
-      }
-      // Every load issued must have landed before the CTA exits: the last one of each barrier.
-      for (int x = 0; x < QT; ++x)
-        if (qn[x]) wait_or_abort(q_full + x, qn[x] - 1, abort_flag);
-      for (uint32_t i = kn > KS ? kn - KS : 0; i < kn; ++i)
-        wait_or_abort(k_full + i % KS, i / KS, abort_flag);
-      for (uint32_t i = vn > VS ? vn - VS : 0; i < vn; ++i)
-        wait_or_abort(v_full + i % VS, i / VS, abort_flag);
-    }
-    __syncwarp();
-  } else if (warp == 1) {
-    // -------------------------------------------------------------- product issuer
-    if (tc::elect_one()) {
-      const uint32_t idesc_s = tc::idesc_bf16(128, BN, 0, 0);
-      const uint32_t idesc_o = tc::idesc_bf16(128, 16 * p.ksteps, 0, 1);
-      const uint32_t q_addr = tc::smem_u32(smem + L::kQ), k_addr = tc::smem_u32(smem + L::kK),
-                     v_addr = tc::smem_u32(smem + L::kV);
-      uint32_t base = 0, qn[2] = {0, 0}, pn[2] = {0, 0}, on[2] = {0, 0};
-      bool ok = true;
-      for (int idx = blockIdx.x; idx < p.items && ok && !*abort_flag.cta; idx += gridDim.x) {
-        const Item it = item_of<QT, BN>(p, idx);
-        int issued[2] = {it.n, it.n};  // the last tile whose scores were issued; n: none ever
-#pragma unroll
+        // Every load issued must have landed before the CTA exits: the last one of each barrier.
         for (int x = 0; x < QT; ++x)
-          if (it.any[x]) issued[x] = -1;
-        // Scores of tile j; K_j is free once every query tile that uses it has issued its own.
-        auto scores = [&](int x, int j) -> bool {
-          const uint32_t st = (base + j) % KS;
-          if (!wait_or_abort(k_full + st, (base + j) / KS, abort_flag)) return false;
-          tc::tc_fence_after();
-          const uint32_t qa = q_addr + x * L::kQTile, ka = k_addr + st * L::kKTile;
-          uint32_t acc = 0;
+          if (qn[x]) wait_or_abort(q_full + x, qn[x] - 1, abort_flag);
+        for (uint32_t i = kn > KS ? kn - KS : 0; i < kn; ++i)
+          wait_or_abort(k_full + i % KS, i / KS, abort_flag);
+        for (uint32_t i = vn > VS ? vn - VS : 0; i < vn; ++i)
+          wait_or_abort(v_full + i % VS, i / VS, abort_flag);
+      }
+      __syncwarp();
+    } else if (warp == 1) {
+      // -------------------------------------------------------------- product issuer
+      if (tc::elect_one()) {
+        const uint32_t idesc_s = tc::idesc_bf16(128, BN, 0, 0);
+        const uint32_t idesc_o = tc::idesc_bf16(128, 16 * p.ksteps, 0, 1);
+        const uint32_t q_addr = tc::smem_u32(smem + L::kQ), k_addr = tc::smem_u32(smem + L::kK),
+                       v_addr = tc::smem_u32(smem + L::kV);
+        uint32_t base = 0, qn[2] = {0, 0}, pn[2] = {0, 0}, on[2] = {0, 0};
+        bool ok = true;
+        for (int idx = blockIdx.x; idx < p.items && ok && !*abort_flag.cta; idx += gridDim.x) {
+          const Item it = item_of<QT, BN>(p, idx);
+          int issued[2] = {it.n, it.n};  // the last tile whose scores were issued; n: none ever
 #pragma unroll
-          for (int pr = 0; pr < kProducts<NP>; ++pr)
+          for (int x = 0; x < QT; ++x)
+            if (it.any[x]) issued[x] = -1;
+          // Scores of tile j; K_j is free once every query tile that uses it has issued its own.
+          auto scores = [&](int x, int j) -> bool {
+            const uint32_t st = (base + j) % KS;
+            if (!wait_or_abort(k_full + st, (base + j) / KS, abort_flag)) return false;
+            tc::tc_fence_after();
+            const uint32_t qa = kmajor_low(q_addr + x * L::kQTile), ka = kmajor_low(k_addr + st * L::kKTile);
+            uint32_t acc = 0;
 #pragma unroll
-            for (int ks = 0; ks < DH / 16; ++ks)
-              if (ks < p.ksteps) {
-                tc::mma_f16(tmem + x * L::kCols,
-                            kmajor(qa + plane_a<NP>(pr) * kBoxes * 16384, 128, ks),
-                            kmajor(ka + plane_b<NP>(pr) * kBoxes * BN * 128, BN, ks), idesc_s, acc);
-                acc = 1;
-              }
-          tc::mma_commit(s_full + x);
-          issued[x] = j;
-          const int y = x ^ 1;
-          if (QT == 1 || !it.any[y] || next_tile(it, y, j) != j || issued[y] >= j)
-            tc::mma_commit(k_empty + st);
-          if (next_tile(it, x, j + 1) == it.n) tc::mma_commit(q_empty + x);
-          return true;
-        };
+            for (int pr = 0; pr < kProducts<NP>; ++pr)
 #pragma unroll
-        for (int x = 0; x < QT; ++x) {
-          if (!ok || !it.any[x]) continue;
-          if (!(ok = wait_or_abort(q_full + x, qn[x], abort_flag))) break;
-          ++qn[x];
-          if (next_tile(it, x, 0) == 0) ok = scores(x, 0);
-        }
-        for (int j = 0; j < it.n && ok; ++j) {
-          const uint32_t st = (base + j) % VS;
+              for (int ks = 0; ks < DH / 16; ++ks)
+                if (ks < p.ksteps) {
+                  tc::mma_f16(tmem + x * L::kCols, desc(qa + kmajor_step(128, plane_a<NP>(pr), kBoxes, ks)),
+                              desc(ka + kmajor_step(BN, plane_b<NP>(pr), kBoxes, ks)), idesc_s, acc);
+                  acc = 1;
+                }
+            tc::mma_commit(s_full + x);
+            issued[x] = j;
+            const int y = x ^ 1;
+            if (QT == 1 || !it.any[y] || next_tile(it, y, j) != j || issued[y] >= j)
+              tc::mma_commit(k_empty + st);
+            if (next_tile(it, x, j + 1) == it.n) tc::mma_commit(q_empty + x);
+            return true;
+          };
 #pragma unroll
           for (int x = 0; x < QT; ++x) {
             if (!ok || !it.any[x]) continue;
-            if (next_tile(it, x, j) == j) {
-              if (!(ok = wait_or_abort(p_full + x, pn[x], abort_flag))) break;
-              ++pn[x];
-              const bool first = next_tile(it, x, 0) == j;
-              if (first && !(ok = wait_or_abort(o_empty + x, on[x] + 1, abort_flag))) break;
-              if (!(ok = wait_or_abort(v_full + st, (base + j) / VS, abort_flag))) break;
-              tc::tc_fence_after();
-              uint32_t acc = NP == 1 && !first;
-              const uint32_t va = v_addr + st * L::kKTile;
-#pragma unroll
-              for (int pr = 0; pr < kProducts<NP>; ++pr)
-#pragma unroll
-                for (int ks = 0; ks < BN / 16; ++ks) {
-                  tc::mma_f16_ts(tmem + x * L::kCols + L::kS,
-                                 tmem + x * L::kCols + plane_a<NP>(pr) * (BN / 2) + ks * 8,
-                                 mnmajor(va + plane_b<NP>(pr) * kBoxes * BN * 128, BN, ks), idesc_o,
-                                 acc);
-                  acc = 1;
-                }
-              if (next_tile(it, x, j + 1) == it.n) {
-                tc::mma_commit(o_full + x);
-                ++on[x];
-              }
-            }
-            // The next scores overwrite P, which the product above reads: one thread's products run
-            // in the order of their issue. Never more than one tile ahead of the products over
-            // keys, so that a query tile that skips tiles cannot wait for a stage still in use.
-            if (j + 1 < it.n && next_tile(it, x, j + 1) == j + 1) ok = scores(x, j + 1);
+            if (!(ok = wait_or_abort(q_full + x, qn[x], abort_flag))) break;
+            ++qn[x];
+            if (next_tile(it, x, 0) == 0) ok = scores(x, 0);
           }
-          if (ok) tc::mma_commit(v_empty + st);
+          for (int j = 0; j < it.n && ok; ++j) {
+            const uint32_t st = (base + j) % VS;
+#pragma unroll
+            for (int x = 0; x < QT; ++x) {
+              if (!ok || !it.any[x]) continue;
+              if (next_tile(it, x, j) == j) {
+                if (!(ok = wait_or_abort(p_full + x, pn[x], abort_flag))) break;
+                const bool first = next_tile(it, x, 0) == j;
+                if (first && !(ok = wait_or_abort(o_empty + x, on[x] + 1, abort_flag))) break;
+                if (!(ok = wait_or_abort(v_full + st, (base + j) / VS, abort_flag))) break;
+                tc::tc_fence_after();
+                uint32_t acc = NP == 1 && !first;
+                const uint32_t va = mnmajor_low(v_addr + st * L::kKTile, BN);
+#pragma unroll
+                for (int pr = 0; pr < kProducts<NP>; ++pr)
+#pragma unroll
+                  for (int ks = 0; ks < BN / 16; ++ks) {
+                    // The product over the first half of the keys runs while the second half's
+                    // weights are made.
+                    if (NP == 1 && ks == BN / 32) {
+                      if (!(ok = wait_or_abort(p_rest + x, pn[x], abort_flag))) break;
+                      tc::tc_fence_after();
+                    }
+                    tc::mma_f16_ts(tmem + x * L::kCols + L::kS,
+                                   tmem + x * L::kCols + plane_a<NP>(pr) * (BN / 2) + ks * 8,
+                                   desc(va + mnmajor_step(BN, plane_b<NP>(pr), kBoxes, ks)), idesc_o, acc);
+                    acc = 1;
+                  }
+                if (!ok) break;
+                ++pn[x];
+                if (next_tile(it, x, j + 1) == it.n) {
+                  tc::mma_commit(o_full + x);
+                  ++on[x];
+                }
+              }
+              // The next scores overwrite P, which the product above reads: one thread's products run
+              // in the order of their issue. Never more than one tile ahead of the products over
+              // keys, so that a query tile that skips tiles cannot wait for a stage still in use.
+              if (j + 1 < it.n && next_tile(it, x, j + 1) == j + 1) ok = scores(x, j + 1);
+            }
+            if (ok) tc::mma_commit(v_empty + st);
+          }
+          base += it.n;
         }
-        base += it.n;
+        tc::mma_commit(drain);
+        wait_or_abort(drain, 0, abort_flag);
       }
-      tc::mma_commit(drain);
-      wait_or_abort(drain, 0, abort_flag);
+      __syncwarp();
     }
-    __syncwarp();
   } else {
     // -------------------------------------------------------------- softmax
-    const int x = (warp - 2) >> 2;
+    if constexpr (QT == 2) registers_up<208>();
+    const int x = (warp >> 2) - 1;
     const uint32_t quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lanes = tmem + ((quarter * 32) << 16) + x * L::kCols;
@@ -454,9 +564,10 @@ __global__ void __launch_bounds__(64 + 128 * QT, 1) window_forward_kernel(
             }
           }
           uint32_t v[BN / 32][32];
-#pragma unroll
-          for (int c = 0; c < BN / 64; ++c)
-            tc::tmem_load_2x32(lanes + c * 64, lanes + c * 64 + 32, v[2 * c], v[2 * c + 1]);
+          if constexpr (BN == 128)
+            tc::tmem_load_4x32(lanes, v[0], v[1], v[2], v[3]);
+          else
+            tc::tmem_load_2x32(lanes, lanes + 32, v[0], v[1]);
           // Keys of this tile that this row sees: c <= last and (c >= near or c < kept).
           const bool all_seen = key + BN - 1 <= first_pos && first_pos + 31 < it.s.n && first_pos >= 0 &&
                                 (j < it.ns ? key + BN <= w.sinks
@@ -467,14 +578,16 @@ __global__ void __launch_bounds__(64 + 128 * QT, 1) window_forward_kernel(
             if (!valid) last = -1;
             const int near = pos - w.window + 1 - key, kept = w.sinks - key;
 #pragma unroll
-            for (int c = 0; c < BN; ++c)
-              if (c > last || (c < near && c >= kept)) v[c / 32][c % 32] = 0xff800000u;
+            for (int c = 0; c < BN / 32; ++c)
+              hide32(v[c], below(last + 1 - c * 32) & (~below(near - c * 32) | below(kept - c * 32)));
           }
           float mxs[8];
 #pragma unroll
           for (int i = 0; i < 8; ++i) mxs[i] = -INFINITY;
 #pragma unroll
-          for (int c = 0; c < BN; ++c) mxs[c & 7] = fmaxf(mxs[c & 7], __uint_as_float(v[c / 32][c % 32]));
+          for (int c = 0; c < BN; c += 2)
+            mxs[c / 2 & 7] = fmaxf(fmaxf(mxs[c / 2 & 7], __uint_as_float(v[c / 32][c % 32])),
+                                   __uint_as_float(v[c / 32][c % 32 + 1]));
           const float mx = fmaxf(fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])),
                                  fmaxf(fmaxf(mxs[4], mxs[5]), fmaxf(mxs[6], mxs[7]))) * p.scale_log2;
           const bool move = m == -INFINITY ? mx > m : mx > m + kRescaleLog2;
@@ -500,19 +613,6 @@ __global__ void __launch_bounds__(64 + 128 * QT, 1) window_forward_kernel(
             pending = f;
           }
           const float base_m = m == -INFINITY ? 0.f : m;
-          float sums[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int half = 0; half < BN / 64; ++half) {
-            float pr[64];
-#pragma unroll
-            for (int c = 0; c < 64; ++c) {
-              const int at = half * 64 + c;
-              pr[c] = ex2(fmaf(__uint_as_float(v[at / 32][at % 32]), p.scale_log2, -base_m));
-              sums[c & 3] += pr[c];
-            }
-            store_planes<NP, 64>(lanes + half * 32, BN / 2, pr);
-          }
-          sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
           // Value rows behind the sequence may hold anything, and 0 times NaN is NaN: clear them.
           if (key + BN > it.s.n && it.s.n < w.kv_len) {
             const uint32_t st = (base + j) % VS;
@@ -523,9 +623,40 @@ __global__ void __launch_bounds__(64 + 128 * QT, 1) window_forward_kernel(
                 *reinterpret_cast<uint4*>(vt + box * BN * 128 + i * 16) = make_uint4(0, 0, 0, 0);
             tc::fence_proxy_async_smem();
           }
-          tc::tc_fence_before();
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(p_full + x);
+          if constexpr (NP == 1) {
+            const uint64_t scale = both(p.scale_log2, p.scale_log2), minus_m = both(-base_m, -base_m);
+            uint64_t sums[2] = {both(0.f, 0.f), both(0.f, 0.f)};
+#pragma unroll
+            for (int c = 0; c < BN / 32; ++c) {
+              uint32_t u[16];
+              if (all_seen)
+                weights32<kPolyShare>(v[c], scale, minus_m, sums, u);
+              else
+                weights32<0>(v[c], scale, minus_m, sums, u);
+              tc::tmem_store_32x16_async(lanes + c * 16, u);
+              if (c == BN / 64 - 1 || c == BN / 32 - 1) {
+                tc::tmem_store_wait();
+                tc::tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive((c == BN / 32 - 1 ? p_rest : p_full) + x);
+              }
+            }
+            const float2 t = halves(add2(sums[0], sums[1]));
+            sum += t.x + t.y;
+          } else {
+            float sums[4] = {0.f, 0.f, 0.f, 0.f};
+            float pr[64];
+#pragma unroll
+            for (int c = 0; c < 64; ++c) {
+              pr[c] = ex2(fmaf(__uint_as_float(v[c / 32][c % 32]), p.scale_log2, -base_m));
+              sums[c & 3] += pr[c];
+            }
+            store_planes<NP, 64>(lanes, BN / 2, pr);
+            sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(p_full + x);
+          }
         }
         if (!ok) break;
         if (!(ok = wait_or_abort(o_full + x, on, abort_flag))) break;
@@ -838,16 +969,16 @@ __global__ void __launch_bounds__(320, 1) window_backward_kernel(
         tc::tc_fence_after();
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-          const uint32_t a = a_addr + half * L::kStat, b = b_addr + (2 * st + half) * L::kMov;
+          const uint32_t a = kmajor_low(a_addr + half * L::kStat),
+                         b = kmajor_low(b_addr + (2 * st + half) * L::kMov);
           uint32_t acc = 0;
 #pragma unroll
           for (int pr = 0; pr < kProducts<NP>; ++pr)
 #pragma unroll
             for (int ks = 0; ks < DH / 16; ++ks)
               if (ks < p.ksteps) {
-                tc::mma_f16(buf + half * 64, kmajor(a + plane_a<NP>(pr) * kBoxes * 16384, 128, ks),
-                            kmajor(b + plane_b<NP>(pr) * kBoxes * kMoving * 128, kMoving, ks), idesc_s,
-                            acc);
+                tc::mma_f16(buf + half * 64, desc(a + kmajor_step(128, plane_a<NP>(pr), kBoxes, ks)),
+                            desc(b + kmajor_step(kMoving, plane_b<NP>(pr), kBoxes, ks)), idesc_s, acc);
                 acc = 1;
               }
         }
@@ -875,15 +1006,14 @@ __global__ void __launch_bounds__(320, 1) window_backward_kernel(
           for (int out = 0; out < static_cast<int>(L::kOuts); ++out) {
             // queries: dq += dS k; keys: dk += dS^T q, dv += P^T dout
             const int which = KEYS ? 1 - out : 0;
-            const uint32_t b = b_addr + (2 * st + out) * L::kMov;
+            const uint32_t b = mnmajor_low(b_addr + (2 * st + out) * L::kMov, kMoving);
             uint32_t acc = NP == 1 && i > 0;
 #pragma unroll
             for (int pr = 0; pr < kProducts<NP>; ++pr)
 #pragma unroll
               for (int ks = 0; ks < kMoving / 16; ++ks) {
                 tc::mma_f16_ts(tmem + L::kAcc + out * DH, buf + operand_col<KEYS>(which, plane_a<NP>(pr), ks),
-                               mnmajor(b + plane_b<NP>(pr) * kBoxes * kMoving * 128, kMoving, ks), idesc_o,
-                               acc);
+                               desc(b + mnmajor_step(kMoving, plane_b<NP>(pr), kBoxes, ks)), idesc_o, acc);
                 acc = 1;
               }
           }
@@ -1261,7 +1391,7 @@ cudaError_t launch_forward(TcParams& p, int device, cudaStream_t stream) {
   const int64_t per = p.pair_heads ? w.heads / 2 : w.heads;
   p.items = static_cast<int>(w.batch * per * (p.pair_heads ? p.tiles : (p.tiles + QT - 1) / QT));
   const unsigned grid = static_cast<unsigned>(std::min(p.items, sm_count(device)));
-  return launch(kernel, dim3(grid), dim3(64 + 128 * QT), L::kSmem, stream, p);
+  return launch(kernel, dim3(grid), dim3(128 + 128 * QT), L::kSmem, stream, p);
 }
 
 struct BackwardPlan {
