@@ -203,9 +203,46 @@ __device__ __forceinline__ void store_planes(uint32_t taddr, uint32_t plane_cols
   }
 }
 
+// 32 rows of results (lane = row) on their way to memory: 16-byte chunks into a box of 32 rows x 128
+// bytes (128-byte swizzle, so that neighbouring lanes hit other banks), stored by TMA, which leaves
+// out rows and elements outside the tensor. Stores straight from the registers, 16 bytes in each of
+// 32 rows, took 4800 cycles per 128 x 128 tile.
+struct Box {
+  uint8_t* at;  // 4 KB of this warp, 1024-byte aligned
+  // Columns col .. col + 31 of the row; NP = 1 packs them to bf16, and two calls fill a box.
+  template <int NP>
+  __device__ __forceinline__ void put(const CUtensorMap* map, const float (&o)[32], int col, int row,
+                                      int head, int batch) const {
+    const int lane = threadIdx.x & 31;
+    const int chunk = NP == 1 ? (col & 32) / 8 : 0;
+    if (chunk == 0) {
+      if (lane == 0) tc::bulk_wait_read<0>();
+      __syncwarp();
+    }
+#pragma unroll
+    for (int i = 0; i < (NP == 1 ? 4 : 8); ++i) {
+      uint4 u;
+      if constexpr (NP == 1)
+        u = make_uint4(pack_bf16(o[8 * i], o[8 * i + 1]), pack_bf16(o[8 * i + 2], o[8 * i + 3]),
+                       pack_bf16(o[8 * i + 4], o[8 * i + 5]), pack_bf16(o[8 * i + 6], o[8 * i + 7]));
+      else
+        u = make_uint4(__float_as_uint(o[4 * i]), __float_as_uint(o[4 * i + 1]),
+                       __float_as_uint(o[4 * i + 2]), __float_as_uint(o[4 * i + 3]));
+      *reinterpret_cast<uint4*>(at + lane * 128 + (((chunk + i) ^ (lane & 7)) << 4)) = u;
+    }
+    if (NP == 1 && chunk == 0) return;
+    tc::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tc::tma_store_5d(map, at, NP == 1 ? col - 32 : col, row, head, batch, 0);
+      tc::bulk_commit();
+    }
+  }
+};
+
 struct TcParams {
   WindowParams w;
-  CUtensorMap q, k, v;
+  CUtensorMap q, k, v, out;
   int* wait_flag;
   int tiles;        // query tiles of 128 rows
   int pair_heads;   // 1: items are (query tile, two heads); 0: (two query tiles, head)
@@ -309,7 +346,8 @@ struct Fwd {
   static constexpr uint32_t kQ = 0;
   static constexpr uint32_t kK = kQ + QT * kQTile;
   static constexpr uint32_t kV = kK + KS * kKTile;
-  static constexpr uint32_t kBar = kV + VS * kKTile;
+  static constexpr uint32_t kOut = kV + VS * kKTile;  // 4 KB per softmax warp
+  static constexpr uint32_t kBar = kOut + QT * 16384;
   static constexpr uint32_t kSmem = kBar + 256 + 1024;
   static_assert(kSmem <= kMaxSmem, "forward shared memory");
   // TMEM columns of one query tile: scores, which P overwrites, then O of the current key tile
@@ -532,6 +570,7 @@ __global__ void __launch_bounds__(128 + 128 * QT, 1) window_forward_kernel(
     const uint32_t quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lanes = tmem + ((quarter * 32) << 16) + x * L::kCols;
+    const Box box = {smem + L::kOut + (warp - 4) * 4096};
     uint32_t base = 0, sn = 0, on = 0;
     bool ok = true;
     for (int idx = blockIdx.x; idx < p.items && ok; idx += gridDim.x) {
@@ -687,23 +726,8 @@ __global__ void __launch_bounds__(128 + 128 * QT, 1) window_forward_kernel(
             for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(u[e]) * inv;
           }
         }
-        if (stored) {
-          if constexpr (NP == 1) {
-            __nv_bfloat16* dst = row_out<__nv_bfloat16>(w.out, it.b, row + r, it.h[x]) + c * 32;
-#pragma unroll
-            for (int e = 0; e < 32; e += 8)
-              if (c * 32 + e < w.head_dim)
-                *reinterpret_cast<uint4*>(dst + e) =
-                    make_uint4(pack_bf16(o[e], o[e + 1]), pack_bf16(o[e + 2], o[e + 3]),
-                               pack_bf16(o[e + 4], o[e + 5]), pack_bf16(o[e + 6], o[e + 7]));
-          } else {
-            float* dst = row_out<float>(w.out, it.b, row + r, it.h[x]) + c * 32;
-#pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              if (c * 32 + e < w.head_dim)
-                *reinterpret_cast<float4*>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          }
-        }
+        if (row + quarter * 32 < w.q_len)
+          box.put<NP>(&p.out, o, c * 32, row + quarter * 32, it.h[x], it.b);
       }
       if (it.any[x]) {
         tc::tc_fence_before();
@@ -714,6 +738,8 @@ __global__ void __launch_bounds__(128 + 128 * QT, 1) window_forward_kernel(
         w.lse[(static_cast<uint64_t>(it.b) * w.heads + it.h[x]) * w.q_len + row + r] =
             valid ? m * kLn2 + logf(sum) : -INFINITY;
     }
+    if (lane == 0) tc::bulk_wait_all();
+    __syncwarp();
   }
   tc::tc_fence_before();
   __syncthreads();
@@ -740,6 +766,7 @@ constexpr int kMoving = 64;
 struct BackwardParams {
   WindowParams w;
   CUtensorMap s1, s2, m1, m2;  // stationary and moving operands: q, dout / k, v or k, v / q, dout
+  CUtensorMap out1, out2;      // dq, or dk and dv
   int* wait_flag;
   int items, tiles, ksteps;
   float scale_log2;
@@ -802,7 +829,8 @@ struct Bwd {
   static constexpr uint32_t kMov = NP * DH * kMoving * 2;     // one moving operand
   static constexpr uint32_t kA = 0;
   static constexpr uint32_t kB = kA + 2 * kStat;
-  static constexpr uint32_t kRows = kB + ST * 2 * kMov;       // [ST][64] (lse log2 e, D)
+  static constexpr uint32_t kOut = kB + ST * 2 * kMov;        // 4 KB per softmax warp
+  static constexpr uint32_t kRows = kOut + 8 * 4096;          // [ST][64] (lse log2 e, D)
   static constexpr uint32_t kBar = kRows + (KEYS ? ST * kMoving * 8 : 0);
   static constexpr uint32_t kSmem = kBar + 256 + 1024;
   static_assert(kSmem <= kMaxSmem, "backward shared memory");
@@ -1034,6 +1062,7 @@ __global__ void __launch_bounds__(320, 1) window_backward_kernel(
     const uint32_t quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lanes = tmem + ((quarter * 32) << 16);
+    const Box box = {smem + L::kOut + (warp - 2) * 4096};
     uint32_t mn = 0, sums = 0;
     bool ok = true;
     // NP = 3: adds the last tile's products to the sums of the earlier ones; the groups share the
@@ -1174,11 +1203,13 @@ __global__ void __launch_bounds__(320, 1) window_backward_kernel(
         if constexpr (NP > 1) add_sums(n == 1);
       }
       // queries: both groups store half of dq; keys: group 0 stores dk, group 1 dv.
-      constexpr int cols = L::kOuts * DH / 2;
+      // (bf16 heads of 64: group 0 stores dq, whose 64 columns are one box)
+      constexpr int cols = NP == 1 && L::kOuts * DH == 64 ? 64 : L::kOuts * DH / 2;
       const uint32_t from = lanes + (NP > 1 ? L::kSum : L::kAcc) + g * cols;
       const float factor = !KEYS || g == 0 ? w.scale : 1.f;
+      const int warp_row = row - lane;
 #pragma unroll 1
-      for (int c = 0; c < cols; c += 32) {
+      for (int c = 0; c < cols && g * cols < static_cast<int>(L::kOuts) * DH; c += 32) {
         float o[32];
         uint32_t u[32];
         if (n) tc::tmem_load_32x32(from + c, u);
@@ -1191,24 +1222,8 @@ __global__ void __launch_bounds__(320, 1) window_backward_kernel(
           for (int e = 0; e < 32; e += 4)
             if (col + e < w.head_dim)
               *reinterpret_cast<float4*>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-        } else if (row < (KEYS ? w.kv_len : w.q_len)) {
-          const View& view = KEYS ? (g ? w.dv : w.dk) : w.dq;
-          const int h = KEYS ? k.kh : q.h[0];
-          if constexpr (NP == 1) {
-            __nv_bfloat16* dst = row_out<__nv_bfloat16>(view, b, row, h) + col;
-#pragma unroll
-            for (int e = 0; e < 32; e += 8)
-              if (col + e < w.head_dim)
-                *reinterpret_cast<uint4*>(dst + e) =
-                    make_uint4(pack_bf16(o[e], o[e + 1]), pack_bf16(o[e + 2], o[e + 3]),
-                               pack_bf16(o[e + 4], o[e + 5]), pack_bf16(o[e + 6], o[e + 7]));
-          } else {
-            float* dst = row_out<float>(view, b, row, h) + col;
-#pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              if (col + e < w.head_dim)
-                *reinterpret_cast<float4*>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-          }
+        } else if (warp_row < (KEYS ? w.kv_len : w.q_len)) {
+          box.put<NP>(KEYS && g ? &p.out2 : &p.out1, o, col, warp_row, KEYS ? k.kh : q.h[0], b);
         }
       }
       if (n) {
@@ -1217,6 +1232,8 @@ __global__ void __launch_bounds__(320, 1) window_backward_kernel(
         if (lane == 0) tc::mbar_arrive(sum_empty);
       }
     }
+    if (lane == 0) tc::bulk_wait_all();
+    __syncwarp();
   }
   tc::tc_fence_before();
   __syncthreads();
@@ -1323,16 +1340,16 @@ __global__ void __launch_bounds__(256) split_planes_kernel(const __grid_constant
 }
 
 // ------------------------------------------------------------------------------- host side
-// bf16 view as a 5-D map (element, token, head, batch, plane), boxes of 64 elements x `rows`.
+// bf16 (or fp32) view as a 5-D map (element, token, head, batch, plane), boxes of 128 bytes x `rows`.
 bool make_view_map(CUtensorMap* map, const void* base, const uint64_t (&dims)[5],
-                   const uint64_t (&strides)[4], uint32_t rows) {
+                   const uint64_t (&strides)[4], uint32_t rows, bool f32 = false) {
   auto fn = encode_fn();
   if (!fn) return false;
   cuuint64_t d[5], s[4];
   for (int i = 0; i < 5; ++i) d[i] = dims[i];
-  for (int i = 0; i < 4; ++i) s[i] = dims[i + 1] > 1 ? strides[i] * 2 : 16;
-  cuuint32_t box[5] = {64, rows, 1, 1, 1}, unit[5] = {1, 1, 1, 1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), d, s, box, unit,
+  for (int i = 0; i < 4; ++i) s[i] = dims[i + 1] > 1 ? strides[i] * (f32 ? 4 : 2) : 16;
+  cuuint32_t box[5] = {f32 ? 32u : 64u, rows, 1, 1, 1}, unit[5] = {1, 1, 1, 1, 1};
+  return fn(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), d, s, box, unit,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -1352,6 +1369,12 @@ bool operand_map(CUtensorMap* map, const WindowParams& w, const Operand& o, uint
                          {o.view->token, o.view->head, o.view->batch, 8}, rows);
   return make_view_map(map, o.planes, {d, o.tokens, o.heads, b, 3},
                        {d, d * o.tokens, d * o.tokens * o.heads, d * o.tokens * o.heads * b}, rows);
+}
+// Results in place, in boxes of 32 rows.
+bool result_map(CUtensorMap* map, const WindowParams& w, const View& v, uint64_t tokens, uint64_t heads) {
+  return make_view_map(map, v.data,
+                       {static_cast<uint64_t>(w.head_dim), tokens, heads, static_cast<uint64_t>(w.batch), 1},
+                       {v.token, v.head, v.batch, 8}, 32, w.dtype == SPAR_B200_FLOAT32);
 }
 uint64_t planes_bytes(const WindowParams& w, uint64_t tokens, uint64_t heads) {
   return w.dtype == SPAR_B200_BFLOAT16
@@ -1476,7 +1499,7 @@ cudaError_t tc_forward(const WindowParams& w, void* scratch, int device, cudaStr
   const bool wide = w.head_dim > 64, f32 = w.dtype == SPAR_B200_FLOAT32;
   const uint32_t rows = f32 ? 64 : 128;
   if (!operand_map(&p.q, w, o[0], 128) || !operand_map(&p.k, w, o[1], rows) ||
-      !operand_map(&p.v, w, o[2], rows))
+      !operand_map(&p.v, w, o[2], rows) || !result_map(&p.out, w, w.out, w.q_len, w.heads))
     return cudaErrorInvalidValue;
   if (f32) {
     const cudaError_t e = split(w, o, 3, stream);
@@ -1523,7 +1546,8 @@ cudaError_t tc_backward(const WindowParams& w, void* scratch, int device, cudaSt
   if (e != cudaSuccess) return e;
 
   if (!operand_map(&p.s1, w, o[0], 128) || !operand_map(&p.s2, w, o[3], 128) ||
-      !operand_map(&p.m1, w, o[1], kMoving) || !operand_map(&p.m2, w, o[2], kMoving))
+      !operand_map(&p.m1, w, o[1], kMoving) || !operand_map(&p.m2, w, o[2], kMoving) ||
+      !result_map(&p.out1, w, w.dq, ql, h))
     return cudaErrorInvalidValue;
   p.items = static_cast<int>(w.batch * h * ((ql + 127) / 128));
   e = f32    ? launch_backward<false, 64, 3, 2>(p, device, stream)
@@ -1532,12 +1556,13 @@ cudaError_t tc_backward(const WindowParams& w, void* scratch, int device, cudaSt
   if (e != cudaSuccess) return e;
 
   if (!operand_map(&p.s1, w, o[1], 128) || !operand_map(&p.s2, w, o[2], 128) ||
-      !operand_map(&p.m1, w, o[0], kMoving) || !operand_map(&p.m2, w, o[3], kMoving))
+      !operand_map(&p.m1, w, o[0], kMoving) || !operand_map(&p.m2, w, o[3], kMoving) ||
+      !result_map(&p.out1, w, w.dk, kl, kh) || !result_map(&p.out2, w, w.dv, kl, kh))
     return cudaErrorInvalidValue;
   p.items = static_cast<int>(w.batch * kh * p.head_parts *
                              (p.first_tiles * static_cast<uint64_t>(p.chunks) + p.tiles - p.first_tiles));
   e = f32    ? launch_backward<true, 64, 3, 2>(p, device, stream)
-      : wide ? launch_backward<true, 128, 1, 4>(p, device, stream)
+      : wide ? launch_backward<true, 128, 1, 3>(p, device, stream)
              : launch_backward<true, 64, 1, 6>(p, device, stream);
   if (e != cudaSuccess || !plan.slots) return e;
 
