@@ -105,6 +105,12 @@ __device__ __forceinline__ uint32_t take_upper(float& lo, float& hi) {
   return __byte_perm(a, b, 0x7632);
 }
 
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // Registers a thread of this warpgroup may use from here on (all its warps take part; the shares
 // of all groups add up to the launch's).
 template <int N>
@@ -755,9 +761,8 @@ __global__ void __launch_bounds__(128 + 128 * QT, 1) window_forward_kernel(
 //       every query head of the group: S^T = k q^T, dP^T = v dout^T;  dv += P^T dout;  dk += dS^T q
 // P = exp(S - lse) is recomputed on both sides, so every gradient element is summed in one CTA and
 // no order is left to chance. P and dS replace S and dP in TMEM and are read there as the A operand.
-// All eight softmax warps work on every tile (thread = stationary row, half of the 64 columns);
-// with two buffers the next tile's S and dP run meanwhile. `scale` is applied to dq and dk at the
-// end.
+// With two buffers of S and dP the next tile's products run meanwhile. `scale` is applied to dq and dk
+// at the end.
 // First tokens are seen by every later row: their key tiles' rows are cut into chunks of
 // `chunk` rows that are items of their own (and, where there are few key tiles, so are groups of
 // query heads); such items leave fp32 partial sums that a last launch adds in order.
@@ -830,7 +835,7 @@ struct Bwd {
   static constexpr uint32_t kA = 0;
   static constexpr uint32_t kB = kA + 2 * kStat;
   static constexpr uint32_t kOut = kB + ST * 2 * kMov;        // 4 KB per softmax warp
-  static constexpr uint32_t kRows = kOut + 8 * 4096;          // [ST][64] (lse log2 e, D)
+  static constexpr uint32_t kRows = kOut + 8 * 4096;          // [ST][2][64] -lse log2 e, -D
   static constexpr uint32_t kBar = kRows + (KEYS ? ST * kMoving * 8 : 0);
   static constexpr uint32_t kSmem = kBar + 256 + 1024;
   static_assert(kSmem <= kMaxSmem, "backward shared memory");
@@ -881,7 +886,7 @@ __global__ void __launch_bounds__(320, 1) window_backward_kernel(
     tc::mbar_init(a_empty, 1);
     for (int i = 0; i < 2; ++i) {
       tc::mbar_init(s_full + i, 1);
-      tc::mbar_init(pd_full + i, 8);
+      tc::mbar_init(pd_full + i, NP == 1 ? 4 : 8);
     }
     tc::mbar_init(sum_full, 1);
     tc::mbar_init(sum_empty, 8);
@@ -965,13 +970,13 @@ __global__ void __launch_bounds__(320, 1) window_backward_kernel(
             }
         }
         if constexpr (KEYS) {
-          float2* stats = reinterpret_cast<float2*>(smem + L::kRows) + st * kMoving;
+          float* stats = reinterpret_cast<float*>(smem + L::kRows) + st * 2 * kMoving;
           const uint64_t at = (static_cast<uint64_t>(b) * w.heads + h) * w.q_len;
 #pragma unroll
           for (int e = lane; e < kMoving; e += 32) {
             const bool in = row + e < k.end;
-            stats[e] = make_float2(in ? __ldg(w.lse + at + row + e) * kLog2e : 0.f,
-                                   in ? __ldg(w.delta + at + row + e) : 0.f);
+            stats[e] = in ? -__ldg(w.lse + at + row + e) * kLog2e : 0.f;
+            stats[kMoving + e] = in ? -__ldg(w.delta + at + row + e) : 0.f;
           }
           __syncwarp();
           if (lane == 0) tc::mbar_arrive(m_full + st);
@@ -1058,11 +1063,17 @@ __global__ void __launch_bounds__(320, 1) window_backward_kernel(
     __syncwarp();
   } else {
     // -------------------------------------------------------------- softmax and results
+    // bf16: the two groups take the tiles in turn, all 64 columns each (in two halves, as registers
+    // allow): while one waits the other works. Half of every tile each took 1460 cycles a tile of
+    // 64, most of it in waits and in the latency of two warps a scheduler that did the same.
+    // fp32, whose keys have one buffer: half of every tile each.
+    constexpr bool kTurns = NP == 1;
     const int g = (warp - 2) >> 2;
     const uint32_t quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lanes = tmem + ((quarter * 32) << 16);
     const Box box = {smem + L::kOut + (warp - 2) * 4096};
+    const uint64_t scale = both(p.scale_log2, p.scale_log2);
     uint32_t mn = 0, sums = 0;
     bool ok = true;
     // NP = 3: adds the last tile's products to the sums of the earlier ones; the groups share the
@@ -1090,96 +1101,118 @@ __global__ void __launch_bounds__(320, 1) window_backward_kernel(
       // queries: this row's position and statistics; keys: this row's key
       const int row = (KEYS ? k.key : q.row[0]) + r;
       const int pos = KEYS ? row : s.p0 + row;
+      const int first_pos = pos - lane;  // of this warp
       const bool valid = KEYS ? row < s.n : row < w.q_len && pos >= 0 && pos < s.n;
-      float lse2 = 0.f, delta = 0.f;
+      const bool rows_in = KEYS ? first_pos + 31 < s.n
+                                : first_pos >= 0 && first_pos + 31 < s.n && row - lane + 31 < w.q_len;
+      uint64_t minus_lse = 0, minus_delta = 0;
       if (!KEYS && valid && n) {
         const uint64_t at = (static_cast<uint64_t>(b) * w.heads + q.h[0]) * w.q_len + row;
-        lse2 = __ldg(w.lse + at) * kLog2e;
-        delta = __ldg(w.delta + at);
+        const float lse2 = __ldg(w.lse + at) * kLog2e, delta = __ldg(w.delta + at);
+        minus_lse = both(-lse2, -lse2);
+        minus_delta = both(-delta, -delta);
       }
       for (int i = 0; i < n && ok; ++i) {
         const uint32_t m = mn + i, st = m % ST;
+        if (kTurns && (m & 1) != static_cast<uint32_t>(g)) continue;
         const uint32_t buf = lanes + (m % L::kBuffers) * L::kBuf;
-        if (!(ok = wait_or_abort(s_full + m % L::kBuffers, m / L::kBuffers, abort_flag))) break;
-        tc::tc_fence_after();
-        uint32_t sv[32], dv[32];
-        tc::tmem_load_2x32(buf + g * 32, buf + 64 + g * 32, sv, dv);
-        const int c0 = g * 32;
-        float pr[32], ds[32];
-        int clear;  // moving rows from here on may hold anything
+        // Columns lo .. hi of the tile are seen, but for the query side's columns before `near`
+        // that are not below `kept`. `clear`: moving rows from here on may hold anything.
+        int lo = 0, hi, near = 0, kept = 0, clear, key = 0, base = 0, upto = 0;
         if constexpr (KEYS) {
           const int head = i / k.jobs_per_head;
           const int at = k.row + (i - head * k.jobs_per_head) * kMoving;  // first moving row
-          const int base = s.p0 + at;                                     // its position
+          base = s.p0 + at;                                               // its position
+          upto = k.end - at;
           clear = min(s.n - base, kMoving);
-          // This key is seen from columns lo .. hi; a warp's keys all by all of this group's
-          // columns?
-          const int lo = pos - base;
-          int hi = min(k.end - 1 - at, pos < w.sinks ? kMoving : pos - base + w.window - 1);
-          if (!valid) hi = -1;
-          const int k0 = k.key + static_cast<int>(quarter) * 32;
-          const bool all_seen = k0 + 31 <= base + c0 && at + c0 + 32 <= k.end && k0 + 31 < s.n &&
-                                (base + c0 + 31 < k0 + w.window || k0 + 32 <= w.sinks);
-          if (!(ok = wait_or_abort(m_full + st, m / ST, abort_flag))) break;
-          const float2* stats = reinterpret_cast<const float2*>(smem + L::kRows) + st * kMoving + c0;
-#pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            const float2 t = stats[e];
-            pr[e] = ex2(fmaf(__uint_as_float(sv[e]), p.scale_log2, -t.x));
-            ds[e] = pr[e] * (__uint_as_float(dv[e]) - t.y);
-          }
-          if (!all_seen) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (c0 + e < lo || c0 + e > hi) pr[e] = ds[e] = 0.f;
-          }
+          lo = pos - base;
+          hi = min(upto - 1, pos < w.sinks ? kMoving : pos - base + w.window - 1);
         } else {
-          const int key = key_of<kMoving>(q, i);
+          key = key_of<kMoving>(q, i);
           clear = min(s.n - key, kMoving);
-          const int first_pos = s.p0 + q.row[0] + static_cast<int>(quarter) * 32;
-          const bool all_seen =
-              key + c0 + 31 <= first_pos && first_pos >= 0 && first_pos + 31 < s.n &&
-              first_pos + 31 < s.p0 + w.q_len &&
-              (i < q.ns ? key + c0 + 32 <= w.sinks
-                        : key + c0 > first_pos + 31 - w.window || key + c0 + 32 <= w.sinks);
+          hi = min(pos, s.n - 1) - key;
+          if (i < q.ns) hi = min(hi, w.sinks - 1 - key);
+          near = pos - w.window + 1 - key;
+          kept = w.sinks - key;
+        }
+        if (!valid) hi = -1;
+        if (!(ok = wait_or_abort(s_full + m % L::kBuffers, m / L::kBuffers, abort_flag))) break;
+        tc::tc_fence_after();
+        if (KEYS && !(ok = wait_or_abort(m_full + st, m / ST, abort_flag))) break;
+        const float* stats = reinterpret_cast<const float*>(smem + L::kRows) + st * 2 * kMoving;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) {
-            pr[e] = ex2(fmaf(__uint_as_float(sv[e]), p.scale_log2, -lse2));
-            ds[e] = pr[e] * (__uint_as_float(dv[e]) - delta);
+        for (int half = kTurns ? 0 : g; half < (kTurns ? 2 : g + 1); ++half) {
+          const int c0 = half * 32;
+          uint32_t sv[32], dv[32];
+          tc::tmem_load_2x32(buf + c0, buf + 64 + c0, sv, dv);
+          bool all_seen = rows_in;
+          if constexpr (KEYS)
+            all_seen = all_seen && first_pos + 31 <= base + c0 && c0 + 32 <= upto &&
+                       (base + c0 + 31 < first_pos + w.window || first_pos + 32 <= w.sinks);
+          else
+            all_seen = all_seen && key + c0 + 31 <= first_pos &&
+                       (i < q.ns ? key + c0 + 32 <= w.sinks
+                                 : key + c0 > first_pos + 31 - w.window || key + c0 + 32 <= w.sinks);
+          uint64_t pr[16], ds[16];
+#pragma unroll
+          for (int e = 0; e < 16; e += 2) {
+            uint64_t l0 = minus_lse, l1 = minus_lse, d0 = minus_delta, d1 = minus_delta;
+            if constexpr (KEYS) {
+              const float4 l = *reinterpret_cast<const float4*>(stats + c0 + 2 * e);
+              const float4 d = *reinterpret_cast<const float4*>(stats + kMoving + c0 + 2 * e);
+              l0 = both(l.x, l.y), l1 = both(l.z, l.w), d0 = both(d.x, d.y), d1 = both(d.z, d.w);
+            }
+            const uint64_t x0 = fma2(both(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), scale, l0);
+            const uint64_t x1 =
+                fma2(both(__uint_as_float(sv[2 * e + 2]), __uint_as_float(sv[2 * e + 3])), scale, l1);
+            const float2 t0 = halves(x0), t1 = halves(x1);
+            pr[e] = both(ex2(t0.x), ex2(t0.y));
+            pr[e + 1] = both(ex2(t1.x), ex2(t1.y));
+            ds[e] = mul2(pr[e], add2(both(__uint_as_float(dv[2 * e]), __uint_as_float(dv[2 * e + 1])), d0));
+            ds[e + 1] =
+                mul2(pr[e + 1], add2(both(__uint_as_float(dv[2 * e + 2]), __uint_as_float(dv[2 * e + 3])), d1));
           }
           if (!all_seen) {
-            int last = min(pos, s.n - 1) - key;
-            if (i < q.ns) last = min(last, w.sinks - 1 - key);
-            if (!valid) last = -1;
-            const int near = pos - w.window + 1 - key, kept = w.sinks - key;
+            uint32_t seen = below(hi + 1 - c0) & ~below(lo - c0);
+            if (!KEYS) seen &= ~below(near - c0) | below(kept - c0);
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (c0 + e > last || (c0 + e < near && c0 + e >= kept)) ds[e] = 0.f;
+            for (int e = 0; e < 16; ++e) {
+              const float2 a = halves(pr[e]), d = halves(ds[e]);
+              const bool first = seen & (1u << (2 * e)), second = seen & (2u << (2 * e));
+              pr[e] = both(first ? a.x : 0.f, second ? a.y : 0.f);
+              ds[e] = both(first ? d.x : 0.f, second ? d.y : 0.f);
+            }
           }
-        }
-        // Operands over this group's own columns: plane pl of both K steps is 16 columns.
+          // Operands over the columns just read: plane pl of both K steps is 16 columns.
 #pragma unroll
-        for (int pl = 0; pl < NP; ++pl) {
-          uint32_t u[16];
-          if constexpr (KEYS) {
+          for (int pl = 0; pl < NP; ++pl) {
+            uint32_t u[16];
+            auto pack = [&](uint64_t& v) -> uint32_t {
+              float2 t = halves(v);
+              if constexpr (NP == 1) return pack_bf16(t.x, t.y);
+              const uint32_t upper = take_upper(t.x, t.y);
+              v = both(t.x, t.y);
+              return upper;
+            };
+            if constexpr (KEYS) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e)
-              u[e] = NP == 1 ? pack_bf16(pr[2 * e], pr[2 * e + 1]) : take_upper(pr[2 * e], pr[2 * e + 1]);
-            tc::tmem_store_32x16(buf + operand_col<KEYS>(0, pl, 0) + (pl < 2 ? g * 32 : g * 16), u);
+              for (int e = 0; e < 16; ++e) u[e] = pack(pr[e]);
+              tc::tmem_store_32x16_async(
+                  buf + operand_col<KEYS>(0, pl, 0) + (pl < 2 ? half * 32 : half * 16), u);
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) u[e] = pack(ds[e]);
+            tc::tmem_store_32x16_async(
+                buf + operand_col<KEYS>(KEYS ? 1 : 0, pl, 0) + (pl < 2 || !KEYS ? half * 32 : half * 16), u);
           }
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            u[e] = NP == 1 ? pack_bf16(ds[2 * e], ds[2 * e + 1]) : take_upper(ds[2 * e], ds[2 * e + 1]);
-          tc::tmem_store_32x16(
-              buf + operand_col<KEYS>(KEYS ? 1 : 0, pl, 0) + (pl < 2 || !KEYS ? g * 32 : g * 16), u);
         }
         // Moving rows behind the sequence may hold anything, and 0 times NaN is NaN: clear them.
         if (clear < kMoving && s.n < (KEYS ? s.p0 + w.q_len : w.kv_len)) {
           if (!KEYS && !(ok = wait_or_abort(m_full + st, m / ST, abort_flag))) break;
           uint8_t* mt = smem + L::kB + st * 2 * L::kMov;
-          for (int c = max(clear, 0) * 8 + (static_cast<int>(threadIdx.x) - 64); c < kMoving * 8; c += 256)
-            for (int box = 0; box < (KEYS ? 2 : 1) * NP * kBoxes; ++box)
-              *reinterpret_cast<uint4*>(mt + box * kMoving * 128 + c * 16) = make_uint4(0, 0, 0, 0);
+          for (int c = max(clear, 0) * 8 + (kTurns ? r : g * 128 + r); c < kMoving * 8; c += kTurns ? 128 : 256)
+            for (int op = 0; op < (KEYS ? 2 : 1) * NP * kBoxes; ++op)
+              *reinterpret_cast<uint4*>(mt + op * kMoving * 128 + c * 16) = make_uint4(0, 0, 0, 0);
           tc::fence_proxy_async_smem();
         }
         if constexpr (NP > 1) {
@@ -1190,6 +1223,7 @@ __global__ void __launch_bounds__(320, 1) window_backward_kernel(
             add_sums(i == 1);
           }
         }
+        tc::tmem_store_wait();
         tc::tc_fence_before();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(pd_full + m % L::kBuffers);
