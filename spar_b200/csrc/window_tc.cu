@@ -829,15 +829,20 @@ __device__ __forceinline__ KeyItem key_item(const BackwardParams& p, int idx) {
 
 template <bool KEYS, int DH, int NP, int ST>
 struct Bwd {
-  static constexpr int kBuffers = KEYS && NP > 1 ? 1 : 2;
+  // Buffers of S and dP: three where TMEM has room, so that the two softmax groups find their next
+  // scores ready; not more than stages, as scores run that far ahead of the last use of a stage.
+  static constexpr int kBuffers = NP > 1 ? (KEYS ? 1 : 2) : KEYS && DH == 128 ? 2 : 3;
+  static_assert(kBuffers <= ST, "stages");
+  static constexpr uint32_t kStats = NP == 1 && DH == 64 ? 2 : 1;  // pairs of stationary operands
   static constexpr uint32_t kStat = NP * DH * 256;            // one stationary operand
   static constexpr uint32_t kMov = NP * DH * kMoving * 2;     // one moving operand
   static constexpr uint32_t kA = 0;
-  static constexpr uint32_t kB = kA + 2 * kStat;
+  static constexpr uint32_t kB = kA + kStats * 2 * kStat;
   static constexpr uint32_t kOut = kB + ST * 2 * kMov;        // 4 KB per softmax warp
   static constexpr uint32_t kRows = kOut + 8 * 4096;          // [ST][2][64] -lse log2 e, -D
   static constexpr uint32_t kBar = kRows + (KEYS ? ST * kMoving * 8 : 0);
   static constexpr uint32_t kSmem = kBar + 256 + 1024;
+  static_assert((13 + 2 * ST) * 8 + 8 <= 256, "backward barriers");
   static_assert(kSmem <= kMaxSmem, "backward shared memory");
   // TMEM: buffers of S | dP (| the third planes of P and dS), then the products' sums, then
   // (NP = 3) the sums of earlier tiles.
@@ -860,21 +865,21 @@ __host__ __device__ constexpr uint32_t operand_col(int which, int pl, int ks) {
 }
 
 template <bool KEYS, int DH, int NP, int ST>
-__global__ void __launch_bounds__(320, 1) window_backward_kernel(
+__global__ void __launch_bounds__(384, 1) window_backward_kernel(
     const __grid_constant__ BackwardParams p) {
   using L = Bwd<KEYS, DH, NP, ST>;
   constexpr int kBoxes = DH / 64;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBar);
-  uint64_t* a_full = bars;
-  uint64_t* a_empty = bars + 1;
-  uint64_t* s_full = bars + 2;    // [2]
-  uint64_t* pd_full = bars + 4;   // [2]
-  uint64_t* sum_full = bars + 6;  // the products of a tile (NP = 3) or item are complete
-  uint64_t* sum_empty = bars + 7;
-  uint64_t* drain = bars + 8;
-  uint64_t* m_full = bars + 9;    // [ST]
+  uint64_t* a_full = bars;         // [2]
+  uint64_t* a_empty = bars + 2;    // [2]
+  uint64_t* s_full = bars + 4;     // [3]
+  uint64_t* pd_full = bars + 7;    // [3]
+  uint64_t* sum_full = bars + 10;  // the products of a tile (NP = 3) or item are complete
+  uint64_t* sum_empty = bars + 11;
+  uint64_t* drain = bars + 12;
+  uint64_t* m_full = bars + 13;    // [ST]
   uint64_t* m_empty = m_full + ST;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(m_empty + ST);
   const Abort abort_flag = {reinterpret_cast<volatile int*>(tmem_slot + 1), p.wait_flag};
@@ -882,9 +887,11 @@ __global__ void __launch_bounds__(320, 1) window_backward_kernel(
   const WindowParams& w = p.w;
 
   if (threadIdx.x == 0) {
-    tc::mbar_init(a_full, 1);
-    tc::mbar_init(a_empty, 1);
     for (int i = 0; i < 2; ++i) {
+      tc::mbar_init(a_full + i, 1);
+      tc::mbar_init(a_empty + i, 1);
+    }
+    for (int i = 0; i < 3; ++i) {
       tc::mbar_init(s_full + i, 1);
       tc::mbar_init(pd_full + i, NP == 1 ? 4 : 8);
     }
@@ -919,160 +926,168 @@ __global__ void __launch_bounds__(320, 1) window_backward_kernel(
     }
   };
 
-  if (warp == 0) {
-    // -------------------------------------------------------------- TMA producer (whole warp)
-    if (lane == 0) {
-      tc::tma_prefetch(&p.s1);
-      tc::tma_prefetch(&p.s2);
-      tc::tma_prefetch(&p.m1);
-      tc::tma_prefetch(&p.m2);
-    }
-    uint32_t an = 0, mn = 0;
-    bool ok = true;
-    for (int idx = blockIdx.x; idx < p.items && ok && !*abort_flag.cta; idx += gridDim.x) {
-      Item q;
-      KeyItem k;
-      const int n = jobs_of(idx, q, k);
-      if (!n) continue;
-      const int b = KEYS ? k.b : q.b;
-      if (!(ok = wait_or_abort(a_empty, an + 1, abort_flag))) break;
-      ++an;
+  // As in the forward: 88 registers a thread for the four feeding warps, 208 for the eight others.
+  if (warp < 4) {
+    registers_down<88>();
+    if (warp == 0) {
+      // -------------------------------------------------------------- TMA producer (whole warp)
       if (lane == 0) {
-        tc::mbar_arrive_expect_tx(a_full, 2 * L::kStat);
-        for (int pl = 0; pl < NP; ++pl)
-          for (int c = 0; c < kBoxes; ++c) {
-            uint8_t* dst = smem + L::kA + (pl * kBoxes + c) * 16384;
-            const int row = KEYS ? k.key : q.row[0], h = KEYS ? k.kh : q.h[0];
-            tc::tma_load_5d(dst, &p.s1, a_full, 64 * c, row, h, b, pl);
-            tc::tma_load_5d(dst + L::kStat, &p.s2, a_full, 64 * c, row, h, b, pl);
-          }
+        tc::tma_prefetch(&p.s1);
+        tc::tma_prefetch(&p.s2);
+        tc::tma_prefetch(&p.m1);
+        tc::tma_prefetch(&p.m2);
       }
-      __syncwarp();
-      for (int i = 0; i < n && ok; ++i, ++mn) {
-        const uint32_t st = mn % ST;
-        if (!(ok = wait_or_abort(m_empty + st, mn / ST + 1, abort_flag))) break;
-        int row, h;
-        if constexpr (KEYS) {
-          const int head = i / k.jobs_per_head;
-          row = k.row + (i - head * k.jobs_per_head) * kMoving;
-          h = k.head + head;
-        } else {
-          row = key_of<kMoving>(q, i);
-          h = q.kh;
-        }
-        if (lane == 0) {
-          tc::mbar_arrive_expect_tx(m_full + st, 2 * L::kMov);
-          for (int pl = 0; pl < NP; ++pl)
-            for (int c = 0; c < kBoxes; ++c) {
-              uint8_t* dst = smem + L::kB + st * 2 * L::kMov + (pl * kBoxes + c) * kMoving * 128;
-              tc::tma_load_5d(dst, &p.m1, m_full + st, 64 * c, row, h, b, pl);
-              tc::tma_load_5d(dst + L::kMov, &p.m2, m_full + st, 64 * c, row, h, b, pl);
-            }
-        }
-        if constexpr (KEYS) {
-          float* stats = reinterpret_cast<float*>(smem + L::kRows) + st * 2 * kMoving;
-          const uint64_t at = (static_cast<uint64_t>(b) * w.heads + h) * w.q_len;
-#pragma unroll
-          for (int e = lane; e < kMoving; e += 32) {
-            const bool in = row + e < k.end;
-            stats[e] = in ? -__ldg(w.lse + at + row + e) * kLog2e : 0.f;
-            stats[kMoving + e] = in ? -__ldg(w.delta + at + row + e) : 0.f;
-          }
-          __syncwarp();
-          if (lane == 0) tc::mbar_arrive(m_full + st);
-        }
-        __syncwarp();
-      }
-    }
-    if (an) wait_or_abort(a_full, an - 1, abort_flag);
-    for (uint32_t i = mn > ST ? mn - ST : 0; i < mn; ++i)
-      wait_or_abort(m_full + i % ST, i / ST, abort_flag);
-  } else if (warp == 1) {
-    // -------------------------------------------------------------- product issuer
-    if (tc::elect_one()) {
-      const uint32_t idesc_s = tc::idesc_bf16(128, kMoving, 0, 0);
-      const uint32_t idesc_o = tc::idesc_bf16(128, 16 * p.ksteps, 0, 1);
-      const uint32_t a_addr = tc::smem_u32(smem + L::kA), b_addr = tc::smem_u32(smem + L::kB);
-      uint32_t an = 0, mn = 0, sums = 0;
+      uint32_t an = 0, mn = 0;
       bool ok = true;
-      // S and dP of moving tile number m; after the item's last one the stationary operands are free.
-      auto scores = [&](uint32_t m, bool last) -> bool {
-        const uint32_t st = m % ST, buf = tmem + (m % L::kBuffers) * L::kBuf;
-        if (!wait_or_abort(m_full + st, m / ST, abort_flag)) return false;
-        tc::tc_fence_after();
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          const uint32_t a = kmajor_low(a_addr + half * L::kStat),
-                         b = kmajor_low(b_addr + (2 * st + half) * L::kMov);
-          uint32_t acc = 0;
-#pragma unroll
-          for (int pr = 0; pr < kProducts<NP>; ++pr)
-#pragma unroll
-            for (int ks = 0; ks < DH / 16; ++ks)
-              if (ks < p.ksteps) {
-                tc::mma_f16(buf + half * 64, desc(a + kmajor_step(128, plane_a<NP>(pr), kBoxes, ks)),
-                            desc(b + kmajor_step(kMoving, plane_b<NP>(pr), kBoxes, ks)), idesc_s, acc);
-                acc = 1;
-              }
-        }
-        tc::mma_commit(s_full + m % L::kBuffers);
-        if (last) tc::mma_commit(a_empty);
-        return true;
-      };
       for (int idx = blockIdx.x; idx < p.items && ok && !*abort_flag.cta; idx += gridDim.x) {
         Item q;
         KeyItem k;
         const int n = jobs_of(idx, q, k);
         if (!n) continue;
-        if (!(ok = wait_or_abort(a_full, an, abort_flag))) break;
+        const int b = KEYS ? k.b : q.b;
+        const uint32_t as = an % L::kStats;
+        if (!(ok = wait_or_abort(a_empty + as, an / L::kStats + 1, abort_flag))) break;
         ++an;
-        ok = scores(mn, n == 1);
-        for (int i = 0; i < n && ok; ++i) {
-          const uint32_t m = mn + i, st = m % ST, buf = tmem + (m % L::kBuffers) * L::kBuf;
-          // The other buffer was last read by the products of two tiles back, issued before.
-          if (L::kBuffers == 2 && i + 1 < n && !(ok = scores(m + 1, i + 2 == n))) break;
-          if (!(ok = wait_or_abort(pd_full + m % L::kBuffers, m / L::kBuffers, abort_flag))) break;
-          // Sums start afresh with an item; the softmax warps have read the ones before.
-          if (i == 0 && !(ok = wait_or_abort(sum_empty, sums + 1, abort_flag))) break;
+        if (lane == 0) {
+          tc::mbar_arrive_expect_tx(a_full + as, 2 * L::kStat);
+          for (int pl = 0; pl < NP; ++pl)
+            for (int c = 0; c < kBoxes; ++c) {
+              uint8_t* dst = smem + L::kA + as * 2 * L::kStat + (pl * kBoxes + c) * 16384;
+              const int row = KEYS ? k.key : q.row[0], h = KEYS ? k.kh : q.h[0];
+              tc::tma_load_5d(dst, &p.s1, a_full + as, 64 * c, row, h, b, pl);
+              tc::tma_load_5d(dst + L::kStat, &p.s2, a_full + as, 64 * c, row, h, b, pl);
+            }
+        }
+        __syncwarp();
+        for (int i = 0; i < n && ok; ++i, ++mn) {
+          const uint32_t st = mn % ST;
+          if (!(ok = wait_or_abort(m_empty + st, mn / ST + 1, abort_flag))) break;
+          int row, h;
+          if constexpr (KEYS) {
+            const int head = i / k.jobs_per_head;
+            row = k.row + (i - head * k.jobs_per_head) * kMoving;
+            h = k.head + head;
+          } else {
+            row = key_of<kMoving>(q, i);
+            h = q.kh;
+          }
+          if (lane == 0) {
+            tc::mbar_arrive_expect_tx(m_full + st, 2 * L::kMov);
+            for (int pl = 0; pl < NP; ++pl)
+              for (int c = 0; c < kBoxes; ++c) {
+                uint8_t* dst = smem + L::kB + st * 2 * L::kMov + (pl * kBoxes + c) * kMoving * 128;
+                tc::tma_load_5d(dst, &p.m1, m_full + st, 64 * c, row, h, b, pl);
+                tc::tma_load_5d(dst + L::kMov, &p.m2, m_full + st, 64 * c, row, h, b, pl);
+              }
+          }
+          if constexpr (KEYS) {
+            float* stats = reinterpret_cast<float*>(smem + L::kRows) + st * 2 * kMoving;
+            const uint64_t at = (static_cast<uint64_t>(b) * w.heads + h) * w.q_len;
+#pragma unroll
+            for (int e = lane; e < kMoving; e += 32) {
+              const bool in = row + e < k.end;
+              stats[e] = in ? -__ldg(w.lse + at + row + e) * kLog2e : 0.f;
+              stats[kMoving + e] = in ? -__ldg(w.delta + at + row + e) : 0.f;
+            }
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(m_full + st);
+          }
+          __syncwarp();
+        }
+      }
+      for (uint32_t i = an > L::kStats ? an - L::kStats : 0; i < an; ++i)
+        wait_or_abort(a_full + i % L::kStats, i / L::kStats, abort_flag);
+      for (uint32_t i = mn > ST ? mn - ST : 0; i < mn; ++i)
+        wait_or_abort(m_full + i % ST, i / ST, abort_flag);
+    } else if (warp == 1) {
+      // -------------------------------------------------------------- product issuer
+      if (tc::elect_one()) {
+        const uint32_t idesc_s = tc::idesc_bf16(128, kMoving, 0, 0);
+        const uint32_t idesc_o = tc::idesc_bf16(128, 16 * p.ksteps, 0, 1);
+        const uint32_t a_addr = tc::smem_u32(smem + L::kA), b_addr = tc::smem_u32(smem + L::kB);
+        uint32_t an = 0, mn = 0, sums = 0;
+        bool ok = true;
+        // S and dP of moving tile number m; after the item's last one the stationary operands are free.
+        auto scores = [&](uint32_t m, bool last) -> bool {
+          const uint32_t st = m % ST, buf = tmem + (m % L::kBuffers) * L::kBuf;
+          if (!wait_or_abort(m_full + st, m / ST, abort_flag)) return false;
           tc::tc_fence_after();
 #pragma unroll
-          for (int out = 0; out < static_cast<int>(L::kOuts); ++out) {
-            // queries: dq += dS k; keys: dk += dS^T q, dv += P^T dout
-            const int which = KEYS ? 1 - out : 0;
-            const uint32_t b = mnmajor_low(b_addr + (2 * st + out) * L::kMov, kMoving);
-            uint32_t acc = NP == 1 && i > 0;
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t a = kmajor_low(a_addr + (2 * (an % L::kStats) + half) * L::kStat),
+                           b = kmajor_low(b_addr + (2 * st + half) * L::kMov);
+            uint32_t acc = 0;
 #pragma unroll
             for (int pr = 0; pr < kProducts<NP>; ++pr)
 #pragma unroll
-              for (int ks = 0; ks < kMoving / 16; ++ks) {
-                tc::mma_f16_ts(tmem + L::kAcc + out * DH, buf + operand_col<KEYS>(which, plane_a<NP>(pr), ks),
-                               desc(b + mnmajor_step(kMoving, plane_b<NP>(pr), kBoxes, ks)), idesc_o, acc);
-                acc = 1;
-              }
+              for (int ks = 0; ks < DH / 16; ++ks)
+                if (ks < p.ksteps) {
+                  tc::mma_f16(buf + half * 64, desc(a + kmajor_step(128, plane_a<NP>(pr), kBoxes, ks)),
+                              desc(b + kmajor_step(kMoving, plane_b<NP>(pr), kBoxes, ks)), idesc_s, acc);
+                  acc = 1;
+                }
           }
-          tc::mma_commit(m_empty + st);
-          if (NP > 1 || i + 1 == n) tc::mma_commit(sum_full);
-          if (L::kBuffers == 1 && i + 1 < n) ok = scores(m + 1, i + 2 == n);
+          tc::mma_commit(s_full + m % L::kBuffers);
+          if (last) tc::mma_commit(a_empty + an % L::kStats);
+          return true;
+        };
+        for (int idx = blockIdx.x; idx < p.items && ok && !*abort_flag.cta; idx += gridDim.x) {
+          Item q;
+          KeyItem k;
+          const int n = jobs_of(idx, q, k);
+          if (!n) continue;
+          if (!(ok = wait_or_abort(a_full + an % L::kStats, an / L::kStats, abort_flag))) break;
+          constexpr int kAhead = L::kBuffers > 1 ? L::kBuffers - 1 : 1;
+          for (int i = 0; i < kAhead && i < n && ok; ++i) ok = scores(mn + i, i + 1 == n);
+          for (int i = 0; i < n && ok; ++i) {
+            const uint32_t m = mn + i, st = m % ST, buf = tmem + (m % L::kBuffers) * L::kBuf;
+            // The buffer of tile i + kAhead was last read by the products of tile i - 1, issued before.
+            if (L::kBuffers > 1 && i + kAhead < n && !(ok = scores(m + kAhead, i + kAhead + 1 == n))) break;
+            if (!(ok = wait_or_abort(pd_full + m % L::kBuffers, m / L::kBuffers, abort_flag))) break;
+            // Sums start afresh with an item; the softmax warps have read the ones before.
+            if (i == 0 && !(ok = wait_or_abort(sum_empty, sums + 1, abort_flag))) break;
+            tc::tc_fence_after();
+#pragma unroll
+            for (int out = 0; out < static_cast<int>(L::kOuts); ++out) {
+              // queries: dq += dS k; keys: dk += dS^T q, dv += P^T dout
+              const int which = KEYS ? 1 - out : 0;
+              const uint32_t b = mnmajor_low(b_addr + (2 * st + out) * L::kMov, kMoving);
+              uint32_t acc = NP == 1 && i > 0;
+#pragma unroll
+              for (int pr = 0; pr < kProducts<NP>; ++pr)
+#pragma unroll
+                for (int ks = 0; ks < kMoving / 16; ++ks) {
+                  tc::mma_f16_ts(tmem + L::kAcc + out * DH, buf + operand_col<KEYS>(which, plane_a<NP>(pr), ks),
+                                 desc(b + mnmajor_step(kMoving, plane_b<NP>(pr), kBoxes, ks)), idesc_o, acc);
+                  acc = 1;
+                }
+            }
+            tc::mma_commit(m_empty + st);
+            if (NP > 1 || i + 1 == n) tc::mma_commit(sum_full);
+            if (L::kBuffers == 1 && i + 1 < n) ok = scores(m + 1, i + 2 == n);
+          }
+          mn += n;
+          ++sums;
+          ++an;
         }
-        mn += n;
-        ++sums;
+        tc::mma_commit(drain);
+        wait_or_abort(drain, 0, abort_flag);
       }
-      tc::mma_commit(drain);
-      wait_or_abort(drain, 0, abort_flag);
+      __syncwarp();
     }
-    __syncwarp();
   } else {
     // -------------------------------------------------------------- softmax and results
+    registers_up<208>();
     // bf16: the two groups take the tiles in turn, all 64 columns each (in two halves, as registers
     // allow): while one waits the other works. Half of every tile each took 1460 cycles a tile of
     // 64, most of it in waits and in the latency of two warps a scheduler that did the same.
     // fp32, whose keys have one buffer: half of every tile each.
     constexpr bool kTurns = NP == 1;
-    const int g = (warp - 2) >> 2;
+    const int g = (warp - 4) >> 2;
     const uint32_t quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const uint32_t lanes = tmem + ((quarter * 32) << 16);
-    const Box box = {smem + L::kOut + (warp - 2) * 4096};
+    const Box box = {smem + L::kOut + (warp - 4) * 4096};
     const uint64_t scale = both(p.scale_log2, p.scale_log2);
     uint32_t mn = 0, sums = 0;
     bool ok = true;
@@ -1485,7 +1500,7 @@ cudaError_t launch_backward(const BackwardParams& p, int device, cudaStream_t st
   const cudaError_t e = raise_dynamic_smem(reinterpret_cast<const void*>(kernel), device, L::kSmem);
   if (e != cudaSuccess) return e;
   const unsigned grid = static_cast<unsigned>(std::min(p.items, sm_count(device)));
-  return launch(kernel, dim3(grid), dim3(320), L::kSmem, stream, p);
+  return launch(kernel, dim3(grid), dim3(384), L::kSmem, stream, p);
 }
 
 }  // namespace
