@@ -27,6 +27,7 @@ namespace spar_b200 {
 namespace {
 
 constexpr uint64_t kMaxUnits = 1ull << 31;
+constexpr int kBackwardThreads = 128;
 
 // Exact quotient by a fixed divisor for dividends below 2^31: with 2^(s-1) < d <= 2^s and
 // m = ceil(2^(31+s) / d) < 2^32, floor(n m / 2^(31+s)) = floor(n / d) since n (m d - 2^(31+s)) <
@@ -328,9 +329,46 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
 // Backward of the norm and the rotation. Blocks are split between queries and keys in proportion
 // to their heads and walk their (token, head) units with the grid's stride, so a lane keeps the
 // sums of its slots' weight gradients in registers for the whole launch; a block adds its lane
-// groups' sums in a fixed order and leaves one partial row of head_dim floats.
+// groups' sums in a fixed order and leaves one partial row of head_dim floats. The next unit's x and
+// dy are under way while one is worked on: loaded on arrival the launch ran at half the bandwidth
+// (77 us for 2 x 4095 tokens of 40 heads of 128 bf16).
+template <typename T, int VEC, int U>
+struct Unit {
+  Raw<T, VEC> xa[U], xb[U], ga[U], gb[U];
+  uint64_t row, out;
+  bool live, good;
+};
+
 template <typename T, int VEC, int U, bool HALF>
-__global__ void __launch_bounds__(256) qk_norm_rotary_backward_kernel(
+__device__ __forceinline__ void load_unit(const RotaryParams& p, int side, uint64_t unit, uint64_t units,
+                                          uint32_t l, uint32_t lanes, Unit<T, VEC, U>& v) {
+  const View &in = p.in[side], &out = p.out[side], &grad = p.grad[side];
+  const uint32_t heads = p.heads[side];
+  v.live = unit < units;
+  const uint32_t t = v.live ? p.by_heads[side].quotient(static_cast<uint32_t>(unit)) : 0;
+  const uint32_t h = v.live ? static_cast<uint32_t>(unit) - t * heads : 0;
+  const uint32_t b = p.by_seq.quotient(t), in_seq = t - b * p.seq;
+  v.good = row_of(p, t, in_seq, v.row);
+  if (!v.good && v.live && l == 0 && h == 0 && p.invalid) atomicExch(p.invalid, 1);
+  v.out = b * out.batch + in_seq * out.token + h * out.head;
+  const T* px = reinterpret_cast<const T*>(in.data) + b * in.batch + in_seq * in.token + h * in.head;
+  const T* pg = reinterpret_cast<const T*>(grad.data) + b * grad.batch + in_seq * grad.token + h * grad.head;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const Slot s = slot_of<VEC, HALF>(p, l + u * lanes);
+    v.xa[u] = v.xb[u] = v.ga[u] = v.gb[u] = Raw<T, VEC>{};
+    if (!v.live || !v.good || !s.has_a) continue;
+    v.xa[u] = load_raw<T, VEC>(px + s.a);
+    v.ga[u] = load_raw<T, VEC>(pg + s.a);
+    if (s.has_b) {
+      v.xb[u] = load_raw<T, VEC>(px + s.b);
+      v.gb[u] = load_raw<T, VEC>(pg + s.b);
+    }
+  }
+}
+
+template <typename T, int VEC, int U, bool HALF>
+__global__ void __launch_bounds__(kBackwardThreads) qk_norm_rotary_backward_kernel(
     const __grid_constant__ RotaryParams p) {
   pdl_begin();
   extern __shared__ float sums[];  // [groups of the block][head_dim]
@@ -340,57 +378,42 @@ __global__ void __launch_bounds__(256) qk_norm_rotary_backward_kernel(
   const int side = blockIdx.x >= p.blocks_q;
   const uint32_t block = side ? blockIdx.x - p.blocks_q : blockIdx.x;
   const uint32_t blocks = side ? gridDim.x - p.blocks_q : p.blocks_q;
-  const uint32_t heads = p.heads[side];
-  const uint64_t units = static_cast<uint64_t>(p.tokens) * heads;
-  const View &in = p.in[side], &out = p.out[side], &grad = p.grad[side];
-  float wa[U][VEC], wb[U][VEC], da[U][VEC], db[U][VEC];
+  const uint64_t units = static_cast<uint64_t>(p.tokens) * p.heads[side];
+  float da[U][VEC], db[U][VEC];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    load_weights<VEC>(p.weight[side], slot_of<VEC, HALF>(p, l + u * lanes), wa[u], wb[u]);
+  for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int x = 0; x < VEC; ++x) da[u][x] = db[u][x] = 0.f;
-  }
-  for (uint64_t first = static_cast<uint64_t>(block) * groups; first < units;
-       first += static_cast<uint64_t>(blocks) * groups) {  // every lane: the sums are whole-warp
-    const uint64_t unit = first + group;
-    const bool live = unit < units;
-    const uint32_t t = live ? p.by_heads[side].quotient(static_cast<uint32_t>(unit)) : 0;
-    const uint32_t h = live ? static_cast<uint32_t>(unit) - t * heads : 0;
-    const uint32_t b = p.by_seq.quotient(t), in_seq = t - b * p.seq;
-    const T* px = reinterpret_cast<const T*>(in.data) + b * in.batch + in_seq * in.token + h * in.head;
-    const T* pg = reinterpret_cast<const T*>(grad.data) + b * grad.batch + in_seq * grad.token +
-                  h * grad.head;
-    T* po = reinterpret_cast<T*>(out.data) + b * out.batch + in_seq * out.token + h * out.head;
-    uint64_t row = 0;
-    const bool good = row_of(p, t, in_seq, row);
-    if (!good && live && l == 0 && h == 0 && p.invalid) atomicExch(p.invalid, 1);
+  T* out = reinterpret_cast<T*>(p.out[side].data);
+  const uint64_t stride = static_cast<uint64_t>(blocks) * groups;
+  Unit<T, VEC, U> cur, next;
+  uint64_t first = static_cast<uint64_t>(block) * groups;
+  if (first < units) load_unit<T, VEC, U, HALF>(p, side, first + group, units, l, lanes, cur);
+  for (; first < units; first += stride) {  // every lane: the sums are whole-warp
+    float2 cs[U][VEC];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const Slot s = slot_of<VEC, HALF>(p, l + u * lanes);
+      if (s.turns && cur.good) load_angles<VEC, HALF>(p, s, cur.row, cs[u]);
+    }
+    if (first + stride < units)
+      load_unit<T, VEC, U, HALF>(p, side, first + stride + group, units, l, lanes, next);
     float xa[U][VEC], xb[U][VEC], ga[U][VEC], gb[U][VEC];
     float ss = 0.f, dot = 0.f;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const Slot s = slot_of<VEC, HALF>(p, l + u * lanes);
-#pragma unroll
-      for (int x = 0; x < VEC; ++x) xa[u][x] = xb[u][x] = ga[u][x] = gb[u][x] = 0.f;
-      if (!live || !s.has_a || !good) continue;
-      const Raw<T, VEC> rxa = load_raw<T, VEC>(px + s.a), rga = load_raw<T, VEC>(pg + s.a);
-      Raw<T, VEC> rxb, rgb;
-      if (s.has_b) {
-        rxb = load_raw<T, VEC>(px + s.b);
-        rgb = load_raw<T, VEC>(pg + s.b);
-      }
-      float2 cs[VEC];
-      if (s.turns) load_angles<VEC, HALF>(p, s, row, cs);
-      widen<T, VEC>(rxa, xa[u]);
-      widen<T, VEC>(rga, ga[u]);
-      if (s.has_b) {
-        widen<T, VEC>(rxb, xb[u]);
-        widen<T, VEC>(rgb, gb[u]);
-      }
-      if (s.turns) turn<VEC, HALF>(ga[u], gb[u], cs, -1.f);
+      float wa[VEC], wb[VEC];
+      load_weights<VEC>(p.weight[side], s, wa, wb);  // cached; held for the launch they cost occupancy
+      widen<T, VEC>(cur.xa[u], xa[u]);
+      widen<T, VEC>(cur.xb[u], xb[u]);
+      widen<T, VEC>(cur.ga[u], ga[u]);
+      widen<T, VEC>(cur.gb[u], gb[u]);
+      if (s.turns && cur.good) turn<VEC, HALF>(ga[u], gb[u], cs[u], -1.f);
 #pragma unroll
       for (int x = 0; x < VEC; ++x) {
         ss += xa[u][x] * xa[u][x] + xb[u][x] * xb[u][x];
-        dot += ga[u][x] * wa[u][x] * xa[u][x] + gb[u][x] * wb[u][x] * xb[u][x];
+        dot += ga[u][x] * wa[x] * xa[u][x] + gb[u][x] * wb[x] * xb[u][x];
       }
     }
     for (uint32_t o = lanes >> 1; o > 0; o >>= 1) {
@@ -399,25 +422,28 @@ __global__ void __launch_bounds__(256) qk_norm_rotary_backward_kernel(
     }
     const float r = 1.0f / sqrtf(ss * p.inv_dim + p.eps);
     const float m = dot * r * p.inv_dim;  // mean(g w x r)
-    if (!live) continue;
+    if (cur.live) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const Slot s = slot_of<VEC, HALF>(p, l + u * lanes);
-      if (!s.has_a) continue;
-      float oa[VEC], ob[VEC];
+      for (int u = 0; u < U; ++u) {
+        const Slot s = slot_of<VEC, HALF>(p, l + u * lanes);
+        if (!s.has_a) continue;
+        float wa[VEC], wb[VEC], oa[VEC], ob[VEC];
+        load_weights<VEC>(p.weight[side], s, wa, wb);
 #pragma unroll
-      for (int x = 0; x < VEC; ++x) {
-        const float ua = xa[u][x] * r, ub = xb[u][x] * r;
-        oa[x] = good ? r * (ga[u][x] * wa[u][x] - ua * m) : 0.f;
-        ob[x] = good ? r * (gb[u][x] * wb[u][x] - ub * m) : 0.f;
-        if (good) {
-          da[u][x] += ga[u][x] * ua;
-          db[u][x] += gb[u][x] * ub;
+        for (int x = 0; x < VEC; ++x) {
+          const float ua = xa[u][x] * r, ub = xb[u][x] * r;
+          oa[x] = cur.good ? r * (ga[u][x] * wa[x] - ua * m) : 0.f;
+          ob[x] = cur.good ? r * (gb[u][x] * wb[x] - ub * m) : 0.f;
+          if (cur.good) {
+            da[u][x] += ga[u][x] * ua;
+            db[u][x] += gb[u][x] * ub;
+          }
         }
+        store_vec<T, VEC>(out + cur.out + s.a, oa);
+        if (s.has_b) store_vec<T, VEC>(out + cur.out + s.b, ob);
       }
-      store_vec<T, VEC>(po + s.a, oa);
-      if (s.has_b) store_vec<T, VEC>(po + s.b, ob);
     }
+    cur = next;
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -461,19 +487,18 @@ __global__ void __launch_bounds__(1024) qk_weight_partials_kernel(float* dq, flo
   if (x == 0 && c < head_dim && d) d[c] = accumulate ? d[c] + s : s;
 }
 
-// One thread per (pair, run of kRun positions): the first angle's cos and sin, then kRun - 1
-// rotations by one position in double (each adds ~2^-52, far below the fp32 result's 2^-25),
+// One thread per (pair, run of positions): the first angle's cos and sin, then rotations by one position in double (each adds ~2^-52, far below the fp32 result's 2^-25),
 // which turns ~100 double operations per entry into four and leaves the launch bound by its
 // stores.
-constexpr uint32_t kRun = 32;
+// The run is as long as leaves 32768 threads, 8 to 128 positions.
 __global__ void __launch_bounds__(256) rotary_table_kernel(float2* table, uint64_t rows,
-                                                           uint32_t pairs, uint64_t start,
+                                                           uint32_t pairs, uint64_t start, uint32_t length,
                                                            SparB200RotaryScaling sc, double theta) {
   pdl_begin();
   const uint64_t idx = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   const uint64_t run = idx / pairs;
   const uint32_t i = static_cast<uint32_t>(idx - run * pairs);
-  const uint64_t r0 = run * kRun;
+  const uint64_t r0 = run * length;
   if (r0 >= rows) return;
   double f = pow(theta, -static_cast<double>(i) / static_cast<double>(pairs));
   if (sc.kind == SPAR_B200_ROTARY_LINEAR) f /= sc.factor;
@@ -486,7 +511,7 @@ __global__ void __launch_bounds__(256) rotary_table_kernel(float2* table, uint64
   double c, s, dc, ds;
   sincos(static_cast<double>(start + r0) * f, &s, &c);
   sincos(f, &ds, &dc);
-  const uint64_t n = min(static_cast<uint64_t>(kRun), rows - r0);
+  const uint64_t n = min(static_cast<uint64_t>(length), rows - r0);
   float2* out = table + r0 * pairs + i;
   for (uint64_t r = 0; r < n; ++r) {
     out[r * pairs] = make_float2(static_cast<float>(c * sc.magnitude),
@@ -506,7 +531,7 @@ View view_of(const SparB200Heads& v, uint64_t batch, uint64_t seq, uint64_t head
           heads > 1 ? v.head : 0};
 }
 
-constexpr int kBackwardBlocksPerSM = 4;
+constexpr int kBackwardBlocksPerSM = 4;  // as many of 128 threads as run at once (vectorised bf16)
 
 uint32_t backward_blocks(int device) {
   return static_cast<uint32_t>(sm_count(device)) * kBackwardBlocksPerSM;
@@ -625,7 +650,7 @@ SparCudaStatus run_forward(const SparB200Rotary* r, int device, void* stream) {
 
 template <typename T, int VEC, int U, bool HALF>
 cudaError_t launch_backward(RotaryParams& p, int device, cudaStream_t stream, uint32_t& grid) {
-  const uint32_t groups = 256u >> p.lanes_log2;
+  const uint32_t groups = kBackwardThreads >> p.lanes_log2;
   const uint64_t need[2] = {(static_cast<uint64_t>(p.tokens) * p.heads[0] + groups - 1) / groups,
                             (static_cast<uint64_t>(p.tokens) * p.heads[1] + groups - 1) / groups};
   const uint32_t most = backward_blocks(device);
@@ -638,7 +663,7 @@ cudaError_t launch_backward(RotaryParams& p, int device, cudaStream_t stream, ui
   }
   p.blocks_q = static_cast<uint32_t>(nq);
   grid = static_cast<uint32_t>(nq + nk);
-  return launch(qk_norm_rotary_backward_kernel<T, VEC, U, HALF>, dim3(grid), dim3(256),
+  return launch(qk_norm_rotary_backward_kernel<T, VEC, U, HALF>, dim3(grid), dim3(kBackwardThreads),
                 groups * p.head_dim * sizeof(float), stream, p);
 }
 
@@ -676,14 +701,16 @@ extern "C" SparCudaStatus spar_b200_rotary_table(float* table, uint64_t rows, ui
                        : 1.0;
   if (rows == 0) return ok();
   if (!table || (reinterpret_cast<uintptr_t>(table) & 7)) return invalid();
-  const uint64_t pairs = rotary_dim / 2, threads = (rows + kRun - 1) / kRun * pairs;
+  const uint64_t pairs = rotary_dim / 2;
+  const uint64_t length = std::min<uint64_t>(128, std::max<uint64_t>(8, rows * pairs / 32768));
+  const uint64_t threads = (rows + length - 1) / length * pairs;
   if ((threads + 255) / 256 > 0x7fffffffull) return invalid();
   DeviceScope scope(device);
   if (scope.error() != cudaSuccess) return runtime(scope.error());
   const cudaError_t e =
       launch(rotary_table_kernel, dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0,
              static_cast<cudaStream_t>(stream), reinterpret_cast<float2*>(table), rows,
-             static_cast<uint32_t>(pairs), start, sc, theta);
+             static_cast<uint32_t>(pairs), start, static_cast<uint32_t>(length), sc, theta);
   return e == cudaSuccess ? launch_status() : runtime(e);
 }
 

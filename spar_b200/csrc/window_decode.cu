@@ -3,8 +3,9 @@
 //
 // The floor is one read of the visible keys and values, which all query heads of a key head share:
 // a CTA takes up to 8 or 16 rows (heads of one group, times tokens) and a range of the visible keys,
-// so that a cache row is loaded once for all of them, straight from memory into the registers that
-// use it and one step ahead of its use. Each warp (or lane group) keeps its own running maximum,
+// so that a cache row is loaded once for all of them: by cp.async, three steps ahead (one step ahead
+// in registers every step waited for memory: 4 TB/s), each lane into slots of shared memory that it
+// alone reads, so nothing but its own copies is waited for. Each warp (or lane group) keeps its own running maximum,
 // sum and output; they are joined in shared memory, and the ranges of one row over the shared
 // memory of a cluster of up to eight CTAs, or, where it takes more to fill the machine, by a second
 // launch. Both add in a fixed order.
@@ -29,7 +30,8 @@ namespace window {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kKeys = 4;  // rows of the cache in flight per lane group
+constexpr int kKeys = 4;    // rows of the cache that a lane group takes at once
+constexpr int kStages = 4;  // steps of the ring (three under way, about 100 KB an SM)
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -46,6 +48,18 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// 16 bytes of the cache into this lane's slot, or zeros.
+__device__ __forceinline__ void copy16(uint4* slot, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(tc::smem_u32(slot)), "l"(src),
+               "r"(there ? 16 : 0)
+               : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
 template <typename T>
@@ -193,26 +207,30 @@ __global__ void __launch_bounds__(kThreads) window_decode_kernel(
   }
   const T* kb = row_ptr<T>(w.k, b, 0, kh) + l * V;
   const T* vb = row_ptr<T>(w.v, b, 0, kh) + l * V;
-  uint4 ku[kKeys], vu[kKeys];
-  auto fetch = [&](int base) {
+  uint4* ring = reinterpret_cast<uint4*>(shared) + threadIdx.x;  // [stage][key, value][kKeys] slots
+  auto fetch = [&](int base, int stage) {
+    uint4* slot = ring + stage * 2 * kKeys * kThreads;
 #pragma unroll
     for (int x = 0; x < kKeys; ++x) {
-      const int i = base + x * groups;
-      ku[x] = vu[x] = make_uint4(0, 0, 0, 0);
-      if (i < to && in) {
-        const uint64_t key = static_cast<uint64_t>(range.key(i));
-        ku[x] = __ldg(reinterpret_cast<const uint4*>(kb + key * w.k.token));
-        vu[x] = __ldg(reinterpret_cast<const uint4*>(vb + key * w.v.token));
-      }
+      const int i = base + group + x * groups;
+      const bool there = i < to && in;
+      const uint64_t key = static_cast<uint64_t>(there ? range.key(i) : 0);
+      copy16(slot + x * kThreads, kb + key * w.k.token, there);
+      copy16(slot + (kKeys + x) * kThreads, vb + key * w.v.token, there);
     }
+    copies_commit();
   };
-  fetch(from + group);
+#pragma unroll
+  for (int n = 0; n < kStages - 1; ++n) fetch(from + n * step, n);
+  int stage = 0;
   for (int base = from; base < to; base += step) {
     float score[kKeys][RR];
+    copies_wait<kStages - 2>();
+    const uint4* slot = ring + stage * 2 * kKeys * kThreads;
 #pragma unroll
     for (int x = 0; x < kKeys; ++x) {
       float k[V];
-      unpack<T>(ku[x], k);
+      unpack<T>(slot[x * kThreads], k);
 #pragma unroll
       for (int r = 0; r < RR; ++r) {
         score[x][r] = 0.f;
@@ -226,11 +244,8 @@ __global__ void __launch_bounds__(kThreads) window_decode_kernel(
 #pragma unroll
         for (int r = 0; r < RR; ++r) score[x][r] += __shfl_xor_sync(0xffffffffu, score[x][r], o);
     }
-    uint4 held[kKeys];
-#pragma unroll
-    for (int x = 0; x < kKeys; ++x) held[x] = vu[x];
+    fetch(base + (kStages - 1) * step, (stage + kStages - 1) % kStages);
     const int at = base + group;
-    fetch(at + step);
 #pragma unroll
     for (int x = 0; x < kKeys; ++x) {
       const int i = at + x * groups;
@@ -259,13 +274,16 @@ __global__ void __launch_bounds__(kThreads) window_decode_kernel(
 #pragma unroll
     for (int x = 0; x < kKeys; ++x) {
       float v[V];
-      unpack<T>(held[x], v);
+      unpack<T>(slot[(kKeys + x) * kThreads], v);
 #pragma unroll
       for (int r = 0; r < RR; ++r)
 #pragma unroll
         for (int e = 0; e < V; ++e) acc[r][e] = fmaf(score[x][r], v[e], acc[r][e]);
     }
+    stage = (stage + 1) % kStages;
   }
+  copies_wait<0>();
+  __syncthreads();  // the ring's memory is reused
 
   // shared: [group][row][head_dim + 2]
   const int stride = w.head_dim + 2;
@@ -321,7 +339,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 
 // DB: blocks of 32 elements of a head; RB: blocks of 8 rows (1 or 2).
 template <int DB, int RB>
-__global__ void __launch_bounds__(kThreads, RB == 1 ? 3 : 2) window_decode_mma_kernel(
+__global__ void __launch_bounds__(kThreads) window_decode_mma_kernel(
     const __grid_constant__ DecodeParams p) {
   pdl_begin();
   using T = __nv_bfloat16;
@@ -364,35 +382,35 @@ __global__ void __launch_bounds__(kThreads, RB == 1 ? 3 : 2) window_decode_mma_k
 
   const T* kb = row_ptr<T>(w.k, b, 0, kh) + t * 8;
   const T* vb = row_ptr<T>(w.v, b, 0, kh) + g * 8;
-  uint4 ku[2][DB], vu[VB][4];
-  auto fetch_keys = [&](int base) {  // keys base + g, base + 8 + g
+  constexpr int kSlots = 2 * DB + 4 * VB;
+  uint4* ring = reinterpret_cast<uint4*>(shared) + threadIdx.x;  // [stage][slot]
+  auto fetch = [&](int base, int stage) {
+    uint4* slot = ring + stage * kSlots * kThreads;
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
+    for (int x = 0; x < 2; ++x) {  // keys base + g, base + 8 + g
       const int i = base + 8 * x + g;
       const T* src = kb + static_cast<uint64_t>(i < to ? range.key(i) : 0) * w.k.token;
 #pragma unroll
-      for (int d = 0; d < DB; ++d)
-        ku[x][d] = i < to ? __ldg(reinterpret_cast<const uint4*>(src + d * 32)) : make_uint4(0, 0, 0, 0);
+      for (int d = 0; d < DB; ++d) copy16(slot + (x * DB + d) * kThreads, src + d * 32, i < to);
     }
-  };
-  auto fetch_values = [&](int base) {  // keys base + 2t, + 1, + 8, + 9
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
+    for (int x = 0; x < 4; ++x) {  // keys base + 2t, + 1, + 8, + 9
       const int i = base + 2 * t + (x & 1) + (x >> 1) * 8;
       const T* src = vb + static_cast<uint64_t>(i < to ? range.key(i) : 0) * w.v.token;
 #pragma unroll
-      for (int d = 0; d < VB; ++d)
-        vu[d][x] = i < to && (DB % 2 == 0 || d * 64 + g * 8 < DB * 32)
-                       ? __ldg(reinterpret_cast<const uint4*>(src + d * 64))
-                       : make_uint4(0, 0, 0, 0);
+      for (int d = 0; d < VB; ++d) {
+        const bool there = i < to && (DB % 2 == 0 || d * 64 + g * 8 < DB * 32);
+        copy16(slot + (2 * DB + x * VB + d) * kThreads, there ? src + d * 64 : vb, there);
+      }
     }
+    copies_commit();
   };
-  int base = from + warp * 16;
-  if (base < to) {
-    fetch_keys(base);
-    fetch_values(base);
-  }
+  int base = from + warp * 16, stage = 0;
+#pragma unroll
+  for (int n = 0; n < kStages - 1; ++n) fetch(base + n * kStep, n);
   for (; base < to; base += kStep) {
+    copies_wait<kStages - 2>();
+    const uint4* slot = ring + stage * kSlots * kThreads;
     float sc[2][2 * RB];  // [8 keys][row g: keys 2t, 2t + 1; row g + 8: the same]
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
@@ -404,11 +422,12 @@ __global__ void __launch_bounds__(kThreads, RB == 1 ? 3 : 2) window_decode_mma_k
                                 RB > 1 ? q[d][0][RB - 1][1] : 0};
         const uint32_t a1[4] = {q[d][1][0][0], RB > 1 ? q[d][1][RB - 1][0] : 0, q[d][1][0][1],
                                 RB > 1 ? q[d][1][RB - 1][1] : 0};
-        mma_rows<RB>(sc[x], a0, ku[x][d].x, ku[x][d].y);
-        mma_rows<RB>(sc[x], a1, ku[x][d].z, ku[x][d].w);
+        const uint4 k = slot[(x * DB + d) * kThreads];
+        mma_rows<RB>(sc[x], a0, k.x, k.y);
+        mma_rows<RB>(sc[x], a1, k.z, k.w);
       }
     }
-    if (base + kStep < to) fetch_keys(base + kStep);
+    fetch(base + (kStages - 1) * kStep, (stage + kStages - 1) % kStages);
     // Keys of this thread's columns; the whole tile inside every row's window is the usual case.
     const int at = base + 2 * t;
     uint32_t hi[4] = {0, 0, 0, 0}, lo[4] = {0, 0, 0, 0};
@@ -456,20 +475,25 @@ __global__ void __launch_bounds__(kThreads, RB == 1 ? 3 : 2) window_decode_mma_k
     }
 #pragma unroll
     for (int d = 0; d < VB; ++d) {
+      uint32_t v[4][4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const uint4 u = slot[(2 * DB + x * VB + d) * kThreads];
+        v[x][0] = u.x, v[x][1] = u.y, v[x][2] = u.z, v[x][3] = u.w;
+      }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t a = reinterpret_cast<const uint32_t(&)[4]>(vu[d][0])[j / 2],
-                       c = reinterpret_cast<const uint32_t(&)[4]>(vu[d][1])[j / 2],
-                       e = reinterpret_cast<const uint32_t(&)[4]>(vu[d][2])[j / 2],
-                       f = reinterpret_cast<const uint32_t(&)[4]>(vu[d][3])[j / 2];
+        const uint32_t a = v[0][j / 2], c = v[1][j / 2], e = v[2][j / 2], f = v[3][j / 2];
         const uint32_t pick = j & 1 ? 0x7632 : 0x5410;
         const uint32_t b0 = __byte_perm(a, c, pick), b1 = __byte_perm(e, f, pick);
         mma_rows<RB>(acc[d][j], lo, b0, b1);
         mma_rows<RB>(acc[d][j], hi, b0, b1);
       }
     }
-    if (base + kStep < to) fetch_values(base + kStep);
+    stage = (stage + 1) % kStages;
   }
+  copies_wait<0>();
+  __syncthreads();  // the ring's memory is reused
   // A row's sum is spread over the four threads of its group; each has the row's maximum.
   // shared: [warp][row][head_dim + 2]
   const int stride = w.head_dim + 2;
@@ -539,14 +563,25 @@ DecodePlan decode_plan(const WindowParams& w, int device) {
   d.lanes_log2 = 0;
   while ((1 << d.lanes_log2) * vec < w.head_dim) ++d.lanes_log2;
   d.groups = d.mma ? kThreads / 32 : kThreads >> d.lanes_log2;
-  d.smem = (static_cast<size_t>(d.groups) * d.rr * (w.head_dim + 2) + d.rr * (d.groups + 2)) * sizeof(float);
-  // As many ranges as give every SM four CTAs, none of less than two steps' keys. Up to eight are
-  // joined inside a cluster.
+  const int blocks = w.head_dim / 32;
+  const size_t ring = static_cast<size_t>(kStages) * kThreads * 16 *
+                      (d.mma ? 2 * blocks + 4 * ((blocks + 1) / 2) : 2 * kKeys);
+  d.smem = std::max(ring, (static_cast<size_t>(d.groups) * d.rr * (w.head_dim + 2) + d.rr * (d.groups + 2)) *
+                              sizeof(float));
+  // Ranges so that the CTAs fill whole rounds of the machine: rounds x (keys of a range + what a
+  // CTA's start and join cost, about 96 keys' time) at its least, none with less than two steps' keys.
+  // Up to eight are joined inside a cluster.
   const int step = d.mma ? kThreads / 32 * 16 : d.groups * kKeys;
   const int64_t keys = std::min<int64_t>(w.kv_len, static_cast<int64_t>(w.window) + w.q_len + w.sinks);
   const int64_t ctas = static_cast<int64_t>(w.batch) * w.kv_heads * d.row_blocks;
-  const int64_t fill = (4 * sm_count(device) + ctas - 1) / ctas;
-  d.splits = static_cast<int>(std::max<int64_t>(1, std::min(fill, keys / (2 * step))));
+  const int64_t slots = sm_count(device) * std::min<int64_t>(3, (227 << 10) / (d.smem + 1024));
+  const int64_t most = std::max<int64_t>(1, std::min((4 * slots + ctas - 1) / ctas, keys / (2 * step)));
+  int64_t best = INT64_MAX;
+  d.splits = 1;
+  for (int64_t n = 1; n <= most; ++n) {
+    const int64_t cost = (ctas * n + slots - 1) / slots * ((keys + n - 1) / n + 96);
+    if (cost < best) best = cost, d.splits = static_cast<int>(n);
+  }
   return d;
 }
 
