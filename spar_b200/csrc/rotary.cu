@@ -120,11 +120,13 @@ struct Slot {
   bool has_a, has_b, turns;
 };
 
-template <int VEC, bool HALF>
+// FULL: the whole head turns and every lane of the group has a slot, the usual case, which then
+// carries none of the tests.
+template <int VEC, bool HALF, bool FULL>
 __device__ __forceinline__ Slot slot_of(const RotaryParams& p, uint32_t s) {
   Slot o;
-  o.has_a = s < p.slots;
-  o.turns = s < p.rotating;
+  o.has_a = FULL || s < p.slots;
+  o.turns = FULL || s < p.rotating;
   if (o.turns) {
     if (HALF || VEC > 1) {  // vectors s and s + half of the rotated part
       o.a = s * VEC;
@@ -230,8 +232,10 @@ __device__ __forceinline__ float group_sum(float v, uint32_t lanes) {
 // One lane group per (token, HP heads of queries or of keys): the heads of a chunk share the
 // token's angles in registers and put 2 HP vectors in flight per lane before the first is used.
 // U slots per lane (one but for unaligned rows).
-template <typename T, int VEC, int U, int HP, bool HALF, bool NORM>
-__global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryParams p) {
+// (Four blocks an SM where two heads of a group still leave the registers: 116 -> 108 us for the
+// gradients of 3 x 8191 tokens of 40 heads of 128 bf16, half of each turned.)
+template <typename T, int VEC, int U, int HP, bool HALF, bool NORM, bool FULL>
+__global__ void __launch_bounds__(256, HP == 2 ? 4 : 1) rotary_kernel(const __grid_constant__ RotaryParams p) {
   pdl_begin();
   const uint32_t lanes = 1u << p.lanes_log2;
   const uint32_t l = threadIdx.x & (lanes - 1);
@@ -252,13 +256,12 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
                  h0 * in.head;
   T* dst = reinterpret_cast<T*>(out.data) + b * out.batch + in_seq * out.token + h0 * out.head;
   uint64_t row = 0;
-  const bool good = row_of(p, t, in_seq, row);
-  if (!good && live && l == 0 && chunk == 0 && p.invalid) atomicExch(p.invalid, 1);
+  const bool good = row_of(p, t, in_seq, row);  // under way; not looked at before the heads are too
 
   Raw<T, VEC> ra[U][HP], rb[U][HP];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const Slot s = slot_of<VEC, HALF>(p, l + u * lanes);
+    const Slot s = slot_of<VEC, HALF, FULL>(p, l + u * lanes);
 #pragma unroll
     for (int h = 0; h < HP; ++h) {
       if (static_cast<uint32_t>(h) < n && s.has_a) {
@@ -267,6 +270,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
       }
     }
   }
+  if (!good && live && l == 0 && chunk == 0 && p.invalid) atomicExch(p.invalid, 1);
   float r[HP];
   if constexpr (NORM) {
 #pragma unroll
@@ -274,7 +278,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
       float ss = 0.f;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const Slot s = slot_of<VEC, HALF>(p, l + u * lanes);
+        const Slot s = slot_of<VEC, HALF, FULL>(p, l + u * lanes);
         if (static_cast<uint32_t>(h) < n && s.has_a) {
 #pragma unroll
           for (int x = 0; x < VEC; ++x) {
@@ -290,12 +294,12 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
           }
         }
       }
-      r[h] = 1.0f / sqrtf(group_sum(ss, lanes) * p.inv_dim + p.eps);
+      r[h] = rsqrtf(group_sum(ss, lanes) * p.inv_dim + p.eps);  // within two steps of fp32
     }
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const Slot s = slot_of<VEC, HALF>(p, l + u * lanes);
+    const Slot s = slot_of<VEC, HALF, FULL>(p, l + u * lanes);
     if (!s.has_a || !n) continue;
     float2 cs[VEC];
     float wa[VEC], wb[VEC];
@@ -327,47 +331,11 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
 }
 
 // Backward of the norm and the rotation. Blocks are split between queries and keys in proportion
-// to their heads and walk their (token, head) units with the grid's stride, so a lane keeps the
+// to their heads and walk their (token, HB heads) units with the grid's stride, so a lane keeps the
 // sums of its slots' weight gradients in registers for the whole launch; a block adds its lane
-// groups' sums in a fixed order and leaves one partial row of head_dim floats. The next unit's x and
-// dy are under way while one is worked on: loaded on arrival the launch ran at half the bandwidth
-// (77 us for 2 x 4095 tokens of 40 heads of 128 bf16).
-template <typename T, int VEC, int U>
-struct Unit {
-  Raw<T, VEC> xa[U], xb[U], ga[U], gb[U];
-  uint64_t row, out;
-  bool live, good;
-};
-
-template <typename T, int VEC, int U, bool HALF>
-__device__ __forceinline__ void load_unit(const RotaryParams& p, int side, uint64_t unit, uint64_t units,
-                                          uint32_t l, uint32_t lanes, Unit<T, VEC, U>& v) {
-  const View &in = p.in[side], &out = p.out[side], &grad = p.grad[side];
-  const uint32_t heads = p.heads[side];
-  v.live = unit < units;
-  const uint32_t t = v.live ? p.by_heads[side].quotient(static_cast<uint32_t>(unit)) : 0;
-  const uint32_t h = v.live ? static_cast<uint32_t>(unit) - t * heads : 0;
-  const uint32_t b = p.by_seq.quotient(t), in_seq = t - b * p.seq;
-  v.good = row_of(p, t, in_seq, v.row);
-  if (!v.good && v.live && l == 0 && h == 0 && p.invalid) atomicExch(p.invalid, 1);
-  v.out = b * out.batch + in_seq * out.token + h * out.head;
-  const T* px = reinterpret_cast<const T*>(in.data) + b * in.batch + in_seq * in.token + h * in.head;
-  const T* pg = reinterpret_cast<const T*>(grad.data) + b * grad.batch + in_seq * grad.token + h * grad.head;
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const Slot s = slot_of<VEC, HALF>(p, l + u * lanes);
-    v.xa[u] = v.xb[u] = v.ga[u] = v.gb[u] = Raw<T, VEC>{};
-    if (!v.live || !v.good || !s.has_a) continue;
-    v.xa[u] = load_raw<T, VEC>(px + s.a);
-    v.ga[u] = load_raw<T, VEC>(pg + s.a);
-    if (s.has_b) {
-      v.xb[u] = load_raw<T, VEC>(px + s.b);
-      v.gb[u] = load_raw<T, VEC>(pg + s.b);
-    }
-  }
-}
-
-template <typename T, int VEC, int U, bool HALF>
+// groups' sums in a fixed order and leaves one partial row of head_dim floats. The heads of a unit
+// share the token's angles and addresses, and put 4 HB vectors in flight per lane.
+template <typename T, int VEC, int U, int HB, bool HALF, bool FULL>
 __global__ void __launch_bounds__(kBackwardThreads) qk_norm_rotary_backward_kernel(
     const __grid_constant__ RotaryParams p) {
   pdl_begin();
@@ -378,76 +346,108 @@ __global__ void __launch_bounds__(kBackwardThreads) qk_norm_rotary_backward_kern
   const int side = blockIdx.x >= p.blocks_q;
   const uint32_t block = side ? blockIdx.x - p.blocks_q : blockIdx.x;
   const uint32_t blocks = side ? gridDim.x - p.blocks_q : p.blocks_q;
-  const uint64_t units = static_cast<uint64_t>(p.tokens) * p.heads[side];
-  float da[U][VEC], db[U][VEC];
+  const uint32_t heads = p.heads[side], chunks = p.chunks[side];
+  const uint64_t units = static_cast<uint64_t>(p.tokens) * chunks;
+  const View &in = p.in[side], &out = p.out[side], &grad = p.grad[side];
+  float wa[U][VEC], wb[U][VEC], da[U][VEC], db[U][VEC];
 #pragma unroll
-  for (int u = 0; u < U; ++u)
+  for (int u = 0; u < U; ++u) {
+    load_weights<VEC>(p.weight[side], slot_of<VEC, HALF, FULL>(p, l + u * lanes), wa[u], wb[u]);
 #pragma unroll
     for (int x = 0; x < VEC; ++x) da[u][x] = db[u][x] = 0.f;
-  T* out = reinterpret_cast<T*>(p.out[side].data);
-  const uint64_t stride = static_cast<uint64_t>(blocks) * groups;
-  Unit<T, VEC, U> cur, next;
-  uint64_t first = static_cast<uint64_t>(block) * groups;
-  if (first < units) load_unit<T, VEC, U, HALF>(p, side, first + group, units, l, lanes, cur);
-  for (; first < units; first += stride) {  // every lane: the sums are whole-warp
+  }
+  for (uint64_t first = static_cast<uint64_t>(block) * groups; first < units;
+       first += static_cast<uint64_t>(blocks) * groups) {  // every lane: the sums are whole-warp
+    const uint64_t unit = first + group;
+    const bool live = unit < units;
+    const uint32_t t = live ? p.by_heads[side].quotient(static_cast<uint32_t>(unit)) : 0;
+    const uint32_t h0 = live ? (static_cast<uint32_t>(unit) - t * chunks) * HB : 0;
+    const uint32_t n = live ? min(static_cast<uint32_t>(HB), heads - h0) : 0;
+    const uint32_t b = p.by_seq.quotient(t), in_seq = t - b * p.seq;
+    uint64_t row = 0;
+    const bool good = row_of(p, t, in_seq, row);
+    const T* px = reinterpret_cast<const T*>(in.data) + b * in.batch + in_seq * in.token + h0 * in.head;
+    const T* pg =
+        reinterpret_cast<const T*>(grad.data) + b * grad.batch + in_seq * grad.token + h0 * grad.head;
+    T* po = reinterpret_cast<T*>(out.data) + b * out.batch + in_seq * out.token + h0 * out.head;
+    Raw<T, VEC> rxa[HB][U], rxb[HB][U], rga[HB][U], rgb[HB][U];
+#pragma unroll
+    for (int h = 0; h < HB; ++h)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const Slot s = slot_of<VEC, HALF, FULL>(p, l + u * lanes);
+        rxa[h][u] = rxb[h][u] = rga[h][u] = rgb[h][u] = Raw<T, VEC>{};
+        if (static_cast<uint32_t>(h) >= n || !s.has_a) continue;
+        rxa[h][u] = load_raw<T, VEC>(px + h * in.head + s.a);
+        rga[h][u] = load_raw<T, VEC>(pg + h * grad.head + s.a);
+        if (s.has_b) {
+          rxb[h][u] = load_raw<T, VEC>(px + h * in.head + s.b);
+          rgb[h][u] = load_raw<T, VEC>(pg + h * grad.head + s.b);
+        }
+      }
+    if (!good && live && l == 0 && h0 == 0 && p.invalid) atomicExch(p.invalid, 1);
     float2 cs[U][VEC];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const Slot s = slot_of<VEC, HALF>(p, l + u * lanes);
-      if (s.turns && cur.good) load_angles<VEC, HALF>(p, s, cur.row, cs[u]);
+      const Slot s = slot_of<VEC, HALF, FULL>(p, l + u * lanes);
+      if (s.turns) load_angles<VEC, HALF>(p, s, good ? row : 0, cs[u]);
     }
-    if (first + stride < units)
-      load_unit<T, VEC, U, HALF>(p, side, first + stride + group, units, l, lanes, next);
-    float xa[U][VEC], xb[U][VEC], ga[U][VEC], gb[U][VEC];
-    float ss = 0.f, dot = 0.f;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const Slot s = slot_of<VEC, HALF>(p, l + u * lanes);
-      float wa[VEC], wb[VEC];
-      load_weights<VEC>(p.weight[side], s, wa, wb);  // cached; held for the launch they cost occupancy
-      widen<T, VEC>(cur.xa[u], xa[u]);
-      widen<T, VEC>(cur.xb[u], xb[u]);
-      widen<T, VEC>(cur.ga[u], ga[u]);
-      widen<T, VEC>(cur.gb[u], gb[u]);
-      if (s.turns && cur.good) turn<VEC, HALF>(ga[u], gb[u], cs[u], -1.f);
-#pragma unroll
-      for (int x = 0; x < VEC; ++x) {
-        ss += xa[u][x] * xa[u][x] + xb[u][x] * xb[u][x];
-        dot += ga[u][x] * wa[x] * xa[u][x] + gb[u][x] * wb[x] * xb[u][x];
-      }
-    }
-    for (uint32_t o = lanes >> 1; o > 0; o >>= 1) {
-      ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      dot += __shfl_xor_sync(0xffffffffu, dot, o);
-    }
-    const float r = 1.0f / sqrtf(ss * p.inv_dim + p.eps);
-    const float m = dot * r * p.inv_dim;  // mean(g w x r)
-    if (cur.live) {
+    for (int h = 0; h < HB; ++h) {
+      float xa[U][VEC], xb[U][VEC], ga[U][VEC], gb[U][VEC];
+      float ss = 0.f, dot = 0.f;
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const Slot s = slot_of<VEC, HALF>(p, l + u * lanes);
+        const Slot s = slot_of<VEC, HALF, FULL>(p, l + u * lanes);
+        widen<T, VEC>(rxa[h][u], xa[u]);
+        widen<T, VEC>(rxb[h][u], xb[u]);
+        widen<T, VEC>(rga[h][u], ga[u]);
+        widen<T, VEC>(rgb[h][u], gb[u]);
+        if (s.turns) turn<VEC, HALF>(ga[u], gb[u], cs[u], -1.f);  // (unused where the position is not good)
+#pragma unroll
+        for (int x = 0; x < VEC; ++x) {
+          ss += xa[u][x] * xa[u][x] + xb[u][x] * xb[u][x];
+          dot += ga[u][x] * wa[u][x] * xa[u][x] + gb[u][x] * wb[u][x] * xb[u][x];
+        }
+      }
+      for (uint32_t o = lanes >> 1; o > 0; o >>= 1) {
+        ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        dot += __shfl_xor_sync(0xffffffffu, dot, o);
+      }
+      const float r = rsqrtf(ss * p.inv_dim + p.eps);  // within two steps of fp32
+      const float m = dot * r * p.inv_dim;             // mean(g w x r)
+      if (static_cast<uint32_t>(h) >= n) continue;
+      if (!good) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const Slot s = slot_of<VEC, HALF, FULL>(p, l + u * lanes);
+          const float zero[VEC] = {};
+          if (s.has_a) store_vec<T, VEC>(po + h * out.head + s.a, zero);
+          if (s.has_a && s.has_b) store_vec<T, VEC>(po + h * out.head + s.b, zero);
+        }
+        continue;
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const Slot s = slot_of<VEC, HALF, FULL>(p, l + u * lanes);
         if (!s.has_a) continue;
-        float wa[VEC], wb[VEC], oa[VEC], ob[VEC];
-        load_weights<VEC>(p.weight[side], s, wa, wb);
+        float oa[VEC], ob[VEC];
 #pragma unroll
         for (int x = 0; x < VEC; ++x) {
           const float ua = xa[u][x] * r, ub = xb[u][x] * r;
-          oa[x] = cur.good ? r * (ga[u][x] * wa[x] - ua * m) : 0.f;
-          ob[x] = cur.good ? r * (gb[u][x] * wb[x] - ub * m) : 0.f;
-          if (cur.good) {
-            da[u][x] += ga[u][x] * ua;
-            db[u][x] += gb[u][x] * ub;
-          }
+          oa[x] = r * (ga[u][x] * wa[u][x] - ua * m);
+          ob[x] = r * (gb[u][x] * wb[u][x] - ub * m);
+          da[u][x] += ga[u][x] * ua;
+          db[u][x] += gb[u][x] * ub;
         }
-        store_vec<T, VEC>(out + cur.out + s.a, oa);
-        if (s.has_b) store_vec<T, VEC>(out + cur.out + s.b, ob);
+        store_vec<T, VEC>(po + h * out.head + s.a, oa);
+        if (s.has_b) store_vec<T, VEC>(po + h * out.head + s.b, ob);
       }
     }
-    cur = next;
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const Slot s = slot_of<VEC, HALF>(p, l + u * lanes);
+    const Slot s = slot_of<VEC, HALF, FULL>(p, l + u * lanes);
     if (!s.has_a) continue;
 #pragma unroll
     for (int x = 0; x < VEC; ++x) {
@@ -531,7 +531,9 @@ View view_of(const SparB200Heads& v, uint64_t batch, uint64_t seq, uint64_t head
           heads > 1 ? v.head : 0};
 }
 
-constexpr int kBackwardBlocksPerSM = 4;  // as many of 128 threads as run at once (vectorised bf16)
+// More blocks than run at once, so that their ends do not fall together (2 x 4095 tokens of 40 heads of
+// 128 bf16: 4 an SM 76.5 us, 16 an SM 72.2 us).
+constexpr int kBackwardBlocksPerSM = 16;
 
 uint32_t backward_blocks(int device) {
   return static_cast<uint32_t>(sm_count(device)) * kBackwardBlocksPerSM;
@@ -602,29 +604,38 @@ bool make_params(const SparB200Rotary* r, bool norm, bool backward, RotaryParams
   p.eps = static_cast<float>(r->epsilon);
   p.inv_dim = 1.0f / static_cast<float>(r->head_dim);
   p.by_seq = Divider(p.seq ? p.seq : 1);
-  for (int s = 0; s < 2; ++s) p.by_heads[s] = Divider(p.heads[s] ? p.heads[s] : 1);
   p.partial = static_cast<float*>(r->scratch);
   return true;
 }
 
-template <typename T, int VEC, int U, int HP, bool HALF, bool NORM>
+bool full_head(const RotaryParams& p) {
+  return 2 * p.pairs == p.head_dim && p.slots == 1u << p.lanes_log2;
+}
+
+template <typename T, int VEC, int U, int HP, bool HALF, bool NORM, bool FULL = false>
 cudaError_t launch_rotary(RotaryParams& p, cudaStream_t stream) {
   for (int s = 0; s < 2; ++s) p.chunks[s] = (p.heads[s] + HP - 1) / HP;
   p.by_chunks = Divider(p.chunks[0] + p.chunks[1]);
   const uint64_t threads = (static_cast<uint64_t>(p.tokens) * (p.chunks[0] + p.chunks[1]))
                            << p.lanes_log2;
-  return launch(rotary_kernel<T, VEC, U, HP, HALF, NORM>,
+  return launch(rotary_kernel<T, VEC, U, HP, HALF, NORM, FULL>,
                 dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, stream, p);
 }
 
 template <typename T, int VEC, bool HALF, bool NORM>
 cudaError_t launch_forward(RotaryParams& p, bool vec, int device, cudaStream_t stream) {
   if (!vec) return launch_rotary<T, 1, 4, 1, HALF, NORM>(p, stream);
+  // heads of a lane group: as many as keep the registers for four blocks an SM (bf16 with norms: one
+  // head 23 us, two 29 us for 4 x 4096 tokens of 20 heads of 64; fp32: four 45 us, one 50 us)
+  constexpr int kHeads = VEC == 4 ? 4 : NORM ? 1 : 2;
   const uint64_t warps =
       (static_cast<uint64_t>(p.tokens) * (p.heads[0] + p.heads[1]) << p.lanes_log2) / 32;
-  if (warps >= static_cast<uint64_t>(sm_count(device)) * 64)
-    return launch_rotary<T, VEC, 1, VEC == 4 ? 4 : 2, HALF, NORM>(p, stream);
-  return launch_rotary<T, VEC, 1, 1, HALF, NORM>(p, stream);
+  const bool many = warps >= static_cast<uint64_t>(sm_count(device)) * 64;
+  if (full_head(p))
+    return many ? launch_rotary<T, VEC, 1, kHeads, HALF, NORM, true>(p, stream)
+                : launch_rotary<T, VEC, 1, 1, HALF, NORM, true>(p, stream);
+  return many ? launch_rotary<T, VEC, 1, kHeads, HALF, NORM>(p, stream)
+              : launch_rotary<T, VEC, 1, 1, HALF, NORM>(p, stream);
 }
 
 template <bool NORM>
@@ -648,11 +659,16 @@ SparCudaStatus run_forward(const SparB200Rotary* r, int device, void* stream) {
   return e == cudaSuccess ? launch_status() : runtime(e);
 }
 
-template <typename T, int VEC, int U, bool HALF>
-cudaError_t launch_backward(RotaryParams& p, int device, cudaStream_t stream, uint32_t& grid) {
+template <typename T, int VEC, int U, bool HALF, bool FULL>
+cudaError_t launch_backward_as(RotaryParams& p, int device, cudaStream_t stream, uint32_t& grid) {
+  constexpr int HB = VEC == 4 ? 2 : 1;
   const uint32_t groups = kBackwardThreads >> p.lanes_log2;
-  const uint64_t need[2] = {(static_cast<uint64_t>(p.tokens) * p.heads[0] + groups - 1) / groups,
-                            (static_cast<uint64_t>(p.tokens) * p.heads[1] + groups - 1) / groups};
+  uint64_t need[2];
+  for (int s = 0; s < 2; ++s) {
+    p.chunks[s] = (p.heads[s] + HB - 1) / HB;
+    p.by_heads[s] = Divider(p.chunks[s] ? p.chunks[s] : 1);
+    need[s] = (static_cast<uint64_t>(p.tokens) * p.chunks[s] + groups - 1) / groups;
+  }
   const uint32_t most = backward_blocks(device);
   uint64_t nq = need[0], nk = need[1];
   if (nq + nk > most) {  // in proportion to the heads, at least one each
@@ -663,8 +679,15 @@ cudaError_t launch_backward(RotaryParams& p, int device, cudaStream_t stream, ui
   }
   p.blocks_q = static_cast<uint32_t>(nq);
   grid = static_cast<uint32_t>(nq + nk);
-  return launch(qk_norm_rotary_backward_kernel<T, VEC, U, HALF>, dim3(grid), dim3(kBackwardThreads),
+  return launch(qk_norm_rotary_backward_kernel<T, VEC, U, HB, HALF, FULL>, dim3(grid), dim3(kBackwardThreads),
                 groups * p.head_dim * sizeof(float), stream, p);
+}
+
+template <typename T, int VEC, int U, bool HALF>
+cudaError_t launch_backward(RotaryParams& p, int device, cudaStream_t stream, uint32_t& grid) {
+  if (VEC > 1 && full_head(p))
+    return launch_backward_as<T, VEC, U, HALF, (VEC > 1)>(p, device, stream, grid);
+  return launch_backward_as<T, VEC, U, HALF, false>(p, device, stream, grid);
 }
 
 }  // namespace

@@ -3,7 +3,7 @@
 //
 // The floor is one read of the visible keys and values, which all query heads of a key head share:
 // a CTA takes up to 8 or 16 rows (heads of one group, times tokens) and a range of the visible keys,
-// so that a cache row is loaded once for all of them: by cp.async, three steps ahead (one step ahead
+// so that a cache row is loaded once for all of them: by cp.async, two steps ahead (one step ahead
 // in registers every step waited for memory: 4 TB/s), each lane into slots of shared memory that it
 // alone reads, so nothing but its own copies is waited for. Each warp (or lane group) keeps its own running maximum,
 // sum and output; they are joined in shared memory, and the ranges of one row over the shared
@@ -31,7 +31,7 @@ namespace {
 
 constexpr int kThreads = 128;
 constexpr int kKeys = 4;    // rows of the cache that a lane group takes at once
-constexpr int kStages = 4;  // steps of the ring (three under way, about 100 KB an SM)
+constexpr int kStages = 3;  // steps of the ring, two of them under way (96 KB an SM at head_dim 128)
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 

@@ -269,14 +269,14 @@ struct Item {
 };
 
 // Fills in the keys of an item whose heads and rows are set.
-template <int QT, int BN>
+template <int QT, int BN, int TILE = 128>
 __device__ __forceinline__ void place_keys(const WindowParams& w, Item& it) {
   it.kh = it.h[0] / w.group;
   it.s = sequence_of(w, it.b);
   int lo[2], hi[2], ulo = INT_MAX, uhi = -1;
 #pragma unroll
   for (int x = 0; x < QT; ++x) {
-    const int rows = min(128, w.q_len - it.row[x]);
+    const int rows = min(TILE, w.q_len - it.row[x]);
     const int pa = max(it.s.p0 + it.row[x], 0), pb = min(it.s.p0 + it.row[x] + rows - 1, it.s.n - 1);
     it.any[x] = rows > 0 && pb >= pa;
     lo[x] = max(0, pa - w.window + 1);
@@ -323,15 +323,15 @@ __device__ __forceinline__ Item item_of(const TcParams& p, int idx) {
   return it;
 }
 // The item of one query tile: the last rows first (they see the most keys).
-template <int BN>
+template <int BN, int TILE>
 __device__ __forceinline__ Item item_of_tile(const WindowParams& w, int idx) {
-  const int per = w.batch * w.heads, t = (w.q_len + 127) / 128 - 1 - idx / per;
+  const int per = w.batch * w.heads, t = (w.q_len + TILE - 1) / TILE - 1 - idx / per;
   const int bh = idx % per;
   Item it;
   it.b = bh / w.heads;
   it.h[0] = bh - it.b * w.heads;
-  it.row[0] = t * 128;
-  place_keys<1, BN>(w, it);
+  it.row[0] = t * TILE;
+  place_keys<1, BN, TILE>(w, it);
   return it;
 }
 // The next tile of query tile x from j on, or n.
@@ -778,7 +778,8 @@ struct BackwardParams {
   // keys: the first `first_tiles` key tiles are cut into `chunks` row ranges, every tile into
   // `head_parts` groups of query heads.
   int first_tiles, chunks, chunk, head_parts;
-  float* partial;  // [part][2][128][head_dim]: dk, dv
+  int tile;        // stationary rows of a tile
+  float* partial;  // [part][2][tile][head_dim]: dk, dv
 };
 
 // Which part of the key side an item is: batch, key head, tile, rows, heads; `slot`: its partial,
@@ -813,12 +814,12 @@ __device__ __forceinline__ KeyItem key_item(const BackwardParams& p, int idx) {
   }
   it.b = which / w.kv_heads;
   it.kh = which - it.b * w.kv_heads;
-  it.key = tile * 128;
+  it.key = tile * p.tile;
   it.s = sequence_of(w, it.b);
   it.head = it.kh * w.group + w.group * part / p.head_parts;
   it.heads = it.kh * w.group + w.group * (part + 1) / p.head_parts - it.head;
   // rows that see a key of the tile: positions key .. last key + window - 1 (first tokens: n - 1)
-  const int last_key = min(it.key + 127, it.s.n - 1);
+  const int last_key = min(it.key + p.tile - 1, it.s.n - 1);
   const int far = it.key < w.sinks ? it.s.n - 1 : min(it.s.n - 1, last_key + w.window - 1);
   it.row = max(from, it.key - it.s.p0);
   it.end = min(to, far - it.s.p0 + 1);
@@ -827,14 +828,19 @@ __device__ __forceinline__ KeyItem key_item(const BackwardParams& p, int idx) {
   return it;
 }
 
-template <bool KEYS, int DH, int NP, int ST>
+// OUT: which sums of the key side a launch makes (0 both, 1 dk, 2 dv).
+template <bool KEYS, int DH, int NP, int ST, int OUT>
 struct Bwd {
   // Buffers of S and dP: three where TMEM has room, so that the two softmax groups find their next
   // scores ready; not more than stages, as scores run that far ahead of the last use of a stage.
-  static constexpr int kBuffers = NP > 1 ? (KEYS ? 1 : 2) : KEYS && DH == 128 ? 2 : 3;
+  static constexpr int kBuffers = NP > 1 ? (KEYS || ST == 1 ? 1 : 2) : KEYS && DH == 128 ? 2 : 3;
   static_assert(kBuffers <= ST, "stages");
   static constexpr uint32_t kStats = NP == 1 && DH == 64 ? 2 : 1;  // pairs of stationary operands
-  static constexpr uint32_t kStat = NP * DH * 256;            // one stationary operand
+  // Stationary rows. Three planes of two operands of 128 columns leave room for 64 of the 128 rows of a
+  // product: its other rows read whatever follows in shared memory, give results that nobody reads,
+  // and multiply P and dS of zero.
+  static constexpr int kTile = NP > 1 && DH == 128 ? 64 : 128;
+  static constexpr uint32_t kStat = NP * DH * kTile * 2;      // one stationary operand
   static constexpr uint32_t kMov = NP * DH * kMoving * 2;     // one moving operand
   static constexpr uint32_t kA = 0;
   static constexpr uint32_t kB = kA + kStats * 2 * kStat;
@@ -848,7 +854,7 @@ struct Bwd {
   // (NP = 3) the sums of earlier tiles.
   static constexpr uint32_t kBuf = KEYS && NP > 1 ? 192 : 128;
   static constexpr uint32_t kAcc = kBuffers * kBuf;
-  static constexpr uint32_t kOuts = KEYS ? 2 : 1;
+  static constexpr uint32_t kOuts = KEYS && OUT == 0 ? 2 : 1;
   static constexpr uint32_t kSum = kAcc + kOuts * DH;
   static_assert(kAcc + kOuts * DH * (NP > 1 ? 2 : 1) <= kTmemCols, "backward TMEM");
 };
@@ -864,10 +870,10 @@ __host__ __device__ constexpr uint32_t operand_col(int which, int pl, int ks) {
   return KEYS ? 128 + which * 32 + g * 16 + sub : 64 + g * 32 + sub;
 }
 
-template <bool KEYS, int DH, int NP, int ST>
+template <bool KEYS, int DH, int NP, int ST, int OUT>
 __global__ void __launch_bounds__(384, 1) window_backward_kernel(
     const __grid_constant__ BackwardParams p) {
-  using L = Bwd<KEYS, DH, NP, ST>;
+  using L = Bwd<KEYS, DH, NP, ST, OUT>;
   constexpr int kBoxes = DH / 64;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = align1024(smem_raw);
@@ -921,7 +927,7 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
       k = key_item(p, idx);
       return k.jobs_per_head * k.heads;
     } else {
-      q = item_of_tile<kMoving>(w, idx);
+      q = item_of_tile<kMoving, L::kTile>(w, idx);
       return q.n;
     }
   };
@@ -952,7 +958,7 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
           tc::mbar_arrive_expect_tx(a_full + as, 2 * L::kStat);
           for (int pl = 0; pl < NP; ++pl)
             for (int c = 0; c < kBoxes; ++c) {
-              uint8_t* dst = smem + L::kA + as * 2 * L::kStat + (pl * kBoxes + c) * 16384;
+              uint8_t* dst = smem + L::kA + as * 2 * L::kStat + (pl * kBoxes + c) * L::kTile * 128;
               const int row = KEYS ? k.key : q.row[0], h = KEYS ? k.kh : q.h[0];
               tc::tma_load_5d(dst, &p.s1, a_full + as, 64 * c, row, h, b, pl);
               tc::tma_load_5d(dst + L::kStat, &p.s2, a_full + as, 64 * c, row, h, b, pl);
@@ -1013,7 +1019,7 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
           if (!wait_or_abort(m_full + st, m / ST, abort_flag)) return false;
           tc::tc_fence_after();
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
+          for (int half = 0; half < (OUT == 2 ? 1 : 2); ++half) {
             const uint32_t a = kmajor_low(a_addr + (2 * (an % L::kStats) + half) * L::kStat),
                            b = kmajor_low(b_addr + (2 * st + half) * L::kMov);
             uint32_t acc = 0;
@@ -1022,7 +1028,7 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
 #pragma unroll
               for (int ks = 0; ks < DH / 16; ++ks)
                 if (ks < p.ksteps) {
-                  tc::mma_f16(buf + half * 64, desc(a + kmajor_step(128, plane_a<NP>(pr), kBoxes, ks)),
+                  tc::mma_f16(buf + half * 64, desc(a + kmajor_step(L::kTile, plane_a<NP>(pr), kBoxes, ks)),
                               desc(b + kmajor_step(kMoving, plane_b<NP>(pr), kBoxes, ks)), idesc_s, acc);
                   acc = 1;
                 }
@@ -1050,9 +1056,9 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
 #pragma unroll
             for (int out = 0; out < static_cast<int>(L::kOuts); ++out) {
               // queries: dq += dS k; keys: dk += dS^T q, dv += P^T dout
-              const int which = KEYS ? 1 - out : 0;
-              const uint32_t b = mnmajor_low(b_addr + (2 * st + out) * L::kMov, kMoving);
-              uint32_t acc = NP == 1 && i > 0;
+              const int operand = OUT == 2 ? 1 : out, which = KEYS ? 1 - operand : 0;
+              const uint32_t b = mnmajor_low(b_addr + (2 * st + operand) * L::kMov, kMoving);
+            uint32_t acc = NP == 1 && i > 0;
 #pragma unroll
               for (int pr = 0; pr < kProducts<NP>; ++pr)
 #pragma unroll
@@ -1117,8 +1123,10 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
       const int row = (KEYS ? k.key : q.row[0]) + r;
       const int pos = KEYS ? row : s.p0 + row;
       const int first_pos = pos - lane;  // of this warp
-      const bool valid = KEYS ? row < s.n : row < w.q_len && pos >= 0 && pos < s.n;
-      const bool rows_in = KEYS ? first_pos + 31 < s.n
+      const bool valid =
+          r < L::kTile && (KEYS ? row < s.n : row < w.q_len && pos >= 0 && pos < s.n);
+      const bool rows_in = r - lane >= L::kTile ? false
+                           : KEYS               ? first_pos + 31 < s.n
                                 : first_pos >= 0 && first_pos + 31 < s.n && row - lane + 31 < w.q_len;
       uint64_t minus_lse = 0, minus_delta = 0;
       if (!KEYS && valid && n) {
@@ -1209,16 +1217,18 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
               v = both(t.x, t.y);
               return upper;
             };
-            if constexpr (KEYS) {
+            if constexpr (KEYS && OUT != 1) {
 #pragma unroll
               for (int e = 0; e < 16; ++e) u[e] = pack(pr[e]);
               tc::tmem_store_32x16_async(
                   buf + operand_col<KEYS>(0, pl, 0) + (pl < 2 ? half * 32 : half * 16), u);
             }
+            if constexpr (OUT != 2) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) u[e] = pack(ds[e]);
-            tc::tmem_store_32x16_async(
-                buf + operand_col<KEYS>(KEYS ? 1 : 0, pl, 0) + (pl < 2 || !KEYS ? half * 32 : half * 16), u);
+              for (int e = 0; e < 16; ++e) u[e] = pack(ds[e]);
+              tc::tmem_store_32x16_async(
+                  buf + operand_col<KEYS>(KEYS ? 1 : 0, pl, 0) + (pl < 2 || !KEYS ? half * 32 : half * 16), u);
+            }
           }
         }
         // Moving rows behind the sequence may hold anything, and 0 times NaN is NaN: clear them.
@@ -1251,11 +1261,13 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
         tc::tc_fence_after();
         if constexpr (NP > 1) add_sums(n == 1);
       }
-      // queries: both groups store half of dq; keys: group 0 stores dk, group 1 dv.
-      // (bf16 heads of 64: group 0 stores dq, whose 64 columns are one box)
+      // One result: both groups store half of its columns (bf16 heads of 64: group 0 stores all, as 64
+      // columns are one box); both of the key side's: group 0 stores dk, group 1 dv.
+      constexpr bool kBoth = KEYS && OUT == 0;
       constexpr int cols = NP == 1 && L::kOuts * DH == 64 ? 64 : L::kOuts * DH / 2;
+      const int out = kBoth ? g : OUT == 2;
       const uint32_t from = lanes + (NP > 1 ? L::kSum : L::kAcc) + g * cols;
-      const float factor = !KEYS || g == 0 ? w.scale : 1.f;
+      const float factor = KEYS && out ? 1.f : w.scale;
       const int warp_row = row - lane;
 #pragma unroll 1
       for (int c = 0; c < cols && g * cols < static_cast<int>(L::kOuts) * DH; c += 32) {
@@ -1264,15 +1276,16 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
         if (n) tc::tmem_load_32x32(from + c, u);
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[e] = n ? __uint_as_float(u[e]) * factor : 0.f;
-        const int col = KEYS ? c : g * cols + c;
+        const int col = kBoth ? c : g * cols + c;
+        if (r - lane >= L::kTile) continue;
         if (KEYS && k.slot >= 0) {
-          float* dst = p.partial + ((k.slot * 2 + g) * 128 + r) * w.head_dim + col;
+          float* dst = p.partial + ((k.slot * 2 + out) * p.tile + r) * w.head_dim + col;
 #pragma unroll
           for (int e = 0; e < 32; e += 4)
             if (col + e < w.head_dim)
               *reinterpret_cast<float4*>(dst + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         } else if (warp_row < (KEYS ? w.kv_len : w.q_len)) {
-          box.put<NP>(KEYS && g ? &p.out2 : &p.out1, o, col, warp_row, KEYS ? k.kh : q.h[0], b);
+          box.put<NP>(out ? &p.out2 : &p.out1, o, col, warp_row, KEYS ? k.kh : q.h[0], b);
         }
       }
       if (n) {
@@ -1299,12 +1312,12 @@ __global__ void __launch_bounds__(256) window_partials_kernel(const __grid_const
   const uint64_t i = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   const int e = static_cast<int>(i % d4) * 4;
   uint64_t rest = i / d4;
-  const int r = static_cast<int>(rest % 128);
-  rest /= 128;
+  const int r = static_cast<int>(rest % p.tile);
+  rest /= p.tile;
   const int out = static_cast<int>(rest & 1);
   rest >>= 1;
   const int which = static_cast<int>(rest % bk);
-  const int tile = static_cast<int>(rest / bk), row = tile * 128 + r;
+  const int tile = static_cast<int>(rest / bk), row = tile * p.tile + r;
   if (tile >= (p.head_parts > 1 ? p.tiles : p.first_tiles) || row >= w.kv_len) return;
   const int parts_first = p.chunks * p.head_parts;
   const bool is_first = tile < p.first_tiles;
@@ -1313,8 +1326,8 @@ __global__ void __launch_bounds__(256) window_partials_kernel(const __grid_const
       is_first ? (static_cast<uint64_t>(tile) * bk + which) * parts_first
                : static_cast<uint64_t>(p.first_tiles) * bk * parts_first +
                      (static_cast<uint64_t>(tile - p.first_tiles) * bk + which) * p.head_parts;
-  const float* src = p.partial + ((slot * 2 + out) * 128 + r) * w.head_dim + e;
-  const uint64_t step = 2ull * 128 * w.head_dim;
+  const float* src = p.partial + ((slot * 2 + out) * p.tile + r) * w.head_dim + e;
+  const uint64_t step = 2ull * p.tile * w.head_dim;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
   for (int k = 0; k < parts; ++k) {
@@ -1467,7 +1480,7 @@ cudaError_t launch_forward(TcParams& p, int device, cudaStream_t stream) {
 }
 
 struct BackwardPlan {
-  int tiles, first_tiles, chunks, chunk, head_parts;
+  int tile, tiles, first_tiles, chunks, chunk, head_parts;
   uint64_t slots;  // partials
 };
 // Chunks of the first tokens' tiles cost about what another key tile does (window + 127 rows, at
@@ -1475,8 +1488,9 @@ struct BackwardPlan {
 // over items where there would be fewer than two items per SM.
 BackwardPlan backward_plan(const WindowParams& w, int device) {
   BackwardPlan b;
-  b.tiles = (w.kv_len + 127) / 128;
-  b.first_tiles = (std::min(w.sinks, w.kv_len) + 127) / 128;
+  b.tile = w.dtype == SPAR_B200_FLOAT32 && w.head_dim > 64 ? 64 : 128;  // Bwd::kTile
+  b.tiles = (w.kv_len + b.tile - 1) / b.tile;
+  b.first_tiles = (std::min(w.sinks, w.kv_len) + b.tile - 1) / b.tile;
   const int64_t rows = std::max<int64_t>(512, (static_cast<int64_t>(w.window) + 191) / 64 * 64);
   b.chunk = static_cast<int>(std::min<int64_t>(rows, std::max(64, w.q_len)));
   b.chunks = w.q_len > 0 ? (w.q_len + b.chunk - 1) / b.chunk : 1;
@@ -1490,13 +1504,13 @@ BackwardPlan backward_plan(const WindowParams& w, int device) {
   return b;
 }
 uint64_t partial_bytes(const WindowParams& w, const BackwardPlan& b) {
-  return round256(b.slots * 2 * 128 * w.head_dim * sizeof(float));
+  return round256(b.slots * 2 * b.tile * w.head_dim * sizeof(float));
 }
 
-template <bool KEYS, int DH, int NP, int ST>
+template <bool KEYS, int DH, int NP, int ST, int OUT = 0>
 cudaError_t launch_backward(const BackwardParams& p, int device, cudaStream_t stream) {
-  using L = Bwd<KEYS, DH, NP, ST>;
-  auto kernel = window_backward_kernel<KEYS, DH, NP, ST>;
+  using L = Bwd<KEYS, DH, NP, ST, OUT>;
+  auto kernel = window_backward_kernel<KEYS, DH, NP, ST, OUT>;
   const cudaError_t e = raise_dynamic_smem(reinterpret_cast<const void*>(kernel), device, L::kSmem);
   if (e != cudaSuccess) return e;
   const unsigned grid = static_cast<unsigned>(std::min(p.items, sm_count(device)));
@@ -1509,8 +1523,6 @@ bool tc_supported(const WindowParams& w, bool backward) {
   if (w.head_dim % 8 || w.head_dim > 128) return false;
   const int size = w.dtype == SPAR_B200_FLOAT32 ? 4 : 2;
   if (backward) {
-    // three planes of two stationary operands of 128 columns do not fit in shared memory
-    if (w.head_dim > 64 && w.dtype == SPAR_B200_FLOAT32) return false;
     if (w.q_len == 0 || !tiled_view(w.dout, size, w.batch, w.q_len, w.heads) ||
         !tiled_view(w.dq, size, w.batch, w.q_len, w.heads) ||
         !tiled_view(w.dk, size, w.batch, w.kv_len, w.kv_heads) ||
@@ -1578,6 +1590,7 @@ cudaError_t tc_backward(const WindowParams& w, void* scratch, int device, cudaSt
   if (!p.wait_flag) return cudaErrorInvalidDevice;
   p.ksteps = (w.head_dim + 15) / 16;
   p.scale_log2 = w.scale * kLog2e;
+  p.tile = plan.tile;
   p.tiles = plan.tiles;
   p.first_tiles = plan.first_tiles;
   p.chunks = plan.chunks;
@@ -1594,29 +1607,34 @@ cudaError_t tc_backward(const WindowParams& w, void* scratch, int device, cudaSt
   e = launch(delta, dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, stream, w, lanes);
   if (e != cudaSuccess) return e;
 
-  if (!operand_map(&p.s1, w, o[0], 128) || !operand_map(&p.s2, w, o[3], 128) ||
+  if (!operand_map(&p.s1, w, o[0], p.tile) || !operand_map(&p.s2, w, o[3], p.tile) ||
       !operand_map(&p.m1, w, o[1], kMoving) || !operand_map(&p.m2, w, o[2], kMoving) ||
       !result_map(&p.out1, w, w.dq, ql, h))
     return cudaErrorInvalidValue;
-  p.items = static_cast<int>(w.batch * h * ((ql + 127) / 128));
-  e = f32    ? launch_backward<false, 64, 3, 2>(p, device, stream)
+  p.items = static_cast<int>(w.batch * h * ((ql + p.tile - 1) / p.tile));
+  e = f32    ? (wide ? launch_backward<false, 128, 3, 1>(p, device, stream)
+                     : launch_backward<false, 64, 3, 2>(p, device, stream))
       : wide ? launch_backward<false, 128, 1, 4>(p, device, stream)
              : launch_backward<false, 64, 1, 6>(p, device, stream);
   if (e != cudaSuccess) return e;
 
-  if (!operand_map(&p.s1, w, o[1], 128) || !operand_map(&p.s2, w, o[2], 128) ||
+  if (!operand_map(&p.s1, w, o[1], p.tile) || !operand_map(&p.s2, w, o[2], p.tile) ||
       !operand_map(&p.m1, w, o[0], kMoving) || !operand_map(&p.m2, w, o[3], kMoving) ||
       !result_map(&p.out1, w, w.dk, kl, kh) || !result_map(&p.out2, w, w.dv, kl, kh))
     return cudaErrorInvalidValue;
   p.items = static_cast<int>(w.batch * kh * p.head_parts *
                              (p.first_tiles * static_cast<uint64_t>(p.chunks) + p.tiles - p.first_tiles));
-  e = f32    ? launch_backward<true, 64, 3, 2>(p, device, stream)
+  // (the sums of dk and dv and their tiles' products, 512 columns, leave TMEM no room for the scores of
+  // fp32 heads above 64: a launch each)
+  if (f32 && wide && (e = launch_backward<true, 128, 3, 1, 2>(p, device, stream)) != cudaSuccess) return e;
+  e = f32    ? (wide ? launch_backward<true, 128, 3, 1, 1>(p, device, stream)
+                     : launch_backward<true, 64, 3, 2>(p, device, stream))
       : wide ? launch_backward<true, 128, 1, 3>(p, device, stream)
              : launch_backward<true, 64, 1, 6>(p, device, stream);
   if (e != cudaSuccess || !plan.slots) return e;
 
   const uint64_t cut = p.head_parts > 1 ? p.tiles : p.first_tiles;
-  const uint64_t units = w.batch * kh * cut * 2 * 128 * (w.head_dim / 4);
+  const uint64_t units = w.batch * kh * cut * 2 * p.tile * (w.head_dim / 4);
   auto sum = f32 ? window_partials_kernel<float> : window_partials_kernel<__nv_bfloat16>;
   return launch(sum, dim3(static_cast<unsigned>((units + 255) / 256)), dim3(256), 0, stream, p);
 }
