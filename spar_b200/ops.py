@@ -13,8 +13,8 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from ._lib import (SparB200Gemm, SparB200Rotary, SparB200RotaryScaling, SparB200TensorSlice,
-                   SparB200WindowAttention, call)
+from ._lib import (ROTARY, WINDOW_ATTENTION, SparB200Gemm, SparB200RotaryScaling,
+                   SparB200TensorSlice, call)
 
 TF32, TF32X3 = 0, 1
 EPI_NONE, EPI_BIAS, EPI_BIAS_GELU, EPI_GELU_BWD, EPI_BIAS_ADD = 0, 1, 2, 3, 4
@@ -336,7 +336,7 @@ def rope_apply_(x, table, batch: int, t: int, heads: int, d: int, ld: int, inver
 _ELEMENT = {torch.float32: 0, torch.bfloat16: 1}
 _ROTARY_LAYOUT = {"interleaved": 0, "half": 1}
 _ROTARY_SCALING = {"none": 0, "linear": 1, "base": 2, "parts": 3}
-_NO_HEADS = (None, 0, 0, 0)
+_NO_HEADS = (0, 0, 0, 0)
 
 
 def _heads_view(t, name, like=None, shape=None):
@@ -373,9 +373,9 @@ def _out_view(t, name, like):
 
 
 def _small(t, name, dtype, shape, like):
-    """Pointer of an optional contiguous tensor of the given type and shape on like's device."""
+    """Pointer of an optional contiguous tensor of the given type and shape on like's device (None: 0)."""
     if t is None:
-        return None
+        return 0
     if (t.dtype is not dtype or t.shape != shape or t.get_device() != like.get_device()
             or not t.is_contiguous()):
         raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {tuple(shape)} on the "
@@ -420,8 +420,8 @@ def rotary_table(rows: int, rotary_dim: int, theta: float = 10000.0, start: int 
 
 def _rotary_desc(q, k, table, layout, inverse, positions, start, invalid, q_out, k_out, q_weight=None,
                  k_weight=None, eps=0.0, dq=None, dk=None, dq_weight=None, dk_weight=None,
-                 accumulate=0, scratch=None):
-    """The descriptor; q_out, k_out, dq and dk are views (of _heads_view) already."""
+                 accumulate=0, scratch=0):
+    """The descriptor (a SparB200Rotary's bytes); q_out, k_out, dq and dk are views (of _heads_view) already."""
     qv = _heads_view(q, "q")
     batch, seq, heads, dim = q.shape
     kv_heads, kv = 0, _NO_HEADS
@@ -437,7 +437,7 @@ def _rotary_desc(q, k, table, layout, inverse, positions, start, invalid, q_out,
     if len(shape) != 3 or shape[2] != 2 or start < 0:
         raise ValueError("table must be [rows, rotary_dim / 2, 2] and start not negative")
     head = (dim,)
-    return SparB200Rotary(
+    return ROTARY.pack(
         _ELEMENT[q.dtype], tag, inverse, batch, seq, heads, kv_heads, dim, 2 * shape[1],
         _small(table, "table", torch.float32, shape, q), shape[0],
         _small(positions, "positions", torch.int32, (batch, seq), q), start,
@@ -465,7 +465,7 @@ def rotary(q, k, table, *, layout: str = "interleaved", positions=None, start: i
     place. `invalid` (int32 [1]) is set to 1 by a position outside the table (outputs zeros)."""
     q_out, k_out, q_view, k_view = _rotary_outputs(q, k, q_out, k_out)
     desc = _rotary_desc(q, k, table, layout, int(inverse), positions, start, invalid, q_view, k_view)
-    call("spar_b200_rotary", ctypes.byref(desc), _dev(q), _stream(q))
+    call("spar_b200_rotary", desc, _dev(q), _stream(q))
     return q_out, k_out
 
 
@@ -477,7 +477,7 @@ def qk_norm_rotary_forward(q, k, q_weight, k_weight, table, eps: float = 1e-6, *
     q_out, k_out, q_view, k_view = _rotary_outputs(q, k, q_out, k_out)
     desc = _rotary_desc(q, k, table, layout, 0, positions, start, invalid, q_view, k_view, q_weight,
                         k_weight, eps)
-    call("spar_b200_qk_norm_rotary_forward", ctypes.byref(desc), _dev(q), _stream(q))
+    call("spar_b200_qk_norm_rotary_forward", desc, _dev(q), _stream(q))
     return q_out, k_out
 
 
@@ -503,13 +503,14 @@ def qk_norm_rotary_backward(dq_out, dk_out, q, k, q_weight, k_weight, table, eps
                         k_weight, eps, _heads_view(dq_out, "dq_out", q, q.shape),
                         None if k is None else _heads_view(dk_out, "dk_out", q, k.shape), dq_weight,
                         dk_weight, int(accumulate_params), scratch.data_ptr())
-    call("spar_b200_qk_norm_rotary_backward", ctypes.byref(desc), _dev(q), _stream(q))
+    call("spar_b200_qk_norm_rotary_backward", desc, _dev(q), _stream(q))
     return dq, dk, dq_weight, dk_weight
 
 
 # ------------------------------------------------------------------------------- window attention
 def _window_desc(q, k, v, out, lse, window, sinks, scale, lengths, first, back=_NO_HEADS * 4):
-    """The descriptor; out and back (dout, dq, dk, dv) are views (of _heads_view) already."""
+    """The descriptor (a SparB200WindowAttention's bytes); out and back (dout, dq, dk, dv) are views (of
+    _heads_view) already."""
     qv = _heads_view(q, "q")
     kv = _heads_view(k, "k", q)
     batch, q_len, heads, dim = q.shape
@@ -523,21 +524,20 @@ def _window_desc(q, k, v, out, lse, window, sinks, scale, lengths, first, back=_
     elif not scale > 0.0:
         raise ValueError("scale must be positive")
     each = (batch,)
-    return SparB200WindowAttention(
+    return WINDOW_ATTENTION.pack(
         _ELEMENT[q.dtype], batch, q_len, kv_len, heads, kv_heads, dim, window, sinks, scale,
         _small(lengths, "lengths", torch.int32, each, q), _small(first, "first", torch.int32, each, q),
         *qv, *kv, *_heads_view(v, "v", q, k.shape), *out,
-        _small(lse, "lse", torch.float32, (batch, heads, q_len), q), *back, None)
+        _small(lse, "lse", torch.float32, (batch, heads, q_len), q), *back, 0)
 
 
 def _window_call(name, desc, backward, q):
     device = q.get_device()
-    ref = ctypes.byref(desc)
-    nbytes = _lib.load().spar_b200_window_attention_scratch_bytes(ref, backward, device)
+    nbytes = _lib.load().spar_b200_window_attention_scratch_bytes(desc, backward, device)
     if nbytes:
         scratch = torch.empty(nbytes, device=q.device, dtype=torch.uint8)
-        desc.scratch = scratch.data_ptr()
-    call(name, ref, device, _stream(q))
+        desc = desc[:-8] + scratch.data_ptr().to_bytes(8, "little")  # the last field
+    call(name, desc, device, _stream(q))
 
 
 def window_attention_forward(q, k, v, window: int, sinks: int = 0, *, scale: float | None = None,
@@ -551,7 +551,7 @@ def window_attention_forward(q, k, v, window: int, sinks: int = 0, *, scale: flo
     p >= lengths[b] sees nothing (out 0, lse -inf). scale None: 1 / sqrt(head_dim).
     Returns (out like q, lse [batch, heads, q_len])."""
     out, view = _out_view(out, "out", q)
-    lse = torch.empty((q.shape[0], q.shape[2], q.shape[1]), device=q.device, dtype=torch.float32)
+    lse = q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)
     desc = _window_desc(q, k, v, view, lse, window, sinks, scale, lengths, first)
     _window_call("spar_b200_window_attention_forward", desc, 0, q)
     return out, lse

@@ -176,6 +176,11 @@ def test_new_structures_mirror_the_header():
     """Sizes that a C compiler gives the header's structs (all members 8-byte aligned after the tags)."""
     from spar_b200 import _lib
 
-    assert ctypes.sizeof(_lib.SparB200Rotary) == 352
-    assert ctypes.sizeof(_lib.SparB200WindowAttention) == 368
+    assert ctypes.sizeof(_lib.SparB200Rotary) == 352 == _lib.ROTARY.size
+    assert ctypes.sizeof(_lib.SparB200WindowAttention) == 368 == _lib.WINDOW_ATTENTION.size
+    for kind, packed in ((_lib.SparB200Rotary, _lib.ROTARY),
+                         (_lib.SparB200WindowAttention, _lib.WINDOW_ATTENTION)):
+        names = [name for name, _ in kind._fields_]
+        held = kind.from_buffer_copy(packed.pack(*range(1, len(names) + 1)))
+        assert [getattr(held, name) for name in names] == list(range(1, len(names) + 1))
     assert ctypes.sizeof(_lib.SparB200RotaryScaling) == 48
