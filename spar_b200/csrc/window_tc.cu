@@ -40,6 +40,11 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kPolyShare = 2;        // of every 8 weights of an unmasked bf16 tile (see ex2_poly)
 constexpr float kRescaleLog2 = 8.f;  // the running maximum moves only past this margin (P <= 2^8)
 
+// The warp's number, told to the compiler as one value of the warp.
+__device__ __forceinline__ int warp_index() {
+  return __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
+}
+
 // Why a CTA gives up: the CTA's flag, and the one that spar_b200_attention_error reads.
 struct Abort {
   volatile int* cta;
@@ -385,7 +390,7 @@ __global__ void __launch_bounds__(128 + 128 * QT, 1) window_forward_kernel(
   uint64_t* drain = v_empty + VS;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
   const Abort abort_flag = {reinterpret_cast<volatile int*>(tmem_slot + 1), p.wait_flag};
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
   const WindowParams& w = p.w;
 
   if (threadIdx.x == 0) {
@@ -417,7 +422,7 @@ __global__ void __launch_bounds__(128 + 128 * QT, 1) window_forward_kernel(
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   pdl_begin();
 
   // Four warps that feed and four per query tile: the launch's registers (168 a thread of three
@@ -581,13 +586,21 @@ __global__ void __launch_bounds__(128 + 128 * QT, 1) window_forward_kernel(
     bool ok = true;
     for (int idx = blockIdx.x; idx < p.items && ok; idx += gridDim.x) {
       const Item it = item_of<QT, BN>(p, idx);
-      const int row = it.row[x], pos = it.s.p0 + row + r;
+      const int row = x ? it.row[1] : it.row[0], head = x ? it.h[1] : it.h[0];
+      const bool any = x ? it.any[1] : it.any[0];
+      const int from = it.ns + (x ? it.a[1] : it.a[0]), upto = it.ns + (x ? it.b_end[1] : it.b_end[0]);
+      auto next = [&](int j) {  // as next_tile
+        if (j < it.ns) return j;
+        j = max(j, from);
+        return j < upto ? j : it.n;
+      };
+      const int pos = it.s.p0 + row + r;
       const bool valid = row + r < w.q_len && pos >= 0 && pos < it.s.n;
       const int first_pos = it.s.p0 + row + static_cast<int>(quarter) * 32;  // of this warp
       float m = -INFINITY, sum = 0.f, pending = 0.f;
       int done = 0;
-      if (it.any[x]) {
-        for (int j = next_tile(it, x, 0); j < it.n && ok; j = next_tile(it, x, j + 1), ++done) {
+      if (any) {
+        for (int j = next(0); j < it.n && ok; j = next(j + 1), ++done) {
           const int key = key_of<BN>(it, j);
           if (!(ok = wait_or_abort(s_full + x, sn, abort_flag))) break;
           ++sn;
@@ -716,7 +729,7 @@ __global__ void __launch_bounds__(128 + 128 * QT, 1) window_forward_kernel(
         float o[32];
 #pragma unroll
         for (int e = 0; e < 32; ++e) o[e] = 0.f;
-        if (it.any[x]) {
+        if (any) {
           uint32_t u[32];
           if constexpr (NP == 1) {
             tc::tmem_load_32x32(lanes + L::kS + c * 32, u);
@@ -733,15 +746,15 @@ __global__ void __launch_bounds__(128 + 128 * QT, 1) window_forward_kernel(
           }
         }
         if (row + quarter * 32 < w.q_len)
-          box.put<NP>(&p.out, o, c * 32, row + quarter * 32, it.h[x], it.b);
+          box.put<NP>(&p.out, o, c * 32, row + quarter * 32, head, it.b);
       }
-      if (it.any[x]) {
+      if (any) {
         tc::tc_fence_before();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(o_empty + x);
       }
       if (stored && w.lse)
-        w.lse[(static_cast<uint64_t>(it.b) * w.heads + it.h[x]) * w.q_len + row + r] =
+        w.lse[(static_cast<uint64_t>(it.b) * w.heads + head) * w.q_len + row + r] =
             valid ? m * kLn2 + logf(sum) : -INFINITY;
     }
     if (lane == 0) tc::bulk_wait_all();
@@ -889,7 +902,7 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
   uint64_t* m_empty = m_full + ST;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(m_empty + ST);
   const Abort abort_flag = {reinterpret_cast<volatile int*>(tmem_slot + 1), p.wait_flag};
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
   const WindowParams& w = p.w;
 
   if (threadIdx.x == 0) {
@@ -918,7 +931,7 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
   tc::tc_fence_before();
   __syncthreads();
   tc::tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   pdl_begin();
 
   // Moving tiles of an item; both sides number them 0 .. n - 1.
