@@ -787,7 +787,7 @@ struct BackwardParams {
   CUtensorMap out1, out2;      // dq, or dk and dv
   int* wait_flag;
   int items, tiles, ksteps;
-  float scale_log2;
+  float scale_log2, inv_scale;
   // keys: the first `first_tiles` key tiles are cut into `chunks` row ranges, every tile into
   // `head_parts` groups of query heads.
   int first_tiles, chunks, chunk, head_parts;
@@ -858,8 +858,16 @@ struct Bwd {
   static constexpr uint32_t kA = 0;
   static constexpr uint32_t kB = kA + kStats * 2 * kStat;
   static constexpr uint32_t kOut = kB + ST * 2 * kMov;        // 4 KB per softmax warp
-  static constexpr uint32_t kRows = kOut + 8 * 4096;          // [ST][2][64] -lse log2 e, -D
-  static constexpr uint32_t kBar = kRows + (KEYS ? ST * kMoving * 8 : 0);
+  // Keys, statistics of the moving rows. bf16: as a K step of the products themselves, operands of 16
+  // more columns without swizzle (core matrices of 8 rows x 16 bytes, the two of a row group
+  // neighbours): ones on the key side, [ST][2] tiles of three bf16 planes of -lse / scale and of -D
+  // on the row side, so that S and dP arrive with them subtracted. (Read from shared memory by every
+  // thread they took 620 of 2090 cycles a tile.) fp32: [ST][2][64] -lse log2 e, -D.
+  static constexpr bool kAugment = KEYS && NP == 1;
+  static constexpr uint32_t kOnes = kOut + 8 * 4096;
+  static constexpr uint32_t kRows = kOnes + (kAugment ? 4096 : 0);
+  static constexpr uint32_t kRowsBytes = kAugment ? 4096 : 512;  // of a stage
+  static constexpr uint32_t kBar = kRows + (KEYS ? ST * kRowsBytes : 0);
   static constexpr uint32_t kSmem = kBar + 256 + 1024;
   static_assert((13 + 2 * ST) * 8 + 8 <= 256, "backward barriers");
   static_assert(kSmem <= kMaxSmem, "backward shared memory");
@@ -882,6 +890,16 @@ __host__ __device__ constexpr uint32_t operand_col(int which, int pl, int ks) {
   if (pl < 2) return which * 64 + g * 32 + pl * 16 + sub;
   return KEYS ? 128 + which * 32 + g * 16 + sub : 64 + g * 32 + sub;
 }
+
+// Three bf16 planes of a float as the first elements of a 16-byte row of a core matrix.
+__device__ __forceinline__ uint4 plane_row(float v) {
+  float rest = 0.f, x = v;
+  const uint32_t first = take_upper(x, rest) & 0xffffu, second = take_upper(x, rest) << 16;
+  return make_uint4(first | second, take_upper(x, rest) & 0xffffu, 0, 0);
+}
+__device__ __forceinline__ uint32_t core_row(int row) { return (row >> 3) * 256 + (row & 7) * 16; }
+// Descriptor of a 16-column K-major operand of such core matrices.
+__device__ __forceinline__ uint64_t core_desc(uint32_t addr) { return tc::smem_desc(addr, 128, 256, 0); }
 
 template <bool KEYS, int DH, int NP, int ST, int OUT>
 __global__ void __launch_bounds__(384, 1) window_backward_kernel(
@@ -927,6 +945,15 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
   if (warp == 1) {
     tc::tmem_alloc(tmem_slot, kTmemCols);
     tc::tmem_relinquish();
+  }
+  if constexpr (L::kAugment) {  // ones in the columns of the three planes; zeros behind them
+    for (int i = threadIdx.x; i < 128 * 2; i += blockDim.x)
+      *reinterpret_cast<uint4*>(smem + L::kOnes + core_row(i >> 1) + (i & 1) * 128) =
+          i & 1 ? make_uint4(0, 0, 0, 0) : make_uint4(0x3f803f80u, 0x3f80u, 0, 0);
+    for (int i = threadIdx.x; i < ST * 2 * kMoving; i += blockDim.x)
+      *reinterpret_cast<uint4*>(smem + L::kRows + i / kMoving * 2048 + core_row(i % kMoving) + 128) =
+          make_uint4(0, 0, 0, 0);
+    tc::fence_proxy_async_smem();
   }
   tc::tc_fence_before();
   __syncthreads();
@@ -1000,14 +1027,23 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
               }
           }
           if constexpr (KEYS) {
-            float* stats = reinterpret_cast<float*>(smem + L::kRows) + st * 2 * kMoving;
-            const uint64_t at = (static_cast<uint64_t>(b) * w.heads + h) * w.q_len;
+  const uint64_t at = (static_cast<uint64_t>(b) * w.heads + h) * w.q_len;
 #pragma unroll
             for (int e = lane; e < kMoving; e += 32) {
               const bool in = row + e < k.end;
-              stats[e] = in ? -__ldg(w.lse + at + row + e) * kLog2e : 0.f;
-              stats[kMoving + e] = in ? -__ldg(w.delta + at + row + e) : 0.f;
+              const float lse = in ? __ldg(w.lse + at + row + e) : 0.f;
+              const float delta = in ? __ldg(w.delta + at + row + e) : 0.f;
+              if constexpr (L::kAugment) {
+                uint8_t* tile = smem + L::kRows + st * L::kRowsBytes + core_row(e);
+                *reinterpret_cast<uint4*>(tile) = plane_row(-lse * p.inv_scale);
+                *reinterpret_cast<uint4*>(tile + 2048) = plane_row(-delta);
+              } else {
+                float* stats = reinterpret_cast<float*>(smem + L::kRows + st * L::kRowsBytes);
+                stats[e] = -lse * kLog2e;
+                stats[kMoving + e] = -delta;
+              }
             }
+            if (L::kAugment) tc::fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(m_full + st);
           }
@@ -1024,6 +1060,8 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
         const uint32_t idesc_s = tc::idesc_bf16(128, kMoving, 0, 0);
         const uint32_t idesc_o = tc::idesc_bf16(128, 16 * p.ksteps, 0, 1);
         const uint32_t a_addr = tc::smem_u32(smem + L::kA), b_addr = tc::smem_u32(smem + L::kB);
+      [[maybe_unused]] const uint32_t ones = tc::smem_u32(smem + L::kOnes),
+                                      stats = tc::smem_u32(smem + L::kRows);
         uint32_t an = 0, mn = 0, sums = 0;
         bool ok = true;
         // S and dP of moving tile number m; after the item's last one the stationary operands are free.
@@ -1036,6 +1074,11 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
             const uint32_t a = kmajor_low(a_addr + (2 * (an % L::kStats) + half) * L::kStat),
                            b = kmajor_low(b_addr + (2 * st + half) * L::kMov);
             uint32_t acc = 0;
+          if constexpr (L::kAugment) {
+            tc::mma_f16(buf + half * 64, core_desc(ones), core_desc(stats + st * L::kRowsBytes + half * 2048), idesc_s,
+                        0);
+            acc = 1;
+          }
 #pragma unroll
             for (int pr = 0; pr < kProducts<NP>; ++pr)
 #pragma unroll
@@ -1174,8 +1217,8 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
         if (!valid) hi = -1;
         if (!(ok = wait_or_abort(s_full + m % L::kBuffers, m / L::kBuffers, abort_flag))) break;
         tc::tc_fence_after();
-        if (KEYS && !(ok = wait_or_abort(m_full + st, m / ST, abort_flag))) break;
-        const float* stats = reinterpret_cast<const float*>(smem + L::kRows) + st * 2 * kMoving;
+        const float* stats = reinterpret_cast<const float*>(smem + L::kRows + st * L::kRowsBytes);
+        if (KEYS && !L::kAugment && !(ok = wait_or_abort(m_full + st, m / ST, abort_flag))) break;
 #pragma unroll
         for (int half = kTurns ? 0 : g; half < (kTurns ? 2 : g + 1); ++half) {
           const int c0 = half * 32;
@@ -1192,21 +1235,28 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
           uint64_t pr[16], ds[16];
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
-            uint64_t l0 = minus_lse, l1 = minus_lse, d0 = minus_delta, d1 = minus_delta;
-            if constexpr (KEYS) {
-              const float4 l = *reinterpret_cast<const float4*>(stats + c0 + 2 * e);
-              const float4 d = *reinterpret_cast<const float4*>(stats + kMoving + c0 + 2 * e);
-              l0 = both(l.x, l.y), l1 = both(l.z, l.w), d0 = both(d.x, d.y), d1 = both(d.z, d.w);
+            const uint64_t s0 = both(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])),
+                           s1 = both(__uint_as_float(sv[2 * e + 2]), __uint_as_float(sv[2 * e + 3]));
+            uint64_t g0 = both(__uint_as_float(dv[2 * e]), __uint_as_float(dv[2 * e + 1])),
+                     g1 = both(__uint_as_float(dv[2 * e + 2]), __uint_as_float(dv[2 * e + 3]));
+            uint64_t x0, x1;
+            if constexpr (L::kAugment) {
+              x0 = mul2(s0, scale), x1 = mul2(s1, scale);
+            } else {
+              uint64_t l0 = minus_lse, l1 = minus_lse, d0 = minus_delta, d1 = minus_delta;
+              if constexpr (KEYS) {
+                const float4 l = *reinterpret_cast<const float4*>(stats + c0 + 2 * e);
+                const float4 d = *reinterpret_cast<const float4*>(stats + kMoving + c0 + 2 * e);
+                l0 = both(l.x, l.y), l1 = both(l.z, l.w), d0 = both(d.x, d.y), d1 = both(d.z, d.w);
+              }
+              x0 = fma2(s0, scale, l0), x1 = fma2(s1, scale, l1);
+              g0 = add2(g0, d0), g1 = add2(g1, d1);
             }
-            const uint64_t x0 = fma2(both(__uint_as_float(sv[2 * e]), __uint_as_float(sv[2 * e + 1])), scale, l0);
-            const uint64_t x1 =
-                fma2(both(__uint_as_float(sv[2 * e + 2]), __uint_as_float(sv[2 * e + 3])), scale, l1);
             const float2 t0 = halves(x0), t1 = halves(x1);
             pr[e] = both(ex2(t0.x), ex2(t0.y));
             pr[e + 1] = both(ex2(t1.x), ex2(t1.y));
-            ds[e] = mul2(pr[e], add2(both(__uint_as_float(dv[2 * e]), __uint_as_float(dv[2 * e + 1])), d0));
-            ds[e + 1] =
-                mul2(pr[e + 1], add2(both(__uint_as_float(dv[2 * e + 2]), __uint_as_float(dv[2 * e + 3])), d1));
+            ds[e] = mul2(pr[e], g0);
+            ds[e + 1] = mul2(pr[e + 1], g1);
           }
           if (!all_seen) {
             uint32_t seen = below(hi + 1 - c0) & ~below(lo - c0);
@@ -1603,6 +1653,7 @@ cudaError_t tc_backward(const WindowParams& w, void* scratch, int device, cudaSt
   if (!p.wait_flag) return cudaErrorInvalidDevice;
   p.ksteps = (w.head_dim + 15) / 16;
   p.scale_log2 = w.scale * kLog2e;
+  p.inv_scale = 1.f / w.scale;
   p.tile = plan.tile;
   p.tiles = plan.tiles;
   p.first_tiles = plan.first_tiles;
