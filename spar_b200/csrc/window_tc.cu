@@ -786,6 +786,7 @@ struct BackwardParams {
   CUtensorMap s1, s2, m1, m2;  // stationary and moving operands: q, dout / k, v or k, v / q, dout
   CUtensorMap out1, out2;      // dq, or dk and dv
   int* wait_flag;
+  int* ticket;  // counts the items drawn beyond the first of each CTA; zero at the launch
   int items, tiles, ksteps;
   float scale_log2, inv_scale;
   // keys: the first `first_tiles` key tiles are cut into `chunks` row ranges, every tile into
@@ -804,26 +805,26 @@ struct KeyItem {
 };
 __device__ __forceinline__ KeyItem key_item(const BackwardParams& p, int idx) {
   const WindowParams& w = p.w;
-  const int bk = w.batch * w.kv_heads, first_items = p.first_tiles * bk * p.chunks * p.head_parts;
+  const int bk = w.batch * w.kv_heads, parts = p.chunks * p.head_parts;
+  const int others = (p.tiles - p.first_tiles) * bk * p.head_parts;
   KeyItem it;
   int part, which, tile, from = 0, to = w.q_len;
-  if (idx < first_items) {
-    const int parts = p.chunks * p.head_parts;
-    part = idx % parts;
-    const int rest = idx / parts;
+  if (idx < others) {
+    part = idx % p.head_parts;
+    const int rest = idx / p.head_parts;
+    which = rest % bk;
+    tile = p.first_tiles + rest / bk;
+    it.slot = p.head_parts > 1 ? static_cast<int64_t>(p.first_tiles) * bk * parts + idx : -1;
+  } else {
+    const int i = idx - others;
+    part = i % parts;
+    const int rest = i / parts;
     which = rest % bk;
     tile = rest / bk;
     from = (part / p.head_parts) * p.chunk;
     to = min(from + p.chunk, w.q_len);
-    it.slot = parts > 1 ? idx : -1;
+    it.slot = parts > 1 ? i : -1;
     part %= p.head_parts;
-  } else {
-    const int i = idx - first_items;
-    part = i % p.head_parts;
-    const int rest = i / p.head_parts;
-    which = rest % bk;
-    tile = p.first_tiles + rest / bk;
-    it.slot = p.head_parts > 1 ? idx : -1;
   }
   it.b = which / w.kv_heads;
   it.kh = which - it.b * w.kv_heads;
@@ -868,8 +869,8 @@ struct Bwd {
   static constexpr uint32_t kRows = kOnes + (kAugment ? 4096 : 0);
   static constexpr uint32_t kRowsBytes = kAugment ? 4096 : 512;  // of a stage
   static constexpr uint32_t kBar = kRows + (KEYS ? ST * kRowsBytes : 0);
-  static constexpr uint32_t kSmem = kBar + 256 + 1024;
-  static_assert((13 + 2 * ST) * 8 + 8 <= 256, "backward barriers");
+  static constexpr uint32_t kSmem = kBar + 320 + 1024;
+  static_assert((21 + 2 * ST) * 8 + 24 <= 320, "backward barriers");
   static_assert(kSmem <= kMaxSmem, "backward shared memory");
   // TMEM: buffers of S | dP (| the third planes of P and dS), then the products' sums, then
   // (NP = 3) the sums of earlier tiles.
@@ -918,7 +919,10 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
   uint64_t* drain = bars + 12;
   uint64_t* m_full = bars + 13;    // [ST]
   uint64_t* m_empty = m_full + ST;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(m_empty + ST);
+  uint64_t* item_full = m_empty + ST;  // [4]
+  uint64_t* item_empty = item_full + 4;
+  volatile int* items = reinterpret_cast<volatile int*>(item_empty + 4);  // [4]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(item_empty + 4) + 4;
   const Abort abort_flag = {reinterpret_cast<volatile int*>(tmem_slot + 1), p.wait_flag};
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const WindowParams& w = p.w;
@@ -938,6 +942,10 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
     for (int i = 0; i < ST; ++i) {
       tc::mbar_init(m_full + i, KEYS ? 2 : 1);  // TMA, and the rows' statistics
       tc::mbar_init(m_empty + i, 1);
+    }
+    for (int i = 0; i < 4; ++i) {
+      tc::mbar_init(item_full + i, 1);
+      tc::mbar_init(item_empty + i, 1 + 8);  // the issuer, the softmax warps
     }
     *abort_flag.cta = 0;
     tc::fence_barrier_init();
@@ -960,6 +968,14 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
   tc::tc_fence_after();
   const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
   pdl_begin();
+
+  // Items are drawn from a counter when the producer is done with the one before (their costs differ,
+  // and a fixed share left a third of the SMs with half the work), and handed on through `items`.
+  auto take = [&](uint32_t tn, int& idx) -> bool {
+    if (!wait_or_abort(item_full + (tn & 3), tn / 4, abort_flag)) return false;
+    idx = items[tn & 3];
+    return true;
+  };
 
   // Moving tiles of an item; both sides number them 0 .. n - 1.
   auto jobs_of = [&](int idx, Item& q, KeyItem& k) -> int {
@@ -985,7 +1001,17 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
       }
       uint32_t an = 0, mn = 0;
       bool ok = true;
-      for (int idx = blockIdx.x; idx < p.items && ok && !*abort_flag.cta; idx += gridDim.x) {
+      for (uint32_t tn = 0; ok && !*abort_flag.cta; ++tn) {
+        if (!(ok = wait_or_abort(item_empty + (tn & 3), tn / 4 + 1, abort_flag))) break;
+        int idx = blockIdx.x;
+        if (tn && lane == 0) idx = static_cast<int>(gridDim.x) + atomicAdd(p.ticket, 1);
+        idx = __shfl_sync(0xffffffffu, idx, 0);
+        if (lane == 0) {
+          items[tn & 3] = idx;
+          tc::mbar_arrive(item_full + (tn & 3));
+        }
+        __syncwarp();
+        if (idx >= p.items) break;
         Item q;
         KeyItem k;
         const int n = jobs_of(idx, q, k);
@@ -1093,7 +1119,11 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
           if (last) tc::mma_commit(a_empty + an % L::kStats);
           return true;
         };
-        for (int idx = blockIdx.x; idx < p.items && ok && !*abort_flag.cta; idx += gridDim.x) {
+        for (uint32_t tn = 0; ok && !*abort_flag.cta; ++tn) {
+          int idx;
+          if (!(ok = take(tn, idx))) break;
+          tc::mbar_arrive(item_empty + (tn & 3));
+          if (idx >= p.items) break;
           Item q;
           KeyItem k;
           const int n = jobs_of(idx, q, k);
@@ -1169,7 +1199,12 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
         tc::tmem_store_32x32(lanes + L::kSum + c, o);
       }
     };
-    for (int idx = blockIdx.x; idx < p.items && ok; idx += gridDim.x) {
+    for (uint32_t tn = 0; ok; ++tn) {
+      int idx;
+      if (!(ok = take(tn, idx))) break;
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(item_empty + (tn & 3));
+      if (idx >= p.items) break;
       Item q;
       KeyItem k;
       const int n = jobs_of(idx, q, k);
@@ -1405,11 +1440,13 @@ __global__ void __launch_bounds__(256) window_partials_kernel(const __grid_const
     *reinterpret_cast<float4*>(dst) = a;
 }
 
-// D = rowsum(dout o out), `lanes` threads per (token, head) row, eight elements each.
+// D = rowsum(dout o out), `lanes` threads per (token, head) row, eight elements each; and the item
+// counters of the launches that follow, to zero.
 template <typename T>
 __global__ void __launch_bounds__(256) window_delta_kernel(const __grid_constant__ WindowParams w,
-                                                           int lanes) {
+                                                           int lanes, int* tickets, int count) {
   pdl_begin();
+  if (blockIdx.x == 0 && threadIdx.x < static_cast<unsigned>(count)) tickets[threadIdx.x] = 0;
   const uint64_t unit = (static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / lanes;
   const int l = threadIdx.x & (lanes - 1);
   const bool live = unit < static_cast<uint64_t>(w.batch) * w.q_len * w.heads;
@@ -1546,15 +1583,16 @@ struct BackwardPlan {
   int tile, tiles, first_tiles, chunks, chunk, head_parts;
   uint64_t slots;  // partials
 };
-// Chunks of the first tokens' tiles cost about what another key tile does (window + 127 rows, at
-// least 512 so that a short window does not make hundreds). Query heads of a group are split
+// Chunks of the first tokens' tiles cost about half of what another key tile does (window + 127 rows;
+// at least 256 so that a short window does not make hundreds) and come last: they even out what the
+// whole tiles leave. Query heads of a group are split
 // over items where there would be fewer than two items per SM.
 BackwardPlan backward_plan(const WindowParams& w, int device) {
   BackwardPlan b;
   b.tile = w.dtype == SPAR_B200_FLOAT32 && w.head_dim > 64 ? 64 : 128;  // Bwd::kTile
   b.tiles = (w.kv_len + b.tile - 1) / b.tile;
   b.first_tiles = (std::min(w.sinks, w.kv_len) + b.tile - 1) / b.tile;
-  const int64_t rows = std::max<int64_t>(512, (static_cast<int64_t>(w.window) + 191) / 64 * 64);
+  const int64_t rows = std::max<int64_t>(256, (static_cast<int64_t>(w.window) / 2 + 127) / 64 * 64);
   b.chunk = static_cast<int>(std::min<int64_t>(rows, std::max(64, w.q_len)));
   b.chunks = w.q_len > 0 ? (w.q_len + b.chunk - 1) / b.chunk : 1;
   const int64_t bk = static_cast<int64_t>(w.batch) * w.kv_heads, items = bk * b.tiles;
@@ -1601,7 +1639,7 @@ bool tc_supported(const WindowParams& w, bool backward) {
 uint64_t tc_scratch_bytes(const WindowParams& w, bool backward, int device) {
   const uint64_t operands = (backward ? 2 : 1) * planes_bytes(w, w.q_len, w.heads) +
                             2 * planes_bytes(w, w.kv_len, w.kv_heads);
-  return backward ? operands + partial_bytes(w, backward_plan(w, device)) : operands;
+  return backward ? operands + partial_bytes(w, backward_plan(w, device)) + 256 : operands;
 }
 
 cudaError_t tc_forward(const WindowParams& w, void* scratch, int device, cudaStream_t stream) {
@@ -1649,6 +1687,7 @@ cudaError_t tc_backward(const WindowParams& w, void* scratch, int device, cudaSt
   memset(&p, 0, sizeof(p));
   p.w = w;
   p.partial = reinterpret_cast<float*>(at);
+  int* tickets = reinterpret_cast<int*>(at + partial_bytes(w, plan));
   p.wait_flag = attention_wait_flag(device);
   if (!p.wait_flag) return cudaErrorInvalidDevice;
   p.ksteps = (w.head_dim + 15) / 16;
@@ -1668,7 +1707,8 @@ cudaError_t tc_backward(const WindowParams& w, void* scratch, int device, cudaSt
   while (lanes * 8 < w.head_dim) lanes *= 2;
   const uint64_t threads = static_cast<uint64_t>(w.batch) * ql * h * lanes;
   auto delta = f32 ? window_delta_kernel<float> : window_delta_kernel<__nv_bfloat16>;
-  e = launch(delta, dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, stream, w, lanes);
+  e = launch(delta, dim3(static_cast<unsigned>((threads + 255) / 256)), dim3(256), 0, stream, w, lanes,
+             tickets, 4);
   if (e != cudaSuccess) return e;
 
   if (!operand_map(&p.s1, w, o[0], p.tile) || !operand_map(&p.s2, w, o[3], p.tile) ||
@@ -1676,6 +1716,7 @@ cudaError_t tc_backward(const WindowParams& w, void* scratch, int device, cudaSt
       !result_map(&p.out1, w, w.dq, ql, h))
     return cudaErrorInvalidValue;
   p.items = static_cast<int>(w.batch * h * ((ql + p.tile - 1) / p.tile));
+  p.ticket = tickets;
   e = f32    ? (wide ? launch_backward<false, 128, 3, 1>(p, device, stream)
                      : launch_backward<false, 64, 3, 2>(p, device, stream))
       : wide ? launch_backward<false, 128, 1, 4>(p, device, stream)
@@ -1688,9 +1729,11 @@ cudaError_t tc_backward(const WindowParams& w, void* scratch, int device, cudaSt
     return cudaErrorInvalidValue;
   p.items = static_cast<int>(w.batch * kh * p.head_parts *
                              (p.first_tiles * static_cast<uint64_t>(p.chunks) + p.tiles - p.first_tiles));
+  p.ticket = tickets + 1;
   // (the sums of dk and dv and their tiles' products, 512 columns, leave TMEM no room for the scores of
   // fp32 heads above 64: a launch each)
   if (f32 && wide && (e = launch_backward<true, 128, 3, 1, 2>(p, device, stream)) != cudaSuccess) return e;
+  if (f32 && wide) p.ticket = tickets + 2;
   e = f32    ? (wide ? launch_backward<true, 128, 3, 1, 1>(p, device, stream)
                      : launch_backward<true, 64, 3, 2>(p, device, stream))
       : wide ? launch_backward<true, 128, 1, 3>(p, device, stream)
