@@ -304,21 +304,22 @@ __device__ __forceinline__ void place_keys(const WindowParams& w, Item& it) {
   }
 }
 
+// The items' last rows first: they see the most keys.
 template <int QT, int BN>
 __device__ __forceinline__ Item item_of(const TcParams& p, int idx) {
   const WindowParams& w = p.w;
   Item it;
   int bh;
   if (QT == 2 && p.pair_heads) {
-    const int pairs = w.heads / 2, per = w.batch * pairs, t = idx / per;
-    bh = idx - t * per;
+    const int pairs = w.heads / 2, per = w.batch * pairs, t = p.tiles - 1 - idx / per;
+    bh = idx % per;
     it.b = bh / pairs;
     it.h[0] = (bh - it.b * pairs) * 2;
     it.h[1] = it.h[0] + 1;
     it.row[0] = it.row[1] = t * 128;
   } else {
-    const int per = w.batch * w.heads, t = idx / per;
-    bh = idx - t * per;
+    const int per = w.batch * w.heads, t = (p.tiles - 1) / QT - idx / per;
+    bh = idx % per;
     it.b = bh / w.heads;
     it.h[0] = it.h[1] = bh - it.b * w.heads;
     it.row[0] = t * 128 * QT;
@@ -327,7 +328,7 @@ __device__ __forceinline__ Item item_of(const TcParams& p, int idx) {
   place_keys<QT, BN>(w, it);
   return it;
 }
-// The item of one query tile: the last rows first (they see the most keys).
+// The item of one query tile, in the same order.
 template <int BN, int TILE>
 __device__ __forceinline__ Item item_of_tile(const WindowParams& w, int idx) {
   const int per = w.batch * w.heads, t = (w.q_len + TILE - 1) / TILE - 1 - idx / per;
