@@ -414,7 +414,8 @@ struct SparB200Rotary {
   int32_t* invalid; /* optional: set to 1 when a position lies outside the table; that token's   */
                     /* outputs are zeros and it adds nothing to a weight gradient                */
   struct SparB200Heads q, k;         /* inputs */
-  struct SparB200Heads q_out, k_out; /* outputs; may be the inputs themselves (same strides) */
+  struct SparB200Heads q_out, k_out; /* outputs; may be the inputs themselves (same strides), else  */
+                                     /* must not overlap them; no stride of zero over many indexes */
   /* norms of queries and keys */
   const float* q_weight; /* [head_dim] */
   const float* k_weight; /* [head_dim] */
@@ -452,15 +453,21 @@ struct SparCudaStatus spar_b200_qk_norm_rotary_backward(const struct SparB200Rot
 /*   out = softmax(scale q k^T over the visible keys) v,  lse = ln sum exp(scale q k^T).         */
 /* A row that sees nothing (padding behind lengths[b], a position below 0) gives zeros, lse =    */
 /* -infinity, and no gradient. Keys and values at or behind lengths[b] reach no result, whatever */
-/* they hold (a cache's unused slots may hold NaN). A NaN or infinity in a key or value below    */
-/* lengths[b] may also reach rows near those that see it.                                        */
+/* they hold (a cache's unused slots may hold NaN). A NaN in a key or value below lengths[b]      */
+/* makes the rows that see it NaN, and may also reach rows near those.                            */
+/* Outputs must not overlap inputs or one another; an output with a stride of zero over more than */
+/* one index is refused. bf16: products of bf16 operands (P and dS rounded to nearest) with fp32   */
+/* sums; fp32: as exact as fp32 products and sums (values below 2^-110 keep fewer bits). 16-byte   */
+/* aligned rows with head_dim a multiple of 8, at most 128, run on the tensor cores; up to 32 rows */
+/* of a head group (heads / kv_heads * q_len) run as a decoding step; everything else runs one     */
+/* warp per row. A bounded wait that runs out sets the flag of spar_b200_attention_error.          */
 struct SparB200WindowAttention {
   int dtype; /* SparB200Element of q, k, v, out and the gradients */
   uint64_t batch, q_len, kv_len, heads, kv_heads;
   uint64_t head_dim; /* 1 .. 256 */
   uint64_t window;   /* >= 1; at least kv_len: plain causal attention */
   uint64_t sinks;
-  double scale; /* > 0, or 0 for 1 / sqrt(head_dim) */
+  double scale; /* 1e-30 .. 1e30, or 0 for 1 / sqrt(head_dim) */
   const int32_t* lengths; /* [batch] keys of each sequence, clamped to 0 .. kv_len; NULL: kv_len */
   const int32_t* first;   /* [batch] position of each sequence's row 0; NULL: kv_len - q_len    */
   struct SparB200Heads q, k, v, out;

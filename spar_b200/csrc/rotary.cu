@@ -578,6 +578,9 @@ bool make_params(const SparB200Rotary* r, bool norm, bool backward, RotaryParams
       vec = vec && on16(views[x]->data) && views[x]->batch % v == 0 && views[x]->token % v == 0 &&
             views[x]->head % v == 0;
     }
+    const View& o = p.out[s];  // rows on one another (a stride of zero) would be written by many at once
+    if (tokens && ((r->batch > 1 && !o.batch) || (r->seq > 1 && !o.token) || (heads > 1 && !o.head)))
+      return false;
     if (norm && tokens && (!weight[s] || (reinterpret_cast<uintptr_t>(weight[s]) & 3))) return false;
     vec = vec && (!norm || on16(weight[s]));
     p.weight[s] = weight[s];

@@ -186,6 +186,11 @@ View view_of(const SparB200Heads& v, uint64_t batch, uint64_t tokens, uint64_t h
           heads > 1 ? v.head : 0};
 }
 
+// An output whose rows lie on one another (a stride of zero) would be written by many at once.
+bool shared_rows(const View& v, uint64_t batch, uint64_t tokens, uint64_t heads) {
+  return (batch > 1 && !v.batch) || (tokens > 1 && !v.token) || (heads > 1 && !v.head);
+}
+
 bool whole_elements(const SparB200Heads& v, int dtype) {
   return v.data && reinterpret_cast<uintptr_t>(v.data) % (dtype == SPAR_B200_FLOAT32 ? 4 : 2) == 0;
 }
@@ -198,7 +203,7 @@ bool valid_sizes(const SparB200WindowAttention* a) {
       a->heads >= most || a->kv_heads < 1 || a->kv_heads > a->heads || a->heads % a->kv_heads)
     return false;
   if (a->head_dim < 1 || a->head_dim > kMaxHeadDim || a->window < 1) return false;
-  if (!(a->scale >= 0.0) || !std::isfinite(a->scale)) return false;
+  if (a->scale != 0.0 && !(a->scale >= 1e-30 && a->scale <= 1e30)) return false;
   // rows and keys of all heads are numbered in 32 bits of warps and blocks
   if (a->batch * a->heads >= (1ull << 31)) return false;
   const uint64_t longest = a->q_len > a->kv_len ? a->q_len : a->kv_len;
@@ -224,6 +229,12 @@ bool make_params(const SparB200WindowAttention* a, bool backward, WindowParams& 
   w.dq = view_of(a->dq, a->batch, a->q_len, a->heads);
   w.dk = view_of(a->dk, a->batch, a->kv_len, a->kv_heads);
   w.dv = view_of(a->dv, a->batch, a->kv_len, a->kv_heads);
+  if (rows && (shared_rows(w.out, a->batch, a->q_len, a->heads) ||
+               (backward && shared_rows(w.dq, a->batch, a->q_len, a->heads))))
+    return false;
+  if (keys && backward && (shared_rows(w.dk, a->batch, a->kv_len, a->kv_heads) ||
+                           shared_rows(w.dv, a->batch, a->kv_len, a->kv_heads)))
+    return false;
   w.lse = a->lse;
   w.lengths = a->lengths;
   w.first = a->first;

@@ -520,10 +520,15 @@ __global__ void __launch_bounds__(kThreads) window_decode_mma_kernel(
   finish<T>(p, shared, kThreads / 32, 8 * RB, b, kh, row0, split);
 }
 
-// One CTA per row: the ranges' partials added in order.
+// One CTA per row: the ranges' partials, added in an order that depends on the sizes alone. Groups of
+// threads as wide as a head take every (number of groups)-th range.
+constexpr int kJoinThreads = 512;
 template <typename T>
-__global__ void __launch_bounds__(kThreads) window_join_kernel(const __grid_constant__ DecodeParams p) {
+__global__ void __launch_bounds__(kJoinThreads) window_join_kernel(const __grid_constant__ DecodeParams p,
+                                                                   int width) {
   pdl_begin();
+  extern __shared__ float weight[];  // [splits], then [kJoinThreads] sums
+  __shared__ float scratch[32];
   const WindowParams& w = p.w;
   const int row = blockIdx.x, bk = blockIdx.y;
   const int b = bk / w.kv_heads, kh = bk - b * w.kv_heads;
@@ -531,14 +536,27 @@ __global__ void __launch_bounds__(kThreads) window_join_kernel(const __grid_cons
   const int stride = w.head_dim + 2;
   const float* src = p.partial + (static_cast<uint64_t>(bk) * p.rows + row) * p.splits * stride;
   float top = -INFINITY, total = 0.f;
-  for (int s = 0; s < p.splits; ++s) top = fmaxf(top, src[s * stride + w.head_dim]);
+  for (int s = threadIdx.x; s < p.splits; s += kJoinThreads) top = fmaxf(top, src[s * stride + w.head_dim]);
+  top = block_max(top, scratch);
   const float base_m = top == -INFINITY ? 0.f : top;
-  for (int s = 0; s < p.splits; ++s)
-    total += src[s * stride + w.head_dim + 1] * ex2(src[s * stride + w.head_dim] - base_m);
-  for (int e = threadIdx.x; e < w.head_dim; e += kThreads) {
-    float o = 0.f;
-#pragma unroll 4
-    for (int s = 0; s < p.splits; ++s) o += src[s * stride + e] * ex2(src[s * stride + w.head_dim] - base_m);
+  for (int s = threadIdx.x; s < p.splits; s += kJoinThreads) {
+    const float f = ex2(src[s * stride + w.head_dim] - base_m);
+    weight[s] = f;
+    total += src[s * stride + w.head_dim + 1] * f;
+  }
+  total = block_sum(total, scratch);
+  __syncthreads();
+  const int e = threadIdx.x % width, group = threadIdx.x / width, groups = kJoinThreads / width;
+  float o = 0.f;
+  if (e < w.head_dim) {
+#pragma unroll 8
+    for (int s = group; s < p.splits; s += groups) o += src[s * stride + e] * weight[s];
+  }
+  float* sums = weight + p.splits;
+  sums[threadIdx.x] = o;
+  __syncthreads();
+  if (group == 0 && e < w.head_dim) {
+    for (int g = 1; g < groups; ++g) o += sums[g * width + e];
     put(row_out<T>(w.out, b, i, h) + e, total > 0.f || total != total ? o / total : 0.f);
   }
   if (threadIdx.x == 0 && w.lse)
@@ -575,7 +593,7 @@ DecodePlan decode_plan(const WindowParams& w, int device) {
   const int64_t keys = std::min<int64_t>(w.kv_len, static_cast<int64_t>(w.window) + w.q_len + w.sinks);
   const int64_t ctas = static_cast<int64_t>(w.batch) * w.kv_heads * d.row_blocks;
   const int64_t slots = sm_count(device) * std::min<int64_t>(3, (227 << 10) / (d.smem + 1024));
-  const int64_t most = std::max<int64_t>(1, std::min((4 * slots + ctas - 1) / ctas, keys / (2 * step)));
+  const int64_t most = std::max<int64_t>(1, std::min((2 * slots + ctas - 1) / ctas, keys / (2 * step)));
   int64_t best = INT64_MAX;
   d.splits = 1;
   for (int64_t n = 1; n <= most; ++n) {
@@ -595,7 +613,10 @@ cudaError_t launch_decode(void (*kernel)(DecodeParams), const DecodeParams& p, c
   if (p.partial) {
     e = launch(kernel, grid, dim3(kThreads), d.smem, stream, p);
     if (e != cudaSuccess) return e;
-    return launch(window_join_kernel<T>, dim3(p.rows, y), dim3(kThreads), 0, stream, p);
+    int width = 32;
+    while (width < p.w.head_dim) width *= 2;
+    return launch(window_join_kernel<T>, dim3(p.rows, y), dim3(kJoinThreads),
+                  (p.splits + kJoinThreads) * sizeof(float), stream, p, width);
   }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];

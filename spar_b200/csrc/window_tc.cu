@@ -121,6 +121,12 @@ __device__ __forceinline__ void registers_up() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
 }
 
+__device__ __forceinline__ float max_nan(float a, float b, float c) {  // NaN if one of them is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
 // Bits 0 .. n - 1 (none below 0, all from 32 on).
 __device__ __forceinline__ uint32_t below(int n) {
   return n >= 32 ? 0xffffffffu : (1u << max(n, 0)) - 1u;
@@ -645,10 +651,12 @@ __global__ void __launch_bounds__(128 + 128 * QT, 1) window_forward_kernel(
           for (int i = 0; i < 8; ++i) mxs[i] = -INFINITY;
 #pragma unroll
           for (int c = 0; c < BN; c += 2)
-            mxs[c / 2 & 7] = fmaxf(fmaxf(mxs[c / 2 & 7], __uint_as_float(v[c / 32][c % 32])),
-                                   __uint_as_float(v[c / 32][c % 32 + 1]));
-          const float mx = fmaxf(fmaxf(fmaxf(mxs[0], mxs[1]), fmaxf(mxs[2], mxs[3])),
-                                 fmaxf(fmaxf(mxs[4], mxs[5]), fmaxf(mxs[6], mxs[7]))) * p.scale_log2;
+            mxs[c / 2 & 7] = max_nan(mxs[c / 2 & 7], __uint_as_float(v[c / 32][c % 32]),
+                                     __uint_as_float(v[c / 32][c % 32 + 1]));
+          const float mx = max_nan(max_nan(mxs[0], mxs[1], mxs[2]), max_nan(mxs[3], mxs[4], mxs[5]),
+                                   max_nan(mxs[6], mxs[7], mxs[7])) * p.scale_log2;
+          // A score of +infinity or NaN makes the row NaN; the polynomial would not.
+          if (!(mx < INFINITY)) sum = __int_as_float(0x7fffffff);
           const bool move = m == -INFINITY ? mx > m : mx > m + kRescaleLog2;
           float f = 1.f;
           if (move) {
@@ -672,12 +680,14 @@ __global__ void __launch_bounds__(128 + 128 * QT, 1) window_forward_kernel(
             pending = f;
           }
           const float base_m = m == -INFINITY ? 0.f : m;
-          // Value rows behind the sequence may hold anything, and 0 times NaN is NaN: clear them.
-          if (key + BN > it.s.n && it.s.n < w.kv_len) {
+          // Value rows behind the sequence may hold anything, and 0 times NaN is NaN: clear them, and
+          // those behind the first tokens in their tiles, which every row visits.
+          const int held = min(it.s.n, j < it.ns ? w.sinks : w.kv_len) - key;
+          if (held < BN && key + held < w.kv_len) {
             const uint32_t st = (base + j) % VS;
             if (!(ok = wait_or_abort(v_full + st, (base + j) / VS, abort_flag))) break;
             uint8_t* vt = smem + L::kV + st * L::kKTile;
-            for (int i = (max(0, it.s.n - key)) * 8 + r; i < BN * 8; i += 128)
+            for (int i = max(0, held) * 8 + r; i < BN * 8; i += 128)
               for (int box = 0; box < NP * kBoxes; ++box)
                 *reinterpret_cast<uint4*>(vt + box * BN * 128 + i * 16) = make_uint4(0, 0, 0, 0);
             tc::fence_proxy_async_smem();
@@ -1244,7 +1254,7 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
           hi = min(upto - 1, pos < w.sinks ? kMoving : pos - base + w.window - 1);
         } else {
           key = key_of<kMoving>(q, i);
-          clear = min(s.n - key, kMoving);
+          clear = min(min(s.n, i < q.ns ? w.sinks : w.kv_len) - key, kMoving);
           hi = min(pos, s.n - 1) - key;
           if (i < q.ns) hi = min(hi, w.sinks - 1 - key);
           near = pos - w.window + 1 - key;
@@ -1330,8 +1340,9 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
             }
           }
         }
-        // Moving rows behind the sequence may hold anything, and 0 times NaN is NaN: clear them.
-        if (clear < kMoving && s.n < (KEYS ? s.p0 + w.q_len : w.kv_len)) {
+        // Moving rows behind the sequence may hold anything, and 0 times NaN is NaN: clear them (and the
+        // keys behind the first tokens in their tiles, which every row visits).
+        if (clear < kMoving && (KEYS ? s.n < s.p0 + w.q_len : key + clear < w.kv_len)) {
           if (!KEYS && !(ok = wait_or_abort(m_full + st, m / ST, abort_flag))) break;
           uint8_t* mt = smem + L::kB + st * 2 * L::kMov;
           for (int c = max(clear, 0) * 8 + (kTurns ? r : g * 128 + r); c < kMoving * 8; c += kTurns ? 128 : 256)
@@ -1593,12 +1604,16 @@ BackwardPlan backward_plan(const WindowParams& w, int device) {
   b.tile = w.dtype == SPAR_B200_FLOAT32 && w.head_dim > 64 ? 64 : 128;  // Bwd::kTile
   b.tiles = (w.kv_len + b.tile - 1) / b.tile;
   b.first_tiles = (std::min(w.sinks, w.kv_len) + b.tile - 1) / b.tile;
-  const int64_t rows = std::max<int64_t>(256, (static_cast<int64_t>(w.window) / 2 + 127) / 64 * 64);
-  b.chunk = static_cast<int>(std::min<int64_t>(rows, std::max(64, w.q_len)));
-  b.chunks = w.q_len > 0 ? (w.q_len + b.chunk - 1) / b.chunk : 1;
   const int64_t bk = static_cast<int64_t>(w.batch) * w.kv_heads, items = bk * b.tiles;
   b.head_parts = static_cast<int>(
       std::min<int64_t>(w.group, std::max<int64_t>(1, 2 * sm_count(device) / std::max<int64_t>(1, items))));
+  // About 1024 items at most come from cutting (first tokens may be many: whole tiles then suffice).
+  const int64_t most =
+      std::max<int64_t>(1, 1024 / std::max<int64_t>(1, bk * b.first_tiles * b.head_parts));
+  const int64_t rows = std::max<int64_t>(
+      {256, (static_cast<int64_t>(w.window) / 2 + 127) / 64 * 64, (w.q_len + most - 1) / most});
+  b.chunk = static_cast<int>(std::min<int64_t>(rows, std::max(1, w.q_len)));
+  b.chunks = (w.q_len + b.chunk - 1) / b.chunk;
   b.slots = 0;
   const uint64_t first_parts = static_cast<uint64_t>(b.chunks) * b.head_parts;
   if (first_parts > 1) b.slots += bk * b.first_tiles * first_parts;

@@ -125,7 +125,9 @@ def test_rotary_and_window_attention_refuse_bad_calls_without_gpu():
     at = 1 << 20  # never dereferenced: validation fails first
 
     def rotary(**k):
-        base = dict(dtype=0, layout=1, batch=2, seq=3, heads=4, kv_heads=2, head_dim=64, rotary_dim=32,
+        strides = {f"{n}_{part}": x for n in ("q", "k", "q_out", "k_out", "dq", "dk")
+                   for part, x in (("batch", 1024), ("token", 256), ("head", 64))}
+        base = dict(strides, dtype=0, layout=1, batch=2, seq=3, heads=4, kv_heads=2, head_dim=64, rotary_dim=32,
                     table=at, table_rows=3, q=at, k=at, q_out=at, k_out=at, q_weight=at, k_weight=at,
                     epsilon=1e-6, dq=at, dk=at, dq_weight=at, dk_weight=at, scratch=at)
         return ctypes.byref(_lib.SparB200Rotary(**{**base, **k}))
@@ -133,7 +135,8 @@ def test_rotary_and_window_attention_refuse_bad_calls_without_gpu():
     for bad in (dict(dtype=2), dict(layout=2), dict(head_dim=0), dict(head_dim=257), dict(rotary_dim=31),
                 dict(rotary_dim=66), dict(rotary_dim=0), dict(heads=0), dict(table=None), dict(q=None),
                 dict(k_out=None), dict(table_rows=2), dict(start=1), dict(start=2 ** 64 - 1), dict(q=at + 2),
-                dict(batch=1 << 20, seq=1 << 20), dict(batch=1 << 40, seq=1 << 40)):
+                dict(batch=1 << 20, seq=1 << 20), dict(batch=1 << 40, seq=1 << 40),
+                dict(q_out_token=0), dict(k_out_head=0)):  # rows of an output on one another
         assert lib.spar_b200_rotary(rotary(**bad), 0, None).code == 1, bad
         assert lib.spar_b200_qk_norm_rotary_forward(rotary(**bad), 0, None).code == 1, bad
         assert lib.spar_b200_qk_norm_rotary_backward(rotary(**bad), 0, None).code == 1, bad
@@ -150,7 +153,9 @@ def test_rotary_and_window_attention_refuse_bad_calls_without_gpu():
     assert lib.spar_b200_rotary_table(None, 0, 32, 1e4, 0, None, 0, None).code == 0
 
     def window(**k):
-        base = dict(dtype=1, batch=2, q_len=3, kv_len=5, heads=4, kv_heads=2, head_dim=64, window=4,
+        strides = {f"{n}_{part}": x for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")
+                   for part, x in (("batch", 2048), ("token", 256), ("head", 64))}
+        base = dict(strides, dtype=1, batch=2, q_len=3, kv_len=5, heads=4, kv_heads=2, head_dim=64, window=4,
                     sinks=1, q=at, k=at, v=at, out=at, lse=at, dout=at, dq=at, dk=at, dv=at, scratch=at)
         return ctypes.byref(_lib.SparB200WindowAttention(**{**base, **k}))
 
@@ -158,10 +163,12 @@ def test_rotary_and_window_attention_refuse_bad_calls_without_gpu():
                 dict(head_dim=0), dict(head_dim=257), dict(window=0), dict(scale=-1.0),
                 dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None), dict(k=at + 1),
                 dict(q_len=1 << 29), dict(kv_len=1 << 40), dict(batch=1 << 29, heads=64, kv_heads=64),
-                dict(batch=1 << 12, kv_len=1 << 20)):
+                dict(batch=1 << 12, kv_len=1 << 20), dict(scale=1e-31), dict(scale=1e31), dict(out_batch=0),
+                dict(out_token=0), dict(out_head=0)):
         assert lib.spar_b200_window_attention_forward(window(**bad), 0, None).code == 1, bad
         assert lib.spar_b200_window_attention_backward(window(**bad), 0, None).code == 1, bad
-    for bad in (dict(dout=None), dict(lse=None), dict(dv=None), dict(scratch=None), dict(scratch=at + 16)):
+    for bad in (dict(dout=None), dict(lse=None), dict(dv=None), dict(scratch=None), dict(scratch=at + 16),
+                dict(dq_token=0), dict(dk_head=0), dict(dv_batch=0)):
         assert lib.spar_b200_window_attention_backward(window(**bad), 0, None).code == 1, bad
     assert lib.spar_b200_window_attention_forward(window(batch=0, q=None, k=None), 0, None).code == 0
     assert lib.spar_b200_window_attention_forward(window(q_len=0, q=None, out=None), 0, None).code == 0
@@ -170,6 +177,13 @@ def test_rotary_and_window_attention_refuse_bad_calls_without_gpu():
     for none in (dict(batch=0), dict(q_len=0), dict(kv_len=0), dict(q_len=0, kv_len=0)):
         for backward in (0, 1):  # no division by a count of zero
             assert lib.spar_b200_window_attention_scratch_bytes(window(**none), backward, 0) < 1 << 20
+    # Partial sums stay within a quarter of a GB however many first tokens and rows there are.
+    for size in (dict(sinks=4), dict(sinks=1 << 16), dict(sinks=1 << 16, batch=16), dict(sinks=1 << 16, window=1 << 20),
+                 dict(sinks=200, heads=64, kv_heads=1, batch=1), dict(sinks=4, kv_len=130)):
+        size = dict(q_len=1 << 16, kv_len=1 << 16) | size
+        rows = size.get("batch", 2) * size.get("heads", 4) * size["q_len"] * 4
+        got = lib.spar_b200_window_attention_scratch_bytes(window(**size), 1, 0)
+        assert rows <= got <= rows + (1 << 28), (size, got)
 
 
 def test_new_structures_mirror_the_header():

@@ -112,6 +112,9 @@ CACHE = [
     (2, 1, 300, 6, 3, 96, 100, 3),
     (1, 2, 500, 3, 1, 50, 100, 3),
     (2, 1, 700, 2, 1, 256, 300, 4),
+    (1, 1, 9001, 2, 1, 128, 9001, 0),   # ranges joined by a launch of their own
+    (1, 1, 5003, 3, 3, 32, 4000, 70),
+    (1, 1, 3001, 2, 2, 256, 2500, 4),
     (1, 40, 900, 4, 2, 64, 300, 4),     # a chunk of a prompt
     (1, 200, 700, 4, 2, 128, 130, 4),
 ]
@@ -149,6 +152,35 @@ def test_positions_of_the_first_row(cuda):
             _check(q, k, v, 50, 3, dout, first=torch.tensor(first, dtype=torch.int32, device=cuda))
             if t > n:
                 _check(q, k, v, 50, 3, dout)  # default: the first rows stand before position 0
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128, 20])
+def test_nan_in_a_visible_key_or_value(cuda, dim, dtype):
+    """It makes every row that sees it NaN, whichever column of a tile it falls on, and no row of
+    another head or sequence, nor one far behind the window."""
+    from spar_b200 import ops
+
+    g = torch.Generator(device=cuda)
+    g.manual_seed(21)
+    for place in range(100, 108):
+        for part in (1, 2):
+            q, k, v = (x.clone() for x in _packed(cuda, g, dtype, 2, 700, 2, 2, dim))
+            (k if part == 1 else v)[0, place, 0] = math.nan
+            out, lse = ops.window_attention_forward(q, k, v, 90, 2)
+            seen = out[0, place:place + 90, 0]
+            assert bool(torch.isnan(seen).all()), (place, part)
+            if part == 1:
+                assert bool(torch.isnan(lse[0, 0, place:place + 90]).all())
+            assert bool(torch.isfinite(out[0, :, 1]).all() and torch.isfinite(out[1]).all())
+            assert bool(torch.isfinite(out[0, place + 90 + 256:, 0]).all())
+            one, one_lse = ops.window_attention_forward(q[:, :1], k[:, :place + 20], v[:, :place + 20], 90, 2)
+            assert bool(torch.isnan(one[0, 0, 0]).all() and torch.isfinite(one[0, 0, 1]).all())
+            grads = ops.window_attention_backward(torch.ones_like(q), q, k, v, torch.nan_to_num(out),
+                                                  torch.nan_to_num(lse), 90, 2)
+            assert bool(torch.isfinite(grads[0][0, place + 90 + 256:, 0]).all())
+            for x in grads:
+                assert bool(torch.isfinite(x[0, :, 1]).all() and torch.isfinite(x[1]).all())
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -226,6 +258,34 @@ def test_repeats_streams_and_captured_graphs(cuda):
     for (_, held), e, w in zip(graphs, eager, want):
         assert all(torch.equal(a, b) for a, b in zip(held, w))
         assert all(torch.equal(a, b) for a, b in zip(e, w))
+
+
+def test_first_call_of_a_process_may_be_captured():
+    """Nothing needs a call outside a capture first (the kernels' set-up is not stream work)."""
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from spar_b200 import ops
+q = torch.randn(2, 200, 4, 64, device="cuda").bfloat16()
+k, one = torch.randn_like(q[:, :, :2]), torch.randn(2, 1, 4, 64, device="cuda").bfloat16()
+w, table = torch.ones(64, device="cuda"), torch.zeros(200, 32, 2, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+def block():
+    a, b = ops.qk_norm_rotary_forward(q, k, w, w, table)
+    out, lse = ops.window_attention_forward(a, b, k, 50, 4)
+    return (out, *ops.window_attention_backward(out, a, b, k, out, lse, 50, 4),
+            *ops.window_attention_forward(one, b, k, 50, 4), ops.rotary_table(9, 64, device="cuda"))
+with torch.cuda.graph(graph):
+    held = block()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(x, y) for x, y in zip(held, block()))
+"""
+    run = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr[-2000:]
 
 
 def test_nothing_to_do(cuda):
