@@ -858,7 +858,7 @@ template <bool KEYS, int DH, int NP, int ST, int OUT>
 struct Bwd {
   // Buffers of S and dP: three where TMEM has room, so that the two softmax groups find their next
   // scores ready; not more than stages, as scores run that far ahead of the last use of a stage.
-  static constexpr int kBuffers = NP > 1 ? (KEYS || ST == 1 ? 1 : 2) : KEYS && DH == 128 ? 2 : 3;
+  static constexpr int kBuffers = NP > 1 ? (ST == 1 ? 1 : 2) : KEYS && DH == 128 ? 2 : 3;
   static_assert(kBuffers <= ST, "stages");
   static constexpr uint32_t kStats = NP == 1 && DH == 64 ? 2 : 1;  // pairs of stationary operands
   // Stationary rows. Three planes of two operands of 128 columns leave room for 64 of the 128 rows of a
@@ -883,13 +883,12 @@ struct Bwd {
   static constexpr uint32_t kSmem = kBar + 320 + 1024;
   static_assert((21 + 2 * ST) * 8 + 24 <= 320, "backward barriers");
   static_assert(kSmem <= kMaxSmem, "backward shared memory");
-  // TMEM: buffers of S | dP (| the third planes of P and dS), then the products' sums, then
-  // (NP = 3) the sums of earlier tiles.
+  // TMEM: buffers of S | dP (| the third planes of P and dS), then the products' sums: of the item, or
+  // (NP = 3) of a tile, whose sum over tiles the softmax threads keep.
   static constexpr uint32_t kBuf = KEYS && NP > 1 ? 192 : 128;
   static constexpr uint32_t kAcc = kBuffers * kBuf;
   static constexpr uint32_t kOuts = KEYS && OUT == 0 ? 2 : 1;
-  static constexpr uint32_t kSum = kAcc + kOuts * DH;
-  static_assert(kAcc + kOuts * DH * (NP > 1 ? 2 : 1) <= kTmemCols, "backward TMEM");
+  static_assert(kAcc + kOuts * DH <= kTmemCols, "backward TMEM");
 };
 
 // Column (in a buffer) of plane pl of K step ks of the operand that overwrites S (which = 0) or dP
@@ -1194,20 +1193,18 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
     const uint64_t scale = both(p.scale_log2, p.scale_log2);
     uint32_t mn = 0, sums = 0;
     bool ok = true;
-    // NP = 3: adds the last tile's products to the sums of the earlier ones; the groups share the
-    // columns.
+    // NP = 3: the sums over tiles of this thread's row, the groups share the columns; add_sums adds the
+    // last tile's products.
+    constexpr int kSums = NP > 1 ? L::kOuts * DH / 2 : 32;
+    [[maybe_unused]] float tile_sums[kSums];
     auto add_sums = [&](bool first) {
-      constexpr int cols = L::kOuts * DH / 2;
-#pragma unroll 1
-      for (int c = g * cols; c < (g + 1) * cols; c += 32) {
-        uint32_t o[32], a[32];
-        tc::tmem_load_2x32(lanes + L::kAcc + c, lanes + L::kSum + c, o, a);
-        if (!first) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e)
-            o[e] = __float_as_uint(__uint_as_float(a[e]) + __uint_as_float(o[e]));
-        }
-        tc::tmem_store_32x32(lanes + L::kSum + c, o);
+      for (int c = 0; c < kSums; c += 32) {
+        uint32_t o[32];
+        tc::tmem_load_32x32(lanes + L::kAcc + g * kSums + c, o);
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          tile_sums[c + e] = first ? __uint_as_float(o[e]) : tile_sums[c + e] + __uint_as_float(o[e]);
       }
     };
     for (uint32_t tn = 0; ok; ++tn) {
@@ -1376,16 +1373,22 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
       constexpr bool kBoth = KEYS && OUT == 0;
       constexpr int cols = NP == 1 && L::kOuts * DH == 64 ? 64 : L::kOuts * DH / 2;
       const int out = kBoth ? g : OUT == 2;
-      const uint32_t from = lanes + (NP > 1 ? L::kSum : L::kAcc) + g * cols;
+      const uint32_t from = lanes + L::kAcc + g * cols;
       const float factor = KEYS && out ? 1.f : w.scale;
       const int warp_row = row - lane;
-#pragma unroll 1
-      for (int c = 0; c < cols && g * cols < static_cast<int>(L::kOuts) * DH; c += 32) {
+#pragma unroll(NP > 1 ? cols / 32 : 1)
+      for (int c = 0; c < cols; c += 32) {
+        if (g * cols >= static_cast<int>(L::kOuts) * DH) break;
         float o[32];
-        uint32_t u[32];
-        if (n) tc::tmem_load_32x32(from + c, u);
+        if constexpr (NP > 1) {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) o[e] = n ? __uint_as_float(u[e]) * factor : 0.f;
+          for (int e = 0; e < 32; ++e) o[e] = n ? tile_sums[c + e] * factor : 0.f;
+        } else {
+          uint32_t u[32];
+          if (n) tc::tmem_load_32x32(from + c, u);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = n ? __uint_as_float(u[e]) * factor : 0.f;
+        }
         const int col = kBoth ? c : g * cols + c;
         if (r - lane >= L::kTile) continue;
         if (KEYS && k.slot >= 0) {
