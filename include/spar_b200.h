@@ -414,15 +414,17 @@ struct SparB200Rotary {
   int32_t* invalid; /* optional: set to 1 when a position lies outside the table; that token's   */
                     /* outputs are zeros and it adds nothing to a weight gradient                */
   struct SparB200Heads q, k;         /* inputs */
-  struct SparB200Heads q_out, k_out; /* outputs; may be the inputs themselves (same strides), else  */
-                                     /* must not overlap them; no stride of zero over many indexes */
+  struct SparB200Heads q_out, k_out; /* outputs; may be their own inputs (same strides), else must  */
+                                     /* not overlap inputs or one another (refused where they      */
+                                     /* start at the same element); no stride of zero over many    */
+                                     /* indexes                                                    */
   /* norms of queries and keys */
   const float* q_weight; /* [head_dim] */
   const float* k_weight; /* [head_dim] */
   double epsilon;
   /* their backward: gradients of the forward's outputs, weight gradients, scratch */
   struct SparB200Heads dq, dk;
-  float* dq_weight; /* [head_dim] */
+  float* dq_weight; /* [head_dim]; must not overlap */
   float* dk_weight;
   int accumulate; /* 1: add to dq_weight and dk_weight instead of overwriting them */
   void* scratch;  /* spar_b200_qk_norm_rotary_scratch_bytes(head_dim, device) bytes, 16-byte     */
@@ -454,13 +456,15 @@ struct SparCudaStatus spar_b200_qk_norm_rotary_backward(const struct SparB200Rot
 /* A row that sees nothing (padding behind lengths[b], a position below 0) gives zeros, lse =    */
 /* -infinity, and no gradient. Keys and values at or behind lengths[b] reach no result, whatever */
 /* they hold (a cache's unused slots may hold NaN). A NaN in a key or value below lengths[b]      */
-/* makes the rows that see it NaN, and may also reach rows near those.                            */
-/* Outputs must not overlap inputs or one another; an output with a stride of zero over more than */
-/* one index is refused. bf16: products of bf16 operands (P and dS rounded to nearest) with fp32   */
-/* sums; fp32: as exact as fp32 products and sums (values below 2^-110 keep fewer bits). 16-byte   */
-/* aligned rows with head_dim a multiple of 8, at most 128, run on the tensor cores; up to 32 rows */
-/* of a head group (heads / kv_heads * q_len) run as a decoding step; everything else runs one     */
-/* warp per row. A bounded wait that runs out sets the flag of spar_b200_attention_error.          */
+/* makes the rows that see it NaN, and may also reach rows near those. Infinities follow the       */
+/* formula, but fp32 on the tensor cores may take them as NaN.                                    */
+/* Outputs must not overlap inputs or one another (refused where they start at the same element);  */
+/* an output with a stride of zero over more than one index is refused.                          */
+/* bf16: products of bf16 operands (P and dS rounded to nearest) with fp32 sums; fp32: as exact as */
+/* fp32 products and sums (values below 2^-110 keep fewer bits). 16-byte aligned rows with head_dim */
+/* a multiple of 8, at most 128, run on the tensor cores; up to 32 rows of a head group (heads /   */
+/* kv_heads * q_len) run as a decoding step; everything else runs one warp per row. A bounded wait */
+/* that runs out sets the flag of spar_b200_attention_error.                                      */
 struct SparB200WindowAttention {
   int dtype; /* SparB200Element of q, k, v, out and the gradients */
   uint64_t batch, q_len, kv_len, heads, kv_heads;

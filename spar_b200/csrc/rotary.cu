@@ -487,10 +487,11 @@ __global__ void __launch_bounds__(1024) qk_weight_partials_kernel(float* dq, flo
   if (x == 0 && c < head_dim && d) d[c] = accumulate ? d[c] + s : s;
 }
 
-// One thread per (pair, run of positions): the first angle's cos and sin, then rotations by one position in double (each adds ~2^-52, far below the fp32 result's 2^-25),
-// which turns ~100 double operations per entry into four and leaves the launch bound by its
-// stores.
-// The run is as long as leaves 32768 threads, 8 to 128 positions.
+// One thread per (pair, run of positions): the first angle's cos and sin, then rotations by one
+// position in double (each adds ~2^-52, far below the fp32 result's 2^-25): four double operations
+// per entry instead of ~100. The run is as long as leaves 32768 threads, 8 to 128 positions: 131072
+// positions of 64 pairs take 16 us of which the stores' floor is 10 (runs of 128 left a shorter
+// table's few threads with the latency of 128 steps: 4096 positions 21 us, in runs of 8 9 us).
 __global__ void __launch_bounds__(256) rotary_table_kernel(float2* table, uint64_t rows,
                                                            uint32_t pairs, uint64_t start, uint32_t length,
                                                            SparB200RotaryScaling sc, double theta) {
@@ -524,6 +525,7 @@ __global__ void __launch_bounds__(256) rotary_table_kernel(float2* table, uint64
 
 // ------------------------------------------------------------------------------- host side
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+bool on4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
 
 // Strides over a single index never count, so that they cannot spoil the alignment rule.
 View view_of(const SparB200Heads& v, uint64_t batch, uint64_t seq, uint64_t heads) {
@@ -555,7 +557,13 @@ bool make_params(const SparB200Rotary* r, bool norm, bool backward, RotaryParams
     return false;
   if (norm && !(r->epsilon >= 0.0 && r->epsilon <= 1e30)) return false;
   if (backward && (!r->dq_weight || !r->scratch || !on16(r->scratch))) return false;
-  if (backward && r->kv_heads && !r->dk_weight) return false;
+  if (backward && r->kv_heads) {
+    if (!r->dk_weight) return false;
+    const int64_t apart = r->dq_weight - r->dk_weight;  // both are written whole
+    if (apart < static_cast<int64_t>(r->head_dim) && -apart < static_cast<int64_t>(r->head_dim)) return false;
+  }
+  if (!on4(r->positions) || !on4(r->invalid) || (backward && (!on4(r->dq_weight) || !on4(r->dk_weight))))
+    return false;
   p = RotaryParams{};
   const uint64_t tokens = r->batch * r->seq;
   const int sides = r->kv_heads ? 2 : 1;
@@ -581,10 +589,20 @@ bool make_params(const SparB200Rotary* r, bool norm, bool backward, RotaryParams
     const View& o = p.out[s];  // rows on one another (a stride of zero) would be written by many at once
     if (tokens && ((r->batch > 1 && !o.batch) || (r->seq > 1 && !o.token) || (heads > 1 && !o.head)))
       return false;
-    if (norm && tokens && (!weight[s] || (reinterpret_cast<uintptr_t>(weight[s]) & 3))) return false;
+    if (norm && tokens && (!weight[s] || !on4(weight[s]))) return false;
     vec = vec && (!norm || on16(weight[s]));
     p.weight[s] = weight[s];
   }
+  // In place is element by element: the same data with the same strides, on its own side.
+  for (int s = 0; tokens && s < sides; ++s)
+    for (int other = 0; other < sides; ++other)
+      for (const View* v : {&p.in[other], backward ? &p.grad[other] : nullptr}) {
+        const View& o = p.out[s];
+        if (v && v->data == o.data &&
+            (other != s || v->batch != o.batch || v->token != o.token || v->head != o.head))
+          return false;
+      }
+  if (tokens && sides == 2 && p.out[0].data == p.out[1].data) return false;
   if (tokens && !r->positions && (r->table_rows < r->seq || r->start > r->table_rows - r->seq))
     return false;
   if (tokens && (!r->table || (reinterpret_cast<uintptr_t>(r->table) & 7))) return false;

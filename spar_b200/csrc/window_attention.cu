@@ -70,13 +70,13 @@ __global__ void __launch_bounds__(kRowWarps * 32) row_forward_kernel(
       load_row<T, E>(v, row_ptr<T>(w.v, b, j, kh), w.head_dim, lane);
       const float x = dot_row<E>(q, k) * w.scale;
       if (x > top) {
-        const float f = expf(top - x);
+        const float f = expf(top - x);  // (0 for the first key)
         sum *= f;
 #pragma unroll
         for (int e = 0; e < E; ++e) acc[e] *= f;
         top = x;
       }
-      const float pr = expf(x - top);
+      const float pr = expf(x - (top == -INFINITY ? 0.f : top));
       sum += pr;
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] += pr * v[e];
@@ -186,6 +186,8 @@ View view_of(const SparB200Heads& v, uint64_t batch, uint64_t tokens, uint64_t h
           heads > 1 ? v.head : 0};
 }
 
+bool whole_words(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
+
 // An output whose rows lie on one another (a stride of zero) would be written by many at once.
 bool shared_rows(const View& v, uint64_t batch, uint64_t tokens, uint64_t heads) {
   return (batch > 1 && !v.batch) || (tokens > 1 && !v.token) || (heads > 1 && !v.head);
@@ -235,6 +237,19 @@ bool make_params(const SparB200WindowAttention* a, bool backward, WindowParams& 
   if (keys && backward && (shared_rows(w.dk, a->batch, a->kv_len, a->kv_heads) ||
                            shared_rows(w.dv, a->batch, a->kv_len, a->kv_heads)))
     return false;
+  if (!whole_words(a->lse) || !whole_words(a->lengths) || !whole_words(a->first)) return false;
+  // Outputs are written while other rows' inputs are still read (other overlaps are the caller's to
+  // avoid: views of one packed buffer interleave).
+  const char* in[5] = {rows ? w.q.data : nullptr, keys ? w.k.data : nullptr, keys ? w.v.data : nullptr,
+                       backward && rows ? w.dout.data : nullptr, backward && rows ? w.out.data : nullptr};
+  const char* out[3] = {rows ? (backward ? w.dq.data : w.out.data) : nullptr,
+                        backward && keys ? w.dk.data : nullptr, backward && keys ? w.dv.data : nullptr};
+  for (int i = 0; i < 3; ++i) {
+    for (const char* p : in)
+      if (out[i] && out[i] == p) return false;
+    for (int j = 0; j < i; ++j)
+      if (out[i] && out[i] == out[j]) return false;
+  }
   w.lse = a->lse;
   w.lengths = a->lengths;
   w.first = a->first;

@@ -97,6 +97,12 @@ __device__ __forceinline__ Range range_of(const WindowParams& w, const Sequence&
   return r;
 }
 
+// Whether row i sees a key (then its own).
+__device__ __forceinline__ bool sees_any(const WindowParams& w, int b, int i) {
+  const Sequence s = sequence_of(w, b);
+  return s.p0 + i >= 0 && s.p0 + i < s.n;
+}
+
 // Shared-memory address of `p` in CTA `rank` of the cluster, and a load from there.
 __device__ __forceinline__ float load_from(const float* p, uint32_t rank) {
   float v;
@@ -160,7 +166,7 @@ __device__ __forceinline__ void finish(const DecodeParams& p, float* shared, int
       total += load_from(at + w.head_dim + 1, k) * f;
       o += load_from(at + e, k) * f;
     }
-    put(row_out<T>(w.out, b, i, h) + e, total > 0.f || total != total ? o / total : 0.f);
+    put(row_out<T>(w.out, b, i, h) + e, sees_any(w, b, i) ? o / total : 0.f);
     if (e == 0 && w.lse)
       w.lse[(static_cast<uint64_t>(b) * w.heads + h) * w.q_len + i] = base_m * kLn2 + logf(total);
   }
@@ -557,7 +563,7 @@ __global__ void __launch_bounds__(kJoinThreads) window_join_kernel(const __grid_
   __syncthreads();
   if (group == 0 && e < w.head_dim) {
     for (int g = 1; g < groups; ++g) o += sums[g * width + e];
-    put(row_out<T>(w.out, b, i, h) + e, total > 0.f || total != total ? o / total : 0.f);
+    put(row_out<T>(w.out, b, i, h) + e, sees_any(w, b, i) ? o / total : 0.f);
   }
   if (threadIdx.x == 0 && w.lse)
     w.lse[(static_cast<uint64_t>(b) * w.heads + h) * w.q_len + i] = base_m * kLn2 + logf(total);
@@ -596,9 +602,13 @@ DecodePlan decode_plan(const WindowParams& w, int device) {
   const int64_t most = std::max<int64_t>(1, std::min((2 * slots + ctas - 1) / ctas, keys / (2 * step)));
   int64_t best = INT64_MAX;
   d.splits = 1;
-  for (int64_t n = 1; n <= most; ++n) {
-    const int64_t cost = (ctas * n + slots - 1) / slots * ((keys + n - 1) / n + 96);
-    if (cost < best) best = cost, d.splits = static_cast<int>(n);
+  for (int64_t rounds = (ctas + slots - 1) / slots; rounds <= (ctas * most + slots - 1) / slots; ++rounds) {
+    // the most ranges of so many rounds, or fewer that are as long
+    const int64_t longest = std::max<int64_t>(1, (keys + most - 1) / most);
+    const int64_t n_most = std::max<int64_t>(1, std::min(most, rounds * slots / ctas));
+    const int64_t range = std::max(longest, (keys + n_most - 1) / n_most);
+    const int64_t cost = rounds * (range + 96);
+    if (cost < best) best = cost, d.splits = static_cast<int>(std::max<int64_t>(1, (keys + range - 1) / range));
   }
   return d;
 }

@@ -205,17 +205,13 @@ __device__ __forceinline__ void weights32(const uint32_t (&s)[32], uint64_t scal
   }
 }
 
-// 64 consecutive values of a row as bf16 operand columns: one plane rounded to nearest (NP = 1:
-// half a step of bf16, as the stored results have), or three planes that hold all 24 bits.
-template <int NP, int N>
-__device__ __forceinline__ void store_planes(uint32_t taddr, uint32_t plane_cols, float (&v)[N]) {
-  static_assert(N == 64, "one pair of 32-column stores");
+// 64 consecutive values of a row as three planes of 32 bf16 operand columns.
+__device__ __forceinline__ void store_planes(uint32_t taddr, uint32_t plane_cols, float (&v)[64]) {
 #pragma unroll
-  for (int pl = 0; pl < NP; ++pl) {
+  for (int pl = 0; pl < 3; ++pl) {
     uint32_t r[32];
 #pragma unroll
-    for (int e = 0; e < 32; ++e)
-      r[e] = NP == 1 ? pack_bf16(v[2 * e], v[2 * e + 1]) : take_upper(v[2 * e], v[2 * e + 1]);
+    for (int e = 0; e < 32; ++e) r[e] = take_upper(v[2 * e], v[2 * e + 1]);
     tc::tmem_store_32x32(taddr + pl * plane_cols, r);
   }
 }
@@ -720,7 +716,7 @@ __global__ void __launch_bounds__(128 + 128 * QT, 1) window_forward_kernel(
               pr[c] = ex2(fmaf(__uint_as_float(v[c / 32][c % 32]), p.scale_log2, -base_m));
               sums[c & 3] += pr[c];
             }
-            store_planes<NP, 64>(lanes, BN / 2, pr);
+            store_planes(lanes, BN / 2, pr);
             sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
             tc::tc_fence_before();
             __syncwarp();
@@ -734,7 +730,8 @@ __global__ void __launch_bounds__(128 + 128 * QT, 1) window_forward_kernel(
       }
       base += it.n;
       const bool stored = row + r < w.q_len;
-      const float inv = valid ? 1.f / sum : 0.f;
+      // (a row that sees scores of -infinity alone is 0 / 0, whatever the polynomial makes of them)
+      const float inv = !valid ? 0.f : m == -INFINITY ? __int_as_float(0x7fffffff) : 1.f / sum;
 #pragma unroll 1
       for (int c = 0; c < DH / 32; ++c) {
         float o[32];
@@ -785,8 +782,8 @@ __global__ void __launch_bounds__(128 + 128 * QT, 1) window_forward_kernel(
 //       every query head of the group: S^T = k q^T, dP^T = v dout^T;  dv += P^T dout;  dk += dS^T q
 // P = exp(S - lse) is recomputed on both sides, so every gradient element is summed in one CTA and
 // no order is left to chance. P and dS replace S and dP in TMEM and are read there as the A operand.
-// With two buffers of S and dP the next tile's products run meanwhile. `scale` is applied to dq and dk
-// at the end.
+// With two or three buffers of S and dP the next tiles' products run meanwhile. `scale` is applied to
+// dq and dk at the end.
 // First tokens are seen by every later row: their key tiles' rows are cut into chunks of
 // `chunk` rows that are items of their own (and, where there are few key tiles, so are groups of
 // query heads); such items leave fp32 partial sums that a last launch adds in order.
@@ -1063,7 +1060,7 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
               }
           }
           if constexpr (KEYS) {
-  const uint64_t at = (static_cast<uint64_t>(b) * w.heads + h) * w.q_len;
+            const uint64_t at = (static_cast<uint64_t>(b) * w.heads + h) * w.q_len;
 #pragma unroll
             for (int e = lane; e < kMoving; e += 32) {
               const bool in = row + e < k.end;
@@ -1096,8 +1093,8 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
         const uint32_t idesc_s = tc::idesc_bf16(128, kMoving, 0, 0);
         const uint32_t idesc_o = tc::idesc_bf16(128, 16 * p.ksteps, 0, 1);
         const uint32_t a_addr = tc::smem_u32(smem + L::kA), b_addr = tc::smem_u32(smem + L::kB);
-      [[maybe_unused]] const uint32_t ones = tc::smem_u32(smem + L::kOnes),
-                                      stats = tc::smem_u32(smem + L::kRows);
+        [[maybe_unused]] const uint32_t ones = tc::smem_u32(smem + L::kOnes),
+                                        stats = tc::smem_u32(smem + L::kRows);
         uint32_t an = 0, mn = 0, sums = 0;
         bool ok = true;
         // S and dP of moving tile number m; after the item's last one the stationary operands are free.
@@ -1110,11 +1107,11 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
             const uint32_t a = kmajor_low(a_addr + (2 * (an % L::kStats) + half) * L::kStat),
                            b = kmajor_low(b_addr + (2 * st + half) * L::kMov);
             uint32_t acc = 0;
-          if constexpr (L::kAugment) {
-            tc::mma_f16(buf + half * 64, core_desc(ones), core_desc(stats + st * L::kRowsBytes + half * 2048), idesc_s,
-                        0);
-            acc = 1;
-          }
+            if constexpr (L::kAugment) {
+              tc::mma_f16(buf + half * 64, core_desc(ones),
+                          core_desc(stats + st * L::kRowsBytes + half * 2048), idesc_s, 0);
+              acc = 1;
+            }
 #pragma unroll
             for (int pr = 0; pr < kProducts<NP>; ++pr)
 #pragma unroll
@@ -1154,7 +1151,7 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
               // queries: dq += dS k; keys: dk += dS^T q, dv += P^T dout
               const int operand = OUT == 2 ? 1 : out, which = KEYS ? 1 - operand : 0;
               const uint32_t b = mnmajor_low(b_addr + (2 * st + operand) * L::kMov, kMoving);
-            uint32_t acc = NP == 1 && i > 0;
+              uint32_t acc = NP == 1 && i > 0;
 #pragma unroll
               for (int pr = 0; pr < kProducts<NP>; ++pr)
 #pragma unroll
@@ -1183,7 +1180,8 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
     // bf16: the two groups take the tiles in turn, all 64 columns each (in two halves, as registers
     // allow): while one waits the other works. Half of every tile each took 1460 cycles a tile of
     // 64, most of it in waits and in the latency of two warps a scheduler that did the same.
-    // fp32, whose keys have one buffer: half of every tile each.
+    // fp32, whose three planes leave fewer buffers than it has groups and tiles in turn: half of every
+    // tile each.
     constexpr bool kTurns = NP == 1;
     const int g = (warp - 4) >> 2;
     const uint32_t quarter = warp & 3;
@@ -1476,7 +1474,7 @@ __global__ void __launch_bounds__(256) window_delta_kernel(const __grid_constant
 #pragma unroll
     for (int v = 0; v < 8; v += n) {
       alignas(16) T x[n];
-    alignas(16) T y[n];
+      alignas(16) T y[n];
       *reinterpret_cast<uint4*>(x) = *reinterpret_cast<const uint4*>(g + v);
       *reinterpret_cast<uint4*>(y) = *reinterpret_cast<const uint4*>(o + v);
 #pragma unroll
@@ -1526,8 +1524,9 @@ bool make_view_map(CUtensorMap* map, const void* base, const uint64_t (&dims)[5]
   for (int i = 0; i < 5; ++i) d[i] = dims[i];
   for (int i = 0; i < 4; ++i) s[i] = dims[i + 1] > 1 ? strides[i] * (f32 ? 4 : 2) : 16;
   cuuint32_t box[5] = {f32 ? 32u : 64u, rows, 1, 1, 1}, unit[5] = {1, 1, 1, 1, 1};
-  return fn(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), d, s, box, unit,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  return fn(map, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5,
+            const_cast<void*>(base), d, s, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -1600,8 +1599,8 @@ struct BackwardPlan {
 };
 // Chunks of the first tokens' tiles cost about half of what another key tile does (window + 127 rows;
 // at least 256 so that a short window does not make hundreds) and come last: they even out what the
-// whole tiles leave. Query heads of a group are split
-// over items where there would be fewer than two items per SM.
+// whole tiles leave. Query heads of a group are split over items where there would be fewer than two
+// items per SM.
 BackwardPlan backward_plan(const WindowParams& w, int device) {
   BackwardPlan b;
   b.tile = w.dtype == SPAR_B200_FLOAT32 && w.head_dim > 64 ? 64 : 128;  // Bwd::kTile

@@ -128,22 +128,27 @@ def test_rotary_and_window_attention_refuse_bad_calls_without_gpu():
         strides = {f"{n}_{part}": x for n in ("q", "k", "q_out", "k_out", "dq", "dk")
                    for part, x in (("batch", 1024), ("token", 256), ("head", 64))}
         base = dict(strides, dtype=0, layout=1, batch=2, seq=3, heads=4, kv_heads=2, head_dim=64, rotary_dim=32,
-                    table=at, table_rows=3, q=at, k=at, q_out=at, k_out=at, q_weight=at, k_weight=at,
-                    epsilon=1e-6, dq=at, dk=at, dq_weight=at, dk_weight=at, scratch=at)
+                    table=at, table_rows=3, q=at, k=at + 4096, q_out=at, k_out=at + 4096, q_weight=at,
+                    k_weight=at, epsilon=1e-6, dq=at + 8192, dk=at + 12288, dq_weight=at,
+                    dk_weight=at + 256, scratch=at)
         return ctypes.byref(_lib.SparB200Rotary(**{**base, **k}))
 
     for bad in (dict(dtype=2), dict(layout=2), dict(head_dim=0), dict(head_dim=257), dict(rotary_dim=31),
                 dict(rotary_dim=66), dict(rotary_dim=0), dict(heads=0), dict(table=None), dict(q=None),
                 dict(k_out=None), dict(table_rows=2), dict(start=1), dict(start=2 ** 64 - 1), dict(q=at + 2),
                 dict(batch=1 << 20, seq=1 << 20), dict(batch=1 << 40, seq=1 << 40),
-                dict(q_out_token=0), dict(k_out_head=0)):  # rows of an output on one another
+                dict(q_out_token=0), dict(k_out_head=0),  # rows of an output on one another
+                dict(q_out=at + 4096), dict(k_out=at), dict(q_out_token=512), dict(k_out_batch=2048),
+                dict(q_out=at + 16384, k_out=at + 16384),  # not element by element in place
+                dict(positions=at + 2), dict(invalid=at + 1)):
         assert lib.spar_b200_rotary(rotary(**bad), 0, None).code == 1, bad
         assert lib.spar_b200_qk_norm_rotary_forward(rotary(**bad), 0, None).code == 1, bad
         assert lib.spar_b200_qk_norm_rotary_backward(rotary(**bad), 0, None).code == 1, bad
     for bad in (dict(q_weight=None), dict(k_weight=at + 2), dict(epsilon=-1.0), dict(epsilon=float("nan"))):
         assert lib.spar_b200_qk_norm_rotary_forward(rotary(**bad), 0, None).code == 1, bad
     for bad in (dict(dq_weight=None), dict(dk_weight=None), dict(scratch=None), dict(scratch=at + 4),
-                dict(dk=None)):
+                dict(dk=None), dict(dk_weight=at), dict(dk_weight=at + 252), dict(dq_weight=at + 2),
+                dict(q_out=at + 12288), dict(q_out=at + 8192, dq_head=128)):
         assert lib.spar_b200_qk_norm_rotary_backward(rotary(**bad), 0, None).code == 1, bad
     assert lib.spar_b200_rotary(None, 0, None).code == 1
     assert lib.spar_b200_rotary(rotary(seq=0, table=None, q=None, q_out=None), 0, None).code == 0
@@ -156,7 +161,8 @@ def test_rotary_and_window_attention_refuse_bad_calls_without_gpu():
         strides = {f"{n}_{part}": x for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")
                    for part, x in (("batch", 2048), ("token", 256), ("head", 64))}
         base = dict(strides, dtype=1, batch=2, q_len=3, kv_len=5, heads=4, kv_heads=2, head_dim=64, window=4,
-                    sinks=1, q=at, k=at, v=at, out=at, lse=at, dout=at, dq=at, dk=at, dv=at, scratch=at)
+                    sinks=1, lse=at, scratch=at,
+                    **{n: at + 65536 * x for x, n in enumerate(("q", "k", "v", "out", "dout", "dq", "dk", "dv"))})
         return ctypes.byref(_lib.SparB200WindowAttention(**{**base, **k}))
 
     for bad in (dict(dtype=7), dict(heads=0), dict(kv_heads=0), dict(kv_heads=3), dict(kv_heads=8),
@@ -164,9 +170,17 @@ def test_rotary_and_window_attention_refuse_bad_calls_without_gpu():
                 dict(scale=float("nan")), dict(scale=float("inf")), dict(q=None), dict(k=at + 1),
                 dict(q_len=1 << 29), dict(kv_len=1 << 40), dict(batch=1 << 29, heads=64, kv_heads=64),
                 dict(batch=1 << 12, kv_len=1 << 20), dict(scale=1e-31), dict(scale=1e31), dict(out_batch=0),
-                dict(out_token=0), dict(out_head=0)):
+                dict(lse=at + 2), dict(lengths=at + 2), dict(first=at + 1)):
         assert lib.spar_b200_window_attention_forward(window(**bad), 0, None).code == 1, bad
         assert lib.spar_b200_window_attention_backward(window(**bad), 0, None).code == 1, bad
+    for bad in (dict(out_token=0), dict(out_head=0), *(dict(out=at + 65536 * x) for x in range(3))):
+        assert lib.spar_b200_window_attention_forward(window(**bad), 0, None).code == 1, bad
+    written = {"dq": 5, "dk": 6, "dv": 7}
+    for name, own in written.items():  # in the place of an input, or of another output
+        for x in range(8):
+            if x != own:
+                bad = {name: at + 65536 * x}
+                assert lib.spar_b200_window_attention_backward(window(**bad), 0, None).code == 1, bad
     for bad in (dict(dout=None), dict(lse=None), dict(dv=None), dict(scratch=None), dict(scratch=at + 16),
                 dict(dq_token=0), dict(dk_head=0), dict(dv_batch=0)):
         assert lib.spar_b200_window_attention_backward(window(**bad), 0, None).code == 1, bad

@@ -183,6 +183,58 @@ def test_nan_in_a_visible_key_or_value(cuda, dim, dtype):
                 assert bool(torch.isfinite(x[0, :, 1]).all() and torch.isfinite(x[1]).all())
 
 
+@pytest.mark.parametrize("dtype,rows,dim", [(torch.bfloat16, 300, 64), (torch.bfloat16, 1, 64),
+                                            (torch.bfloat16, 1, 40), (torch.float32, 1, 64),
+                                            (torch.float32, 40, 33), (torch.bfloat16, 40, 33)])
+def test_scores_of_minus_infinity(cuda, dtype, rows, dim):
+    """Keys whose scores are -infinity have no weight; a row that sees only such keys is 0 / 0, and its
+    lse is -infinity. (In the tiled, the decoding and the row path.)"""
+    from spar_b200 import ops
+
+    g = torch.Generator(device=cuda)
+    g.manual_seed(27)
+    q = torch.rand(1, rows, 2, dim, generator=g, device=cuda).to(dtype) + 0.5
+    k, v = (torch.randn(1, 300, 1, dim, generator=g, device=cuda).to(dtype) for _ in range(2))
+    k[0, 298:, :, 0] = -math.inf
+    out, lse = ops.window_attention_forward(q, k, v, 2)
+    assert torch.isnan(out[0, -1]).all() and torch.isneginf(lse[0, :, -1]).all()
+    out, lse = ops.window_attention_forward(q, k, v, 290)
+    want, bound = window_attention(*(x.double().cpu() for x in (q[:, -1:], k[:, 10:298], v[:, 10:298])), 300, 0,
+                                   h=half_step(dtype))
+    assert_within(out[:, -1:], want["out"], bound["out"], "out")
+    assert_within(lse[..., -1:], want["lse"], bound["lse"], "lse")
+    assert torch.isfinite(lse).all()
+    torch.cuda.synchronize()
+    assert ops.attention_error() == 0
+
+
+@pytest.mark.parametrize("rows", [1, 100])
+def test_cache_offsets_beyond_32_bits(cuda, rows):
+    """70000 tokens 2^16 elements apart: the visible rows lie beyond 2^32 elements of the cache."""
+    from spar_b200 import ops
+
+    n, d, apart = 70000, 64, 1 << 16
+    cache = torch.zeros(n, apart, device=cuda, dtype=torch.bfloat16)
+    g = torch.Generator(device=cuda)
+    g.manual_seed(28)
+    cache[-400:, :2 * d] = torch.randn(400, 2 * d, generator=g, device=cuda).bfloat16()
+    k, v = (cache[None, :, None, i * d:(i + 1) * d] for i in range(2))
+    q, dout = (torch.randn(1, rows, 2, d, generator=g, device=cuda).bfloat16() for _ in range(2))
+    dk, dv = (cache[None, :, None, i * d:(i + 1) * d] for i in range(2, 4))
+    out, lse = ops.window_attention_forward(q, k, v, 250, 3)
+    dq, _, _ = ops.window_attention_backward(dout, q, k, v, out, lse, 250, 3, dk=dk, dv=dv)
+    torch.cuda.synchronize()
+    assert ops.attention_error() == 0
+    # all that a row sees: the first tokens (zeros) and the last 400
+    pick = [*range(3), *range(n - 400, n)]
+    want, bound = window_attention(*(x.double().cpu() for x in (q, k[:, pick], v[:, pick])), 250, 3,
+                                   dout=dout.double().cpu(), h=half_step(q.dtype))
+    got = {"out": out, "lse": lse, "dq": dq, "dk": dk[:, pick], "dv": dv[:, pick]}
+    for name in want:
+        assert_within(got[name], want[name], bound[name], name)
+    assert not dk[:, 3:n - 400].any() and not dv[:, 3:n - 400].any()
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_large_logits_and_a_given_scale(cuda, dtype):
     g = torch.Generator(device=cuda)
