@@ -1126,48 +1126,114 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
           if (last) tc::mma_commit(a_empty + an % L::kStats);
           return true;
         };
-        for (uint32_t tn = 0; ok && !*abort_flag.cta; ++tn) {
-          int idx;
-          if (!(ok = take(tn, idx))) break;
-          tc::mbar_arrive(item_empty + (tn & 3));
-          if (idx >= p.items) break;
+        // The products of tile m's P and dS: queries dq += dS k; keys dk += dS^T q, dv += P^T dout.
+        auto products = [&](uint32_t m, bool first, bool last) {
+          const uint32_t st = m % ST, buf = tmem + (m % L::kBuffers) * L::kBuf;
+          tc::tc_fence_after();
+#pragma unroll
+          for (int out = 0; out < static_cast<int>(L::kOuts); ++out) {
+            const int operand = OUT == 2 ? 1 : out, which = KEYS ? 1 - operand : 0;
+            const uint32_t b = mnmajor_low(b_addr + (2 * st + operand) * L::kMov, kMoving);
+            uint32_t acc = NP == 1 && !first;
+#pragma unroll
+            for (int pr = 0; pr < kProducts<NP>; ++pr)
+#pragma unroll
+              for (int ks = 0; ks < kMoving / 16; ++ks) {
+                tc::mma_f16_ts(tmem + L::kAcc + out * DH, buf + operand_col<KEYS>(which, plane_a<NP>(pr), ks),
+                               desc(b + mnmajor_step(kMoving, plane_b<NP>(pr), kBoxes, ks)), idesc_o, acc);
+                acc = 1;
+              }
+          }
+          tc::mma_commit(m_empty + st);
+          if (NP > 1 || last) tc::mma_commit(sum_full);
+        };
+        auto tiles_of = [&](int idx) -> int {
           Item q;
           KeyItem k;
-          const int n = jobs_of(idx, q, k);
-          if (!n) continue;
-          if (!(ok = wait_or_abort(a_full + an % L::kStats, an / L::kStats, abort_flag))) break;
-          constexpr int kAhead = L::kBuffers > 1 ? L::kBuffers - 1 : 1;
-          for (int i = 0; i < kAhead && i < n && ok; ++i) ok = scores(mn + i, i + 1 == n);
-          for (int i = 0; i < n && ok; ++i) {
-            const uint32_t m = mn + i, st = m % ST, buf = tmem + (m % L::kBuffers) * L::kBuf;
-            // The buffer of tile i + kAhead was last read by the products of tile i - 1, issued before.
-            if (L::kBuffers > 1 && i + kAhead < n && !(ok = scores(m + kAhead, i + kAhead + 1 == n))) break;
-            if (!(ok = wait_or_abort(pd_full + m % L::kBuffers, m / L::kBuffers, abort_flag))) break;
-            // Sums start afresh with an item; the softmax warps have read the ones before.
-            if (i == 0 && !(ok = wait_or_abort(sum_empty, sums + 1, abort_flag))) break;
-            tc::tc_fence_after();
-#pragma unroll
-            for (int out = 0; out < static_cast<int>(L::kOuts); ++out) {
-              // queries: dq += dS k; keys: dk += dS^T q, dv += P^T dout
-              const int operand = OUT == 2 ? 1 : out, which = KEYS ? 1 - operand : 0;
-              const uint32_t b = mnmajor_low(b_addr + (2 * st + operand) * L::kMov, kMoving);
-              uint32_t acc = NP == 1 && i > 0;
-#pragma unroll
-              for (int pr = 0; pr < kProducts<NP>; ++pr)
-#pragma unroll
-                for (int ks = 0; ks < kMoving / 16; ++ks) {
-                  tc::mma_f16_ts(tmem + L::kAcc + out * DH, buf + operand_col<KEYS>(which, plane_a<NP>(pr), ks),
-                                 desc(b + mnmajor_step(kMoving, plane_b<NP>(pr), kBoxes, ks)), idesc_o, acc);
-                  acc = 1;
-                }
+          return idx < p.items ? jobs_of(idx, q, k) : -1;
+        };
+        if constexpr (NP == 1 || L::kBuffers == 1) {
+          for (uint32_t tn = 0; ok && !*abort_flag.cta; ++tn) {
+            int idx;
+            if (!(ok = take(tn, idx))) break;
+            tc::mbar_arrive(item_empty + (tn & 3));
+            const int n = tiles_of(idx);
+            if (n < 0) break;
+            if (!n) continue;
+            if (!(ok = wait_or_abort(a_full + an % L::kStats, an / L::kStats, abort_flag))) break;
+            constexpr int kAhead = L::kBuffers > 1 ? L::kBuffers - 1 : 1;
+            for (int i = 0; i < kAhead && i < n && ok; ++i) ok = scores(mn + i, i + 1 == n);
+            for (int i = 0; i < n && ok; ++i) {
+              const uint32_t m = mn + i;
+              // The buffer of tile i + kAhead was last read by the products of tile i - 1, issued before.
+              if (L::kBuffers > 1 && i + kAhead < n && !(ok = scores(m + kAhead, i + kAhead + 1 == n))) break;
+              if (!(ok = wait_or_abort(pd_full + m % L::kBuffers, m / L::kBuffers, abort_flag))) break;
+              // Sums start afresh with an item; the softmax warps have read the ones before.
+              if (i == 0 && !(ok = wait_or_abort(sum_empty, sums + 1, abort_flag))) break;
+              products(m, i == 0, i + 1 == n);
+              if (L::kBuffers == 1 && i + 1 < n) ok = scores(m + 1, i + 2 == n);
             }
-            tc::mma_commit(m_empty + st);
-            if (NP > 1 || i + 1 == n) tc::mma_commit(sum_full);
-            if (L::kBuffers == 1 && i + 1 < n) ok = scores(m + 1, i + 2 == n);
+            mn += n;
+            ++sums;
+            ++an;
           }
-          mn += n;
-          ++sums;
-          ++an;
+        } else {
+          // fp32: scores run ahead of the products over both buffers, also into the next item, whichever is
+          // ready first, so that an item's end, its results and the next one's operands cost the tensor
+          // cores less (16 x 1024 x 16 x 64, all keys: 980 -> 894 us). Nothing here waits for one while the
+          // other could go on. (bf16, with six times fewer products, is bound by this thread's and the
+          // softmax's instructions: there it was slower, 137 -> 145 us of 2 x 4096 x 16/4 x 64.)
+          uint32_t tn = 0, done = 0;
+          uint32_t firsts = 0, lasts = 0;  // bit m & 3: tile m is its item's first or last
+          int n = 0, i = 0;                // the item whose scores are under way
+          bool more = true;
+          uint32_t idle = 0;
+          uint64_t since = 0;
+          while (ok && (more || done != mn)) {  // tiles whose products, and whose scores, are issued
+            bool moved = false;
+            if (more && mn - done < static_cast<uint32_t>(L::kBuffers)) {
+              if (i >= n) {
+                if ((moved = tc::mbar_test(item_full + (tn & 3), tn / 4 & 1))) {
+                  const int idx = items[tn & 3];
+                  tc::mbar_arrive(item_empty + (tn & 3));
+                  ++tn;
+                  i = 0;
+                  n = tiles_of(idx);
+                  more = n >= 0;
+                }
+              } else if ((i || tc::mbar_test(a_full + an % L::kStats, an / L::kStats & 1)) &&
+                         tc::mbar_test(m_full + mn % ST, mn / ST & 1)) {
+                const uint32_t bit = 1u << (mn & 3);
+                firsts = i ? firsts & ~bit : firsts | bit;
+                lasts = i + 1 < n ? lasts & ~bit : lasts | bit;
+                ok = scores(mn, i + 1 == n);
+                if (++i == n) ++an;
+                ++mn;
+                moved = true;
+              }
+            }
+            if (done != mn && tc::mbar_test(pd_full + done % L::kBuffers, done / L::kBuffers & 1)) {
+              const bool first = firsts >> (done & 3) & 1;
+              // (sum_empty as above)
+              if (!first || tc::mbar_test(sum_empty, (sums + 1) & 1)) {
+                if (first) ++sums;
+                products(done, first, lasts >> (done & 3) & 1);
+                ++done;
+                moved = true;
+              }
+            }
+            if (moved) {
+              idle = 0;
+            } else if ((++idle & 1023) == 0) {  // the bound on all of these waits
+              const uint64_t now = tc::global_timer_ns();
+              if (idle == 1024) since = now;
+              if (*abort_flag.cta || now - since > tc::kWaitLimitNs) {
+                atomicExch(abort_flag.device, 1);
+                *abort_flag.cta = 1;
+                ok = false;
+              }
+            }
+          }
         }
         tc::mma_commit(drain);
         wait_or_abort(drain, 0, abort_flag);
@@ -1256,10 +1322,30 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
           kept = w.sinks - key;
         }
         if (!valid) hi = -1;
+        const bool behind = clear < kMoving && (KEYS ? s.n < s.p0 + w.q_len : key + clear < w.kv_len);
         if (!(ok = wait_or_abort(s_full + m % L::kBuffers, m / L::kBuffers, abort_flag))) break;
         tc::tc_fence_after();
         const float* stats = reinterpret_cast<const float*>(smem + L::kRows + st * L::kRowsBytes);
         if (KEYS && !L::kAugment && !(ok = wait_or_abort(m_full + st, m / ST, abort_flag))) break;
+        auto seen_of = [&](int c0) {  // bits of columns c0 .. c0 + 31
+          uint32_t seen = below(hi + 1 - c0) & ~below(lo - c0);
+          if (!KEYS) seen &= ~below(near - c0) | below(kept - c0);
+          return seen;
+        };
+        // Where the tile or its rows reach behind the sequence they may hold anything, and 0 times NaN is
+        // NaN: hidden dP become zero. (Here and not beside the hidden scores: few tiles need it, and in
+        // the loop below it cost all of them 3 %.)
+        if ((behind || !rows_in) && r - lane < L::kTile) {
+#pragma unroll 1
+          for (int half = kTurns ? 0 : g; half < (kTurns ? 2 : g + 1); ++half) {
+            const uint32_t seen = seen_of(half * 32);
+            uint32_t v[32];
+            tc::tmem_load_32x32(buf + 64 + half * 32, v);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) v[e] = seen & (1u << e) ? v[e] : 0u;
+            tc::tmem_store_32x32(buf + 64 + half * 32, v);
+          }
+        }
 #pragma unroll
         for (int half = kTurns ? 0 : g; half < (kTurns ? 2 : g + 1); ++half) {
           const int c0 = half * 32;
@@ -1273,6 +1359,7 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
             all_seen = all_seen && key + c0 + 31 <= first_pos &&
                        (i < q.ns ? key + c0 + 32 <= w.sinks
                                  : key + c0 > first_pos + 31 - w.window || key + c0 + 32 <= w.sinks);
+          if (!all_seen) hide32(sv, seen_of(c0));  // P and dS of zero
           uint64_t pr[16], ds[16];
 #pragma unroll
           for (int e = 0; e < 16; e += 2) {
@@ -1298,17 +1385,6 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
             pr[e + 1] = both(ex2(t1.x), ex2(t1.y));
             ds[e] = mul2(pr[e], g0);
             ds[e + 1] = mul2(pr[e + 1], g1);
-          }
-          if (!all_seen) {
-            uint32_t seen = below(hi + 1 - c0) & ~below(lo - c0);
-            if (!KEYS) seen &= ~below(near - c0) | below(kept - c0);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float2 a = halves(pr[e]), d = halves(ds[e]);
-              const bool first = seen & (1u << (2 * e)), second = seen & (2u << (2 * e));
-              pr[e] = both(first ? a.x : 0.f, second ? a.y : 0.f);
-              ds[e] = both(first ? d.x : 0.f, second ? d.y : 0.f);
-            }
           }
           // Operands over the columns just read: plane pl of both K steps is 16 columns.
 #pragma unroll
@@ -1337,7 +1413,7 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
         }
         // Moving rows behind the sequence may hold anything, and 0 times NaN is NaN: clear them (and the
         // keys behind the first tokens in their tiles, which every row visits).
-        if (clear < kMoving && (KEYS ? s.n < s.p0 + w.q_len : key + clear < w.kv_len)) {
+        if (behind) {
           if (!KEYS && !(ok = wait_or_abort(m_full + st, m / ST, abort_flag))) break;
           uint8_t* mt = smem + L::kB + st * 2 * L::kMov;
           for (int c = max(clear, 0) * 8 + (kTurns ? r : g * 128 + r); c < kMoving * 8; c += kTurns ? 128 : 256)
