@@ -462,9 +462,10 @@ struct SparCudaStatus spar_b200_qk_norm_rotary_backward(const struct SparB200Rot
 /* an output with a stride of zero over more than one index is refused.                          */
 /* bf16: products of bf16 operands (P and dS rounded to nearest) with fp32 sums; fp32: as exact as */
 /* fp32 products and sums (values below 2^-110 keep fewer bits). 16-byte aligned rows with head_dim */
-/* a multiple of 8, at most 128, run on the tensor cores; up to 32 rows of a head group (heads /   */
-/* kv_heads * q_len) run as a decoding step; everything else runs one warp per row. A bounded wait */
-/* that runs out sets the flag of spar_b200_attention_error.                                      */
+/* a multiple of 8, at most 128, run on the tensor cores; up to 16 rows of a head group (heads /   */
+/* kv_heads * q_len), or 64 where the visible keys are eight times as many, run as a decoding step; */
+/* everything else runs one warp per row. A bounded wait that runs out sets the flag of            */
+/* spar_b200_attention_error.                                                                      */
 struct SparB200WindowAttention {
   int dtype; /* SparB200Element of q, k, v, out and the gradients */
   uint64_t batch, q_len, kv_len, heads, kv_heads;

@@ -108,6 +108,11 @@ CACHE = [
     (2, 1, 1000, 8, 2, 128, 256, 4),
     (4, 1, 2100, 16, 1, 64, 5000, 0),   # sixteen heads of one cache
     (2, 3, 777, 8, 2, 64, 100, 1),      # a few tokens at once
+    (1, 5, 600, 16, 2, 64, 1000, 4),    # 40 rows of a long cache: still a decoding step
+    (2, 64, 700, 2, 2, 128, 600, 3),    # 64
+    (2, 64, 500, 2, 2, 128, 600, 3),    # too short beside its rows: tiled
+    (1, 65, 900, 1, 1, 64, 900, 0),     # one row more: tiled
+    (3, 6, 30, 4, 1, 96, 20, 2),        # 24 rows of a short cache: tiled
     (1, 5, 640, 32, 4, 128, 600, 64),
     (2, 1, 300, 6, 3, 96, 100, 3),
     (1, 2, 500, 3, 1, 50, 100, 3),
