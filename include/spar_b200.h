@@ -407,7 +407,8 @@ struct SparB200Rotary {
   uint64_t head_dim;   /* 1 .. 256 */
   uint64_t rotary_dim; /* even, 2 .. head_dim: the first rotary_dim elements of a head turn, the */
                        /* others pass                                                           */
-  const float* table;  /* [table_rows, rotary_dim / 2] (cos, sin) */
+  const float* table;  /* [table_rows, rotary_dim / 2] (cos, sin); may be NULL with no rows, when    */
+                       /* every position lies outside it                                        */
   uint64_t table_rows;
   const int32_t* positions; /* [batch, seq] table rows of the tokens; NULL: token t of every     */
   uint64_t start;           /* sequence has row start + t                                        */

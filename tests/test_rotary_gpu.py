@@ -211,6 +211,31 @@ def test_positions_outside_the_table_give_zeros_and_set_the_flag(cuda):
             assert bool(torch.isfinite(dw).all())
 
 
+@pytest.mark.parametrize("d,r", [(64, 64), (64, 32), (33, 10)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_table_without_rows_has_no_position_inside(cuda, dtype, d, r):
+    """Every position lies outside it: zeros, the flag, weight gradients of zero; nothing of it is read
+    (there may be no table at all)."""
+    from spar_b200 import ops
+
+    g = torch.Generator(device=cuda)
+    g.manual_seed(31)
+    q, k = _views(cuda, g, dtype, 2, 6, 4, 2, d)
+    ones = torch.ones(d, device=cuda)
+    positions = torch.zeros(2, 6, dtype=torch.int32, device=cuda)
+    table = torch.empty(0, r // 2, 2, device=cuda)
+    for layout in ("interleaved", "half"):
+        where = dict(layout=layout, positions=positions)
+        for call in (lambda f: ops.rotary(q, k, table, invalid=f, **where),
+                     lambda f: ops.qk_norm_rotary_forward(q, k, ones, ones, table, invalid=f, **where),
+                     lambda f: ops.qk_norm_rotary_backward(q, k, q, k, ones, ones, table, invalid=f, **where)):
+            flag = torch.zeros(1, dtype=torch.int32, device=cuda)
+            got = call(flag)
+            assert int(flag) == 1
+            for x in got:
+                assert not x.any()
+
+
 def test_no_tokens(cuda):
     from spar_b200 import ops
 
