@@ -31,7 +31,9 @@ struct WindowParams {
   float scale;
 };
 
-// What one sequence of the batch holds: n keys, and the position of its first row.
+// What of one sequence of the batch the call's rows can see: its first n keys, which end with its length
+// or with the last row's position (a cache's slots behind them may hold anything), and the position of
+// its first row.
 struct Sequence {
   int n, p0;
 };
@@ -41,6 +43,7 @@ __device__ __forceinline__ Sequence sequence_of(const WindowParams& w, int b) {
   // Positions beyond +-2^29 see nothing, as every position at or behind the length does.
   const int far = 1 << 29;
   s.p0 = w.first ? min(max(__ldg(w.first + b), -far), far) : w.kv_len - w.q_len;
+  s.n = min(s.n, max(s.p0 + w.q_len, 0));
   return s;
 }
 

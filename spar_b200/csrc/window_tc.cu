@@ -1292,10 +1292,12 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
       const int row = (KEYS ? k.key : q.row[0]) + r;
       const int pos = KEYS ? row : s.p0 + row;
       const int first_pos = pos - lane;  // of this warp
-      const bool valid =
-          r < L::kTile && (KEYS ? row < s.n : row < w.q_len && pos >= 0 && pos < s.n);
+      // (keys: older than the first row's window, and no first token, is seen by no row)
+      const int oldest = KEYS ? max(s.p0, 0) - w.window + 1 : 0;
+      const bool valid = r < L::kTile && (KEYS ? row < s.n && (row >= oldest || row < w.sinks)
+                                               : row < w.q_len && pos >= 0 && pos < s.n);
       const bool rows_in = r - lane >= L::kTile ? false
-                           : KEYS               ? first_pos + 31 < s.n
+                           : KEYS               ? first_pos + 31 < s.n && first_pos >= oldest
                                 : first_pos >= 0 && first_pos + 31 < s.n && row - lane + 31 < w.q_len;
       uint64_t minus_lse = 0, minus_delta = 0;
       if (!KEYS && valid && n) {

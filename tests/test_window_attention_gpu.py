@@ -160,6 +160,41 @@ def test_positions_of_the_first_row(cuda):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows,dim", [(200, 64), (130, 128), (70, 96), (3, 64), (90, 33)])
+def test_what_no_row_sees_may_hold_anything(cuda, rows, dim, dtype):
+    """A chunk of a prompt against a cache whose fill only `first` tells: the slots behind the chunk, those
+    older than its first row's window, and rows before position 0 or behind the length reach no result."""
+    from spar_b200 import ops
+
+    g = torch.Generator(device=cuda)
+    g.manual_seed(33)
+    first = torch.tensor([300, 0, 411, -50], dtype=torch.int32, device=cuda)
+    q, dout = (torch.randn(4, rows, 4, dim, generator=g, device=cuda).to(dtype) for _ in range(2))
+    k, v = (torch.randn(4, 700, 2, dim, generator=g, device=cuda).to(dtype) for _ in range(2))
+    longer = torch.tensor([600, 700, 690, 700], dtype=torch.int32, device=cuda)
+    inside = torch.tensor([310, 1, 500, 40], dtype=torch.int32, device=cuda)
+    for lengths in (None, longer, inside):
+        for window, sinks in ((60, 4), (130, 0), (1000, 0)):
+            where = dict(lengths=lengths, first=first)
+            clean = _check(q, k, v, window, sinks, dout, **where)
+            bad = [x.clone() for x in (q, k, v, dout)]
+            for b, f in enumerate(first.tolist()):
+                n = 700 if lengths is None else int(lengths[b])
+                for x in bad[1:3]:
+                    x[b, min(max(f + rows, 0), n):] = math.nan
+                    x[b, min(max(f + rows, 0), n)::2] = math.inf
+                    x[b, sinks:max(max(f, 0) - window + 1, sinks)] = math.nan
+                for x in (bad[0], bad[3]):
+                    x[b, :max(-f, 0)] = math.nan
+                    x[b, max(n - f, 0):] = math.inf
+            bq, bk, bv, bdout = bad
+            out, lse = ops.window_attention_forward(bq, bk, bv, window, sinks, **where)
+            grads = ops.window_attention_backward(bdout, bq, bk, bv, out, lse, window, sinks, **where)
+            for x, name in zip((out, lse, *grads), ("out", "lse", "dq", "dk", "dv")):
+                assert torch.equal(x, clean[name]), (name, window, sinks)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("dim", [64, 128, 20])
 def test_nan_in_a_visible_key_or_value(cuda, dim, dtype):
     """It makes every row that sees it NaN, whichever column of a tile it falls on, and no row of
