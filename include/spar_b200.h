@@ -455,10 +455,16 @@ struct SparCudaStatus spar_b200_qk_norm_rotary_backward(const struct SparB200Rot
 /*   j <= p  and  (j > p - window  or  j < sinks)  and  j < lengths[b]  and  p < lengths[b].     */
 /*   out = softmax(scale q k^T over the visible keys) v,  lse = ln sum exp(scale q k^T).         */
 /* A row that sees nothing (padding behind lengths[b], a position below 0) gives zeros, lse =    */
-/* -infinity, and no gradient. Keys and values at or behind lengths[b] reach no result, whatever */
-/* they hold (a cache's unused slots may hold NaN). A NaN in a key or value below lengths[b]      */
-/* makes the rows that see it NaN, and may also reach rows near those. Infinities follow the       */
-/* formula, but fp32 on the tensor cores may take them as NaN.                                    */
+/* -infinity, and no gradient. Such rows, and keys that no row of the call sees (at or behind     */
+/* lengths[b], behind the last row's position, or older than the first row's window and no first  */
+/* token), reach no other result, whatever they hold: a cache's unused and evicted slots may hold */
+/* NaN, with lengths NULL too.                                                                     */
+/* A NaN or an infinity in a row or key that takes part gives the results it enters what the       */
+/* formula gives or NaN: products are made tile by tile, where a weight of zero times it is NaN,   */
+/* and fp32 on the tensor cores takes every infinity as NaN (elsewhere a score of -infinity gives   */
+/* its key no weight). For the same reason it may make NaN the results of rows within 256           */
+/* positions of one that sees the key, and of keys within 256 positions of one that the row sees,   */
+/* of its sequence and head group; it reaches no others.                                          */
 /* Outputs must not overlap inputs or one another (refused where they start at the same element);  */
 /* an output with a stride of zero over more than one index is refused.                          */
 /* bf16: products of bf16 operands (P and dS rounded to nearest) with fp32 sums; fp32: as exact as */

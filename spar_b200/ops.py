@@ -548,7 +548,9 @@ def window_attention_forward(q, k, v, window: int, sinks: int = 0, *, scale: flo
     projection's parts, or a cache); query head h reads key head h / (heads / kv_heads). Row i of
     sequence b stands at position p = first[b] + i (first None: kv_len - q_len) and sees key j iff
     j <= p, j < lengths[b] (None: kv_len), and j > p - window or j < sinks; a row with p < 0 or
-    p >= lengths[b] sees nothing (out 0, lse -inf). scale None: 1 / sqrt(head_dim).
+    p >= lengths[b] sees nothing (out 0, lse -inf). scale None: 1 / sqrt(head_dim). What no row sees
+    may hold anything (a cache's unused slots); a NaN or infinity elsewhere may make rows within 256
+    positions of those that see it NaN too.
     Returns (out like q, lse [batch, heads, q_len])."""
     out, view = _out_view(out, "out", q)
     lse = q.new_empty((q.shape[0], q.shape[2], q.shape[1]), dtype=torch.float32)

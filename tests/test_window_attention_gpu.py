@@ -223,6 +223,50 @@ def test_nan_in_a_visible_key_or_value(cuda, dim, dtype):
                 assert bool(torch.isfinite(x[0, :, 1]).all() and torch.isfinite(x[1]).all())
 
 
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("part", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("dtype,rows,dim", [(torch.bfloat16, 900, 64), (torch.bfloat16, 900, 128),
+                                            (torch.float32, 900, 64), (torch.float32, 900, 128),
+                                            (torch.bfloat16, 900, 20), (torch.bfloat16, 5, 64),
+                                            (torch.float32, 5, 64)])
+def test_how_far_one_bad_value_reaches(cuda, dtype, rows, dim, part, bad):
+    """Results that it does not enter keep their bits, or become NaN within 256 positions; those of a
+    value's or query's column that it enters are not finite."""
+    from spar_b200 import ops
+
+    n, window, sinks = 900, 100, 3
+    g = torch.Generator(device=cuda)
+    g.manual_seed(34)
+    x = {m: torch.randn(2, rows, 4, dim, generator=g, device=cuda).to(dtype) for m in ("q", "dout")}
+    x |= {m: torch.randn(2, n, 2, dim, generator=g, device=cuda).to(dtype) for m in ("k", "v")}
+    out, lse = ops.window_attention_forward(x["q"], x["k"], x["v"], window, sinks)
+    clean = [out, *ops.window_attention_backward(x["dout"], x["q"], x["k"], x["v"], out, lse, window, sinks)]
+    row, key = torch.arange(n - rows, n, device=cuda), torch.arange(n, device=cuda)
+    see = (key <= row[:, None]) & ((key > row[:, None] - window) | (key < sinks))
+    for place in ((1, 433, 897) if part in "kv" else (rows // 2, rows - 2)):
+        y = {m: t.clone() for m, t in x.items()}
+        y[part][0, place, 1, 0] = bad  # head 1: of the first group as a query, of the second as a key
+        heads, kv = (slice(0, 2), slice(0, 1)) if part in ("q", "dout") else (slice(2, 4), slice(1, 2))
+        got = ops.window_attention_forward(y["q"], y["k"], y["v"], window, sinks)
+        grads = ops.window_attention_backward(y["dout"], y["q"], y["k"], y["v"], out, lse, window, sinks)
+        enter = [see[:, place], key == place] if part in "kv" else [row == row[place], see[place]]
+        for t, was, name in zip((got[0], *grads), clean, ("out", "dq", "dk", "dv")):
+            at, entered, own = (row, enter[0], heads) if name in ("out", "dq") else (key, enter[1], kv)
+            near = ((at[:, None] - at[entered]).abs() <= 256).any(1)
+            reach = torch.zeros(t.shape[:3], dtype=torch.bool, device=cuda)
+            reach[0, near, own] = True
+            changed = ~((t == was) | (torch.isnan(t) & torch.isnan(was)))
+            assert not changed[~reach].any(), (name, place)
+            reach[0, entered, own] = False
+            assert bool(torch.isnan(t[reach])[changed[reach]].all()), (name, place)
+            if (part, name) in (("v", "out"), ("dout", "dv"), ("q", "dq")):
+                own = own if part == "v" else 1 if part == "q" else kv
+                assert not torch.isfinite(t[0, entered][:, own, 0]).any(), (name, place)
+                if name != "dq":
+                    keep = t[0, entered][:, own, 1:] == was[0, entered][:, own, 1:]
+                    assert bool(keep.all()), (name, place)
+
+
 @pytest.mark.parametrize("dtype,rows,dim", [(torch.bfloat16, 300, 64), (torch.bfloat16, 1, 64),
                                             (torch.bfloat16, 1, 40), (torch.float32, 1, 64),
                                             (torch.float32, 40, 33), (torch.bfloat16, 40, 33)])
