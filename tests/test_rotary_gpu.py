@@ -276,6 +276,79 @@ def test_rotary_table(cuda, rows, rotary, start, kind):
     assert_within(got, want, U * want.abs() + slack)
 
 
+def _lanes(dim, rotary, dtype):
+    """Lanes of a head's group in the vectorised forms: the power of two that holds its slots."""
+    v = 4 if dtype == torch.float32 else 8
+    slots = rotary // 2 // v + ((dim - rotary) // v + 1) // 2
+    return 1 << (slots - 1).bit_length()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("rotary", [64, 32])
+def test_enough_tokens_that_heads_share_their_angles(cuda, rotary, layout, dtype):
+    """From 64 warps an SM on, a lane group takes two or four heads of a token; 17 and 3 heads leave
+    chunks that are not full, and the tokens do not fill the last block."""
+    from spar_b200 import ops
+
+    h, kv, d, b = 17, 3, 64, 3
+    warps = 64 * torch.cuda.get_device_properties(cuda).multi_processor_count
+    t = warps * 32 // (b * (h + kv) * _lanes(d, rotary, dtype)) + 3
+    g = torch.Generator(device=cuda)
+    g.manual_seed(41)
+    q, k = _views(cuda, g, dtype, b, t, h, kv, d)
+    table = _table(cuda, t + 40, rotary, g)
+    positions = torch.randint(0, t + 40, (b, t), generator=g, device=cuda).to(torch.int32)
+    w = [1 + 0.3 * torch.randn(d, generator=g, device=cuda) for _ in range(2)]
+    for pos, start, inverse in ((positions, 0, False), (None, 5, True)):
+        where = dict(layout=layout, positions=pos, start=start)
+        turned = ops.rotary(q, k, table, inverse=inverse, **where)
+        normed = ops.qk_norm_rotary_forward(q, k, *w, table, EPS, **where)
+        angles, hs = _angles(table, pos, start, t), half_step(dtype)
+        for x, ww, y, z in zip((q, k), w, turned, normed):
+            x, ww = x.double().cpu(), ww.double().cpu()
+            want = rotate(x, angles, rotary, layout, -1.0 if inverse else 1.0)
+            off = 3 * U * _size(x, angles, rotary, layout)
+            off[..., rotary:] = 0
+            assert_within(y, want, hs * want.abs() + (1 + hs) * off, "turned")
+            want = norm_rotate(x, ww, angles, rotary, layout, EPS)
+            inv = 1.0 / torch.sqrt((x * x).mean(-1, keepdim=True) + EPS)
+            assert_within(z, want, hs * want.abs() + 32 * U * _size(x * inv * ww, angles, rotary, layout), "normed")
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("dim,rotary", [(64, 64), (64, 32), (33, 10)])
+def test_backward_over_more_units_than_the_grid_has_groups(cuda, dim, rotary, layout, dtype):
+    """Sixteen blocks of 128 threads an SM, split between queries and keys, walk the tokens: here every
+    lane group takes two or three units of either side, and the sums of the weights stay in registers."""
+    from spar_b200 import ops
+
+    h, kv, b = 9, 3, 2
+    lanes = 32 if dim == 33 else _lanes(dim, rotary, dtype)
+    shared = 2 if dtype == torch.float32 and dim != 33 else 1  # heads of a unit
+    blocks = 16 * torch.cuda.get_device_properties(cuda).multi_processor_count
+    chunks = -(-h // shared) + -(-kv // shared)
+    t = int(2.5 * blocks * (128 // lanes) / (b * chunks)) + 1
+    g = torch.Generator(device=cuda)
+    g.manual_seed(42)
+    q, k = _views(cuda, g, dtype, b, t, h, kv, dim)
+    dq, dk = _views(cuda, g, dtype, b, t, h, kv, dim)
+    table = _table(cuda, t + 9, rotary, g)
+    w = [1 + 0.3 * torch.randn(dim, generator=g, device=cuda) for _ in range(2)]
+    back = ops.qk_norm_rotary_backward(dq, dk, q, k, *w, table, EPS, layout=layout, start=7)
+    again = ops.qk_norm_rotary_backward(dq, dk, q, k, *w, table, EPS, layout=layout, start=7)
+    assert all(torch.equal(x, y) for x, y in zip(back, again))
+    angles, hs = table.double()[7:7 + t][None], half_step(dtype)
+    for x, dy, ww, dx, dw in zip((q, k), (dq, dk), w, back[:2], back[2:]):
+        wdx, wdw, sdx, sdw = (y.cpu() for y in norm_rotate_backward(dy.double(), x.double(), ww.double(), angles,
+                                                                    rotary, layout, EPS))
+        assert_within(dx, wdx, hs * wdx.abs() + 96 * U * sdx, "dx")
+        # Each term is under 40 u off; their sum goes through at most 3 units x 2 heads of a lane, the
+        # groups of a block and the blocks: fewer additions than blocks + 128 + 8.
+        assert_within(dw, wdw, (40 + blocks + 136) * U * sdw, "dw")
+
+
 def test_captured_on_another_stream_and_replayed(cuda):
     from spar_b200 import ops
 
