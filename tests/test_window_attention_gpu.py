@@ -101,6 +101,31 @@ def test_padded_batch_ignores_what_lies_behind_the_lengths(cuda, dtype, dim):
         assert torch.equal(x, clean[name]), name
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,kv", [(32, 8), (24, 8)])  # pairs of heads, and (groups of three) of tiles
+def test_several_items_for_every_cta(cuda, heads, kv, dim, dtype):
+    """More items than SMs, of differing numbers of key tiles and some of none: what a CTA carries from
+    one to the next (the rings' phases, both stationary buffers, drawn items, scores that run ahead)."""
+    from spar_b200 import ops
+
+    lengths = [400, 0, 217, 385, 1, 129, 400, 384]
+    g = torch.Generator(device=cuda)
+    g.manual_seed(35)
+    q, k, v = _packed(cuda, g, dtype, len(lengths), 400, heads, kv, dim)
+    dout = torch.randn(q.shape, generator=g, device=cuda).to(dtype)
+    n = torch.tensor(lengths, dtype=torch.int32, device=cuda)
+    # sum over sequences of tiles of 128 rows that are not empty, times two tiles or heads an item
+    items = sum(-(-x // 128) for x in lengths) * heads // 2
+    assert items > 1.5 * torch.cuda.get_device_properties(cuda).multi_processor_count
+    for window, sinks in ((100, 4), (260, 0)):
+        one = _check(q, k, v, window, sinks, dout, lengths=n)
+        out, lse = ops.window_attention_forward(q, k, v, window, sinks, lengths=n)
+        grads = ops.window_attention_backward(dout, q, k, v, out, lse, window, sinks, lengths=n)
+        for x, name in zip((out, lse, *grads), ("out", "lse", "dq", "dk", "dv")):
+            assert torch.equal(x, one[name]), name
+
+
 CACHE = [
     # b, q_len, kv_len, heads, kv, dim, window, sinks
     (1, 1, 1, 1, 1, 64, 5, 0),
