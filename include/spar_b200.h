@@ -463,11 +463,12 @@ struct SparCudaStatus spar_b200_qk_norm_rotary_backward(const struct SparB200Rot
 /* formula gives or NaN: products are made tile by tile, where a weight of zero times it is NaN,   */
 /* and fp32 on the tensor cores takes every infinity as NaN (elsewhere a score of -infinity gives   */
 /* its key no weight). For the same reason it may make NaN the results of rows within 256           */
-/* positions of one that sees the key, and of keys within 256 positions of one that the row sees,   */
-/* of its sequence and head group; it reaches no others.                                          */
+/* positions of one that sees the key, and of keys within 256 positions of one that such a row       */
+/* sees, of its sequence and head group; it reaches no others.                                      */
 /* Outputs must not overlap inputs or one another (refused where they start at the same element);  */
 /* an output with a stride of zero over more than one index is refused.                          */
-/* bf16: products of bf16 operands (P and dS rounded to nearest) with fp32 sums; fp32: as exact as */
+/* bf16: products of bf16 operands (P and dS rounded to nearest) with fp32 sums, so that a result   */
+/* is off by its own rounding and one more of that size; fp32: as exact as                          */
 /* fp32 products and sums (values below 2^-110 keep fewer bits). 16-byte aligned rows with head_dim */
 /* a multiple of 8, at most 128, run on the tensor cores; up to 16 rows of a head group (heads /   */
 /* kv_heads * q_len), or 64 where the visible keys are eight times as many, run as a decoding step; */

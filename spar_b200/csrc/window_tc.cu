@@ -780,7 +780,7 @@ __global__ void __launch_bounds__(128 + 128 * QT, 1) window_forward_kernel(
 // ============================================================================ backward
 // Two launches of one kernel, after D = rowsum(dout o out):
 //   queries (KEYS = false)  stationary: 128 rows of q and dout; moving: 64 rows of k and v
-//       S = q k^T, dP = dout v^T;  dS = P o (dP - D);  dq += dS k
+//       S = q k^T, dP = dout v^T;  dS = P o (dP - D);  dq += dS k   (bf16: and P k, see Bwd::kCorrect)
 //   keys (KEYS = true)      stationary: 128 rows of k and v; moving: 64 rows of q and dout, for
 //       every query head of the group: S^T = k q^T, dP^T = v dout^T;  dv += P^T dout;  dk += dS^T q
 // P = exp(S - lse) is recomputed on both sides, so every gradient element is summed in one CTA and
@@ -790,9 +790,12 @@ __global__ void __launch_bounds__(128 + 128 * QT, 1) window_forward_kernel(
 // First tokens are seen by every later row: their key tiles' rows are cut into chunks of
 // `chunk` rows that are items of their own (and, where there are few key tiles, so are groups of
 // query heads); such items leave fp32 partial sums that a last launch adds in order.
-// (2 x 4096 tokens of 16/4 heads of 64 bf16, window 512: 139 us with D and the partials; 482 and 513
-// instructions a warp and tile at 5.4 cycles each, two warps a scheduler, are what bounds it. fp32, 16 x
-// 1024 x 16 heads of 64, all keys: 894 us, bound by the six products.)
+// bf16 rounds P and dS to bf16 for their products, as every such product takes bf16 operands: a second
+// rounding of the size of the result's own. (Two planes would cost a product and the packing of each.)
+// (2 x 4096 tokens of 16/4 heads of 64 bf16, window 512: 145 us with D and the partials, 138 without the
+// sums that correct D; 1 x 8192 x 32/8 heads of 128, window 1024: 571, 523. Some 500 instructions a warp
+// and tile at 5.4 cycles each, two warps a scheduler, are what bounds it. fp32, 16 x 1024 x 16 heads of
+// 64, all keys: 870 us, bound by the six products. Calls repeated.)
 constexpr int kMoving = 64;
 
 struct BackwardParams {
@@ -861,7 +864,7 @@ template <bool KEYS, int DH, int NP, int ST, int OUT>
 struct Bwd {
   // Buffers of S and dP: three where TMEM has room, so that the two softmax groups find their next
   // scores ready; not more than stages, as scores run that far ahead of the last use of a stage.
-  static constexpr int kBuffers = NP > 1 ? (ST == 1 ? 1 : 2) : KEYS && DH == 128 ? 2 : 3;
+  static constexpr int kBuffers = NP > 1 ? (ST == 1 ? 1 : 2) : DH == 128 ? 2 : 3;
   static_assert(kBuffers <= ST, "stages");
   static constexpr uint32_t kStats = NP == 1 && DH == 64 ? 2 : 1;  // pairs of stationary operands
   // Stationary rows. Three planes of two operands of 128 columns leave room for 64 of the 128 rows of a
@@ -879,19 +882,28 @@ struct Bwd {
   // on the row side, so that S and dP arrive with them subtracted. (Read from shared memory by every
   // thread they took 620 of 2090 cycles a tile.) fp32: [ST][2][64] -lse log2 e, -D.
   static constexpr bool kAugment = KEYS && NP == 1;
+  // Queries, bf16: D comes from the rounded `out`, so the rows of dS do not add up to zero. What a row
+  // of the unrounded dS' = P o (dP - D') adds up to is D - D': dq = dS' k - (D - D') P k, and the key
+  // side reads the D so corrected. (Without it dq and dk were 1.5 to 1.75 times as far off as their own
+  // rounding, most where few keys are seen; with it sqrt 2, the rounding of dS.)
+  static constexpr bool kCorrect = !KEYS && NP == 1;
   static constexpr uint32_t kOnes = kOut + 8 * 4096;
   static constexpr uint32_t kRows = kOnes + (kAugment ? 4096 : 0);
   static constexpr uint32_t kRowsBytes = kAugment ? 4096 : 512;  // of a stage
-  static constexpr uint32_t kBar = kRows + (KEYS ? ST * kRowsBytes : 0);
+  static constexpr uint32_t kBar = kRows + (KEYS ? ST * kRowsBytes : kCorrect ? 1024 : 0);
   static constexpr uint32_t kSmem = kBar + 320 + 1024;
-  static_assert((21 + 2 * ST) * 8 + 24 <= 320, "backward barriers");
+  static_assert((22 + 2 * ST) * 8 + 24 <= 320, "backward barriers");
   static_assert(kSmem <= kMaxSmem, "backward shared memory");
   // TMEM: buffers of S | dP (| the third planes of P and dS), then the products' sums: of the item, or
   // (NP = 3) of a tile, whose sum over tiles the softmax threads keep.
   static constexpr uint32_t kBuf = KEYS && NP > 1 ? 192 : 128;
   static constexpr uint32_t kAcc = kBuffers * kBuf;
-  static constexpr uint32_t kOuts = KEYS && OUT == 0 ? 2 : 1;
+  static constexpr uint32_t kOuts = (KEYS && OUT == 0) || kCorrect ? 2 : 1;
+  static constexpr uint32_t kResults = KEYS ? kOuts : 1;
   static_assert(kAcc + kOuts * DH <= kTmemCols, "backward TMEM");
+  // Which operands the softmax writes, and whether dS goes over dP (or over S, where P is not needed).
+  static constexpr bool kP = KEYS ? OUT != 1 : kCorrect, kDs = OUT != 2;
+  static constexpr int kDsAt = KEYS || kCorrect ? 1 : 0;
 };
 
 // Column (in a buffer) of plane pl of K step ks of the operand that overwrites S (which = 0) or dP
@@ -934,8 +946,9 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
   uint64_t* m_empty = m_full + ST;
   uint64_t* item_full = m_empty + ST;  // [4]
   uint64_t* item_empty = item_full + 4;
-  volatile int* items = reinterpret_cast<volatile int*>(item_empty + 4);  // [4]
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(item_empty + 4) + 4;
+  uint64_t* row_sums = item_empty + 4;  // both groups' sums of dS are there
+  volatile int* items = reinterpret_cast<volatile int*>(row_sums + 1);  // [4]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(row_sums + 1) + 4;
   const Abort abort_flag = {reinterpret_cast<volatile int*>(tmem_slot + 1), p.wait_flag};
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const WindowParams& w = p.w;
@@ -960,6 +973,7 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
       tc::mbar_init(item_full + i, 1);
       tc::mbar_init(item_empty + i, 1 + 8);  // the issuer, the softmax warps
     }
+    tc::mbar_init(row_sums, 8);
     *abort_flag.cta = 0;
     tc::fence_barrier_init();
   }
@@ -1132,14 +1146,14 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
           if (last) tc::mma_commit(a_empty + an % L::kStats);
           return true;
         };
-        // The products of tile m's P and dS: queries dq += dS k; keys dk += dS^T q, dv += P^T dout.
+        // The products of tile m's P and dS: queries dq += dS k (and P k); keys dk += dS^T q, dv += P^T dout.
         auto products = [&](uint32_t m, bool first, bool last) {
           const uint32_t st = m % ST, buf = tmem + (m % L::kBuffers) * L::kBuf;
           tc::tc_fence_after();
 #pragma unroll
           for (int out = 0; out < static_cast<int>(L::kOuts); ++out) {
-            const int operand = OUT == 2 ? 1 : out, which = KEYS ? 1 - operand : 0;
-            const uint32_t b = mnmajor_low(b_addr + (2 * st + operand) * L::kMov, kMoving);
+            const int operand = OUT == 2 ? 1 : out, which = operand == 0 ? L::kDsAt : 0;
+            const uint32_t b = mnmajor_low(b_addr + (2 * st + (KEYS ? operand : 0)) * L::kMov, kMoving);
             uint32_t acc = NP == 1 && !first;
 #pragma unroll
             for (int pr = 0; pr < kProducts<NP>; ++pr)
@@ -1262,6 +1276,7 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
     const Box box = {smem + L::kOut + (warp - 4) * 4096};
     const uint64_t scale = both(p.scale_log2, p.scale_log2);
     uint32_t mn = 0, sums = 0;
+    [[maybe_unused]] uint32_t corrected = 0;
     bool ok = true;
     // NP = 3: the sums over tiles of this thread's row, the groups share the columns; add_sums adds the
     // last tile's products.
@@ -1300,9 +1315,10 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
                            : KEYS               ? first_pos + 31 < s.n && first_pos >= oldest
                                 : first_pos >= 0 && first_pos + 31 < s.n && row - lane + 31 < w.q_len;
       uint64_t minus_lse = 0, minus_delta = 0;
+      [[maybe_unused]] uint64_t ds_sums[2] = {0, 0};
       if (!KEYS && valid && n) {
         const uint64_t at = (static_cast<uint64_t>(b) * w.heads + q.h[0]) * w.q_len + row;
-        const float lse2 = __ldg(w.lse + at) * kLog2e, delta = __ldg(w.delta + at);
+        const float lse2 = __ldg(w.lse + at) * kLog2e, delta = w.delta[at];
         minus_lse = both(-lse2, -lse2);
         minus_delta = both(-delta, -delta);
       }
@@ -1393,6 +1409,10 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
             pr[e + 1] = both(ex2(t1.x), ex2(t1.y));
             ds[e] = mul2(pr[e], g0);
             ds[e + 1] = mul2(pr[e + 1], g1);
+            if constexpr (L::kCorrect) {
+              ds_sums[0] = add2(ds_sums[0], ds[e]);
+              ds_sums[1] = add2(ds_sums[1], ds[e + 1]);
+            }
           }
           // Operands over the columns just read: plane pl of both K steps is 16 columns.
 #pragma unroll
@@ -1405,17 +1425,17 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
               v = both(t.x, t.y);
               return upper;
             };
-            if constexpr (KEYS && OUT != 1) {
+            if constexpr (L::kP) {
 #pragma unroll
               for (int e = 0; e < 16; ++e) u[e] = pack(pr[e]);
               tc::tmem_store_32x16_async(
                   buf + operand_col<KEYS>(0, pl, 0) + (pl < 2 ? half * 32 : half * 16), u);
             }
-            if constexpr (OUT != 2) {
+            if constexpr (L::kDs) {
 #pragma unroll
               for (int e = 0; e < 16; ++e) u[e] = pack(ds[e]);
               tc::tmem_store_32x16_async(
-                  buf + operand_col<KEYS>(KEYS ? 1 : 0, pl, 0) + (pl < 2 || !KEYS ? half * 32 : half * 16), u);
+                  buf + operand_col<KEYS>(L::kDsAt, pl, 0) + (pl < 2 || !KEYS ? half * 32 : half * 16), u);
             }
           }
         }
@@ -1450,24 +1470,49 @@ __global__ void __launch_bounds__(384, 1) window_backward_kernel(
         tc::tc_fence_after();
         if constexpr (NP > 1) add_sums(n == 1);
       }
+      // D - D' of this row: the two groups' tiles, in the order of the groups.
+      [[maybe_unused]] float correction = 0.f;
+      if constexpr (L::kCorrect) {
+        if (n) {
+          float* shared_sums = reinterpret_cast<float*>(smem + L::kRows);  // [2][128]
+          const float2 t = halves(add2(ds_sums[0], ds_sums[1]));
+          shared_sums[g * 128 + r] = t.x + t.y;
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(row_sums);
+          if (!(ok = wait_or_abort(row_sums, corrected, abort_flag))) break;
+          ++corrected;
+          correction = shared_sums[r] + shared_sums[128 + r];
+          if (g == 0 && valid)
+            w.delta[(static_cast<uint64_t>(b) * w.heads + q.h[0]) * w.q_len + row] =
+                correction - halves(minus_delta).x;
+        }
+      }
       // One result: both groups store half of its columns (bf16 heads of 64: group 0 stores all, as 64
       // columns are one box); both of the key side's: group 0 stores dk, group 1 dv.
       constexpr bool kBoth = KEYS && OUT == 0;
-      constexpr int cols = NP == 1 && L::kOuts * DH == 64 ? 64 : L::kOuts * DH / 2;
+      constexpr int cols = NP == 1 && L::kResults * DH == 64 ? 64 : L::kResults * DH / 2;
       const int out = kBoth ? g : OUT == 2;
       const uint32_t from = lanes + L::kAcc + g * cols;
       const float factor = KEYS && out ? 1.f : w.scale;
       const int warp_row = row - lane;
 #pragma unroll(NP > 1 ? cols / 32 : 1)
       for (int c = 0; c < cols; c += 32) {
-        if (g * cols >= static_cast<int>(L::kOuts) * DH) break;
+        if (g * cols >= static_cast<int>(L::kResults) * DH) break;
         float o[32];
         if constexpr (NP > 1) {
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = n ? tile_sums[c + e] * factor : 0.f;
         } else {
           uint32_t u[32];
-          if (n) tc::tmem_load_32x32(from + c, u);
+          if constexpr (L::kCorrect) {
+            uint32_t pk[32];
+            if (n) tc::tmem_load_2x32(from + c, from + DH + c, u, pk);
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+              u[e] = __float_as_uint(fmaf(-correction, __uint_as_float(pk[e]), __uint_as_float(u[e])));
+          } else {
+            if (n) tc::tmem_load_32x32(from + c, u);
+          }
 #pragma unroll
           for (int e = 0; e < 32; ++e) o[e] = n ? __uint_as_float(u[e]) * factor : 0.f;
         }
