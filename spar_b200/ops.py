@@ -504,6 +504,8 @@ def qk_norm_rotary_backward(dq_out, dk_out, q, k, q_weight, k_weight, table, eps
                         None if k is None else _heads_view(dk_out, "dk_out", q, k.shape), dq_weight,
                         dk_weight, int(accumulate_params), scratch.data_ptr())
     call("spar_b200_qk_norm_rotary_backward", desc, _dev(q), _stream(q))
+    if k is not None and k.shape[2] == 0 and not accumulate_params:
+        dk_weight.zero_()  # the library has no k without heads: it leaves this alone
     return dq, dk, dq_weight, dk_weight
 
 

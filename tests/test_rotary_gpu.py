@@ -249,6 +249,21 @@ def test_no_tokens(cuda):
     assert ops.rotary_table(0, 64, device=cuda).shape == (0, 32, 2)
 
 
+def test_keys_without_heads(cuda):
+    from spar_b200 import ops
+
+    q, k = torch.ones(2, 3, 4, 64, device=cuda), torch.ones(2, 3, 0, 64, device=cuda)
+    table, w = torch.ones(3, 32, 2, device=cuda), torch.ones(64, device=cuda)
+    held = torch.full((64,), 7.0, device=cuda)
+    dq, dk, dwq, dwk = ops.qk_norm_rotary_backward(q, k, q, k, w, w, table, dk_weight=held)
+    alone = ops.qk_norm_rotary_backward(q, None, q, None, w, None, table)
+    assert torch.equal(dq, alone[0]) and torch.equal(dwq, alone[2])
+    assert dk.shape == k.shape and dwk is held and not held.any()
+    held.fill_(7.0)
+    ops.qk_norm_rotary_backward(q, k, q, k, w, w, table, dq_weight=w.clone(), dk_weight=held, accumulate_params=True)
+    assert bool((held == 7.0).all())
+
+
 @pytest.mark.parametrize("kind", ["none", "linear", "base", "parts"])
 @pytest.mark.parametrize("rows,rotary,start", [(1, 4, 0), (33, 64, 0), (500, 96, 7), (70, 128, 1 << 20)])
 def test_rotary_table(cuda, rows, rotary, start, kind):
