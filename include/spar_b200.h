@@ -367,7 +367,9 @@ enum SparB200Element {
 /*   PARTS   g f_i + (1 - g) f_i / factor, g = clamp((r_i - slow_turns) / (fast_turns -          */
 /*           slow_turns), 0, 1), r_i = original_length f_i / (2 pi) the turns pair i makes over  */
 /*           the trained context; cos and sin times `magnitude` (interpolation by parts, Peng    */
-/*           et al. 2023)                                                                        */
+/*           et al. 2023, whose ramp over the number of turns this is; a model trained with a    */
+/*           ramp over the pair's index between two rounded bounds needs a table of its own:     */
+/*           any [rows, rotary_dim / 2] (cos, sin) is taken)                                      */
 enum SparB200RotaryScalingKind {
   SPAR_B200_ROTARY_NONE = 0,
   SPAR_B200_ROTARY_LINEAR = 1,
@@ -489,7 +491,10 @@ struct SparB200WindowAttention {
   struct SparB200Heads dout, dq, dk, dv;
   void* scratch; /* spar_b200_window_attention_scratch_bytes bytes, 256-byte aligned */
 };
-/* Scratch bytes of the forward (backward = 0) or backward (1) of this call on `device`.         */
+/* Scratch bytes of the forward (backward = 0) or backward (1) of this call on `device`. fp32 on   */
+/* the tensor cores takes 6 bytes for every element of q, k and v (backward: and dout), of the     */
+/* whole kv_len whatever the lengths and the window let a row see: 65 rows or more against a cache */
+/* of 131072 keys x 8 heads x 128 take 1.6 GB a sequence, and the time to write them.              */
 uint64_t spar_b200_window_attention_scratch_bytes(const struct SparB200WindowAttention* w,
                                                   int backward, int device);
 struct SparCudaStatus spar_b200_window_attention_forward(const struct SparB200WindowAttention* w,

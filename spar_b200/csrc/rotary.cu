@@ -490,8 +490,9 @@ __global__ void __launch_bounds__(1024) qk_weight_partials_kernel(float* dq, flo
 // One thread per (pair, run of positions): the first angle's cos and sin, then rotations by one
 // position in double (each adds ~2^-52, far below the fp32 result's 2^-25): four double operations
 // per entry instead of ~100. The run is as long as leaves 32768 threads, 8 to 128 positions: 131072
-// positions of 64 pairs take 16 us of which the stores' floor is 10 (runs of 128 left a shorter
-// table's few threads with the latency of 128 steps: 4096 positions 21 us, in runs of 8 9 us).
+// positions of 64 pairs take 12.2 us from a graph, of which the stores' floor is 10.2, and 17 as a call with
+// a flushed L2: a chain of 128 steps on 256 blocks of 148 SMs. (Runs of 128 left a shorter table's few
+// threads with the latency of 128 steps: 4096 positions 21 us a call, in runs of 8 9 us.)
 __global__ void __launch_bounds__(256) rotary_table_kernel(float2* table, uint64_t rows,
                                                            uint32_t pairs, uint64_t start, uint32_t length,
                                                            SparB200RotaryScaling sc, double theta) {
@@ -533,8 +534,8 @@ View view_of(const SparB200Heads& v, uint64_t batch, uint64_t seq, uint64_t head
           heads > 1 ? v.head : 0};
 }
 
-// More blocks than run at once, so that their ends do not fall together (2 x 4095 tokens of 40 heads of
-// 128 bf16: 4 an SM 76.5 us, 16 an SM 72.2 us).
+// More blocks than run at once (four or five an SM), so that their ends do not fall together (2 x 4095
+// tokens of 40 heads of 128 bf16, calls repeated: 4 an SM 76.5 us, 16 an SM 72.2 us).
 constexpr int kBackwardBlocksPerSM = 16;
 
 uint32_t backward_blocks(int device) {

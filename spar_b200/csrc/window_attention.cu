@@ -23,7 +23,7 @@ namespace {
 // keys with a running maximum and sum. Reads elements one by one, so it takes every head_dim,
 // stride and alignment; it is the path of the rows that the tiled kernels cannot address. Bound by
 // its instructions (five shuffles a dot product): 2 x 1023 x 8/4 heads of 100 bf16, window 256, 500 us
-// forward and 1620 us backward, where the tiled kernels take 15 and 45 us for heads of 96.
+// forward and 1620 us backward, where the tiled kernels take 15 and 48 us for heads of 96.
 constexpr int kRowWarps = 4;
 
 template <typename T, int E>

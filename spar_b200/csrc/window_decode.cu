@@ -2,11 +2,11 @@
 // the top of window_attention.cu.
 //
 // The floor is one read of the visible keys and values, which all query heads of a key head share:
-// a CTA takes up to 8 or 16 rows (heads of one group, times tokens) and a range of the visible keys,
-// so that a cache row is loaded once for all of them: by cp.async, two steps ahead (one step ahead
+// a CTA takes up to 8 (fp32) or 16 (bf16) rows (heads of one group, times tokens) and a range of the
+// visible keys, so that a cache row is loaded once for that many: by cp.async, two steps ahead (one step ahead
 // in registers every step waited for memory: 4 TB/s), each lane into slots of shared memory that it
 // alone reads, so nothing but its own copies is waited for. (32 caches, 4096 visible keys, 32/8 heads of
-// 128 bf16: 114 us, 4.7 TB/s of the 6.55 of a copy.) Each warp (or lane group) keeps its own running
+// 128 bf16: 115 us with a flushed L2, 4.7 TB/s of the 6.55 of a copy.) Each warp (or lane group) keeps its own running
 // maximum, sum and output; they are joined in shared memory, and the ranges of one row over the shared
 // memory of a cluster of up to eight CTAs, or, where it takes more to fill the machine, by a second
 // launch. Both add in a fixed order.
@@ -670,7 +670,9 @@ bool decode_supported(const WindowParams& w) {
   // tiled path's few items do not (64 rows of 1024 keys, 8 x 4 heads of 64 bf16: 21 against 27 us; 40
   // rows of 4096 keys, 8 heads of 128 fp32: 93 against 309 us, as the tiled path splits the whole cache
   // into planes). Short caches are better tiled (64 rows of 64 keys, 32 x 32 heads of 128 bf16: 30
-  // against 213 us).
+  // against 213 us). Rule and plan go by the cache's capacity, since the lengths are on the device: ranges
+  // planned for 16384 keys of which 512 are used, 32/8 heads of 128 bf16, cost one cache 10.2 against 6.6
+  // us, four 10.8 against 7.8, and 32, which fill the machine, nothing.
   const int64_t keys = std::min<int64_t>(w.kv_len, static_cast<int64_t>(w.window) + w.q_len + w.sinks);
   return rows > 0 && (rows <= 16 || (rows <= 64 && keys >= 8 * rows)) && w.head_dim % vec == 0 &&
          w.head_dim / vec <= 32 && w.kv_len > 0 &&

@@ -16,9 +16,10 @@
 // exponentiated the other tile's products run. The keys of an item are its first tokens' tiles,
 // then tiles that start exactly at the first key of the window, so a window of W keys under a tile
 // of 128 rows costs ceil((W + 127) / BN) tiles. Every wait is bounded and leaves an error flag.
-// bf16, 8192 tokens of 32/8 heads of 128, window 1024: 156 us, 830 TFLOP/s; a pair of 128 x 128 tiles
-// takes 1940 cycles where its products take 1024: the exponentials and packing of two softmax warps a
-// scheduler bound it (sixteen warps, half the columns each: 270 us).
+// bf16, 8192 tokens of 32/8 heads of 128, window 1024: 157 us, 825 TFLOP/s, where calls are repeated, and
+// 181 us with other inputs every call and a flushed L2. One 128 x 128 tile (scores and P V) takes about
+// 2000 cycles of an SM where its products take 1024 (tensor pipe active 50 %): the exponentials and
+// packing of two softmax warps a scheduler bound it (sixteen warps, half the columns each: 270 us).
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -169,7 +170,7 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 }
 
 // 2^x of two values on the FMA pipe (Cody and Waite): x = n + f with n the nearest integer, the
-// polynomial 2^f ~ c0 + .. + c4 f^4 on [-1/2, 1/2] (minimax in relative error, 2.6e-6, fitted for
+// polynomial 2^f ~ c0 + .. + c4 f^4 on [-1/2, 1/2] (minimax in relative error, 2.7e-6, fitted for
 // this file), n added to the exponent. x is cut at -126. The special-function unit makes 16 values
 // per cycle and SM, less than the score tiles need; a share of them goes this way.
 __device__ __forceinline__ uint64_t ex2_poly(uint64_t x) {
@@ -188,7 +189,9 @@ __device__ __forceinline__ uint64_t ex2_poly(uint64_t x) {
 }
 
 // P = 2^(s scale - m) of 32 scores as 16 columns of bf16 pairs, rounded to nearest, and the sums of
-// the unrounded values; the last kPoly of every 8 on the FMA pipe.
+// the unrounded values; the last kPoly of every 8 on the FMA pipe. (P in 8 bits is a choice: the product
+// takes operands of one type, and a second plane would double P V and its packing. It leaves out 1.15 to
+// 1.3 times as far off as its own rounding. A row's sum and lse have all bits but the polynomial's.)
 template <int kPoly>
 __device__ __forceinline__ void weights32(const uint32_t (&s)[32], uint64_t scale, uint64_t minus_m,
                                           uint64_t (&sums)[2], uint32_t (&u)[16]) {

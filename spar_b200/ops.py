@@ -388,7 +388,9 @@ class RotaryScaling:
     """How rotary_table scales angles for contexts longer than `original_length`: "linear"
     (position interpolation), "base" (a larger theta) or "parts" (interpolation by parts: pairs of
     more than fast_turns turns over the original length kept, of less than slow_turns divided by
-    `factor`). `magnitude` multiplies cos and sin; None: 0.1 ln(factor) + 1 for "parts", else 1."""
+    `factor`, between them linear in the number of turns; a ramp over the pair's index between
+    rounded bounds is another table, which the caller makes). `magnitude` multiplies cos and sin;
+    None: 0.1 ln(factor) + 1 for "parts", else 1."""
     kind: str
     factor: float
     original_length: float = 0.0
